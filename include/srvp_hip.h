@@ -560,6 +560,79 @@ int srvp_frame_metrics(const float* x, const float* y, int64_t planes, int H, in
 int srvp_skip_grad_reduce(const void* dcat, int cstride, int coff, int C, int HW, int T, int B, void* dsel, void* stream);
 int srvp_skip_grad_reduce_f32(const void* dcat, int cstride, int coff, int C, int HW, int T, int B, void* dsel, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Temporal operators: the parallel counterpart of the posterior LSTM (module/srvp.py:130,366).  Tensors are time-major (T, B, H, D) with any strides
+ * (elements) over t, b, h and contiguous features; elem_f32 = 1: float32, 0: bfloat16.  lengths (int64 [B], may be NULL): tokens of each sequence;
+ * outputs and gradients behind them are zero.  States and carries are float32 [.][H][Dk][Dv], contiguous.
+ * ------------------------------------------------------------------------------------------------ */
+/* S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t.  state_in / state_out may be NULL (zero / not wanted); they may not overlap.
+ * ws: srvp_linear_attention_ws_bytes(desc, 0) bytes (16-byte aligned; may be 0). */
+typedef struct {
+    const void *q, *k, *v; void* o;
+    int64_t qs[3], ks[3], vs[3], os[3];
+    const float* log_decay; const float* state_in; float* state_out; const int64_t* lengths;
+    void* ws; int64_t ws_bytes;
+    int32_t T, B, H, Dk, Dv; float scale; int32_t elem_f32, reserved;
+} srvp_linear_attention_desc;
+/* gradients of the above for d_o and d_state_out (may be NULL); d_state_in may be NULL.  f.o and f.state_out are not read; f.ws:
+ * srvp_linear_attention_ws_bytes(&desc->f, 1) bytes. */
+typedef struct {
+    srvp_linear_attention_desc f;
+    const void* d_o; void *dq, *dk, *dv;
+    int64_t d_os[3], dqs[3], dks[3], dvs[3];
+    const float* d_state_out; float* d_state_in;
+} srvp_linear_attention_bwd_desc;
+/* one token for each of B rows: q, k, v, o (B, H, D) with strides over b, h; state float32 [nslots][H][Dk][Dv], updated in place; slots (int64 [B],
+ * may be NULL: row b has state b).  A slot outside [0, nslots) marks a padded row (output zero, no state touched); rows that name the same slot are
+ * successive tokens of one sequence, in row order. */
+typedef struct {
+    const void *q, *k, *v; void* o;
+    int64_t qs[2], ks[2], vs[2], os[2];
+    const float* log_decay; float* state; const int64_t* slots;
+    int32_t B, H, Dk, Dv, nslots; float scale; int32_t elem_f32, reserved;
+} srvp_linear_attention_step_desc;
+int64_t srvp_linear_attention_ws_bytes(const srvp_linear_attention_desc* d, int32_t backward);
+int srvp_linear_attention_fwd(const srvp_linear_attention_desc* d, void* stream);
+int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* d, void* stream);
+int srvp_linear_attention_step(const srvp_linear_attention_step_desc* d, void* stream);
+/* Rotary positions of q (T, B, Hq, D) and k (T, B, Hk, D; Hk = 0: none): pair p of every head -- features (2p, 2p + 1) if interleaved, (p, pairs + p)
+ * otherwise -- is turned by positions[t][b] * freq[p] radians (back = 1: by the negative angle) and multiplied by `magnitude`; features from 2 * pairs on
+ * are copied.  positions int64 with strides pos_t, pos_b; freq float64 [pairs]. */
+typedef struct {
+    const void *q, *k; void *oq, *ok;
+    int64_t qs[3], ks[3], oqs[3], oks[3];
+    const int64_t* positions; int64_t pos_t, pos_b; const double* freq;
+    int32_t T, B, Hq, Hk, D, pairs, interleaved, back; float magnitude; int32_t elem_f32;
+} srvp_rotary_desc;
+int srvp_rotary(const srvp_rotary_desc* d, void* stream);
+/* h = x + residual (NULL: h = x); y = h * w / sqrt(mean(h^2) + eps) over rows of N features; sum (may be NULL) = h.
+ * q8 != NULL: instead of y, int8 rows and float32 scale [M] with y ~ q8 * scale: scale = max|y| / 127, q8 = round-half-even(h w * (127 / max|h w|)) in 64 bits;
+ * w == NULL then quantises h itself.  A row of zeros has scale 0, a row with an infinity or NaN scale NaN.  xs .. qs: row strides. */
+typedef struct {
+    const void *x, *residual; const float* w; void *y, *sum, *q8; float* scale;
+    int64_t xs, rs, ys, ss, qs, M;
+    int32_t N; float eps; int32_t elem_f32, reserved;
+} srvp_rms_norm_desc;
+int srvp_rms_norm(const srvp_rms_norm_desc* d, void* stream);
+/* dx (the gradient of x and of residual) = rstd (d_y w - n mean(d_y w n)) + d_sum with n = h * rstd, h = x + residual (not rounded),
+ * rstd = 1 / sqrt(mean(h^2) + eps); dw float32 [N].  residual, d_sum may be NULL.
+ * ws: srvp_rms_norm_bwd_ws_bytes(M, N, elem_f32) bytes. */
+typedef struct {
+    const void *x, *residual, *d_y, *d_sum; const float* w; void* dx; float* dw; void* ws;
+    int64_t xs, rs, dys, dss, dxs, M, ws_bytes;
+    int32_t N; float eps; int32_t elem_f32, reserved;
+} srvp_rms_norm_bwd_desc;
+int64_t srvp_rms_norm_bwd_ws_bytes(int64_t M, int32_t N, int32_t elem_f32);
+int srvp_rms_norm_bwd(const srvp_rms_norm_bwd_desc* d, void* stream);
+/* y[m][n] = (sum_k x[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n]; x, w int8 with row strides ldx, ldw >= K (any alignment), sums exact in int32
+ * (K <= 131071); y float32 or bfloat16 with row stride ldy; bias may be NULL. */
+typedef struct {
+    const void *x, *w; const float *x_scale, *w_scale, *bias; void* y;
+    int64_t ldx, ldw, ldy;
+    int32_t M, N, K, out_f32;
+} srvp_linear_int8_desc;
+int srvp_linear_int8(const srvp_linear_int8_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

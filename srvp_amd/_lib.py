@@ -183,6 +183,16 @@ _SIGS = {
     'srvp_pad_f32': ([c_vp, c_vp, c_i64, c_i32, c_i32, c_vp], c_i32),
     'srvp_skip_grad_reduce_f32': ([c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp], c_i32),
     'srvp_frame_metrics': ([c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_f32, c_f32, c_f32, c_vp, c_vp, c_vp], c_i32),
+    # (descriptors of the temporal operators: packed bytes, srvp_amd/temporal.py)
+    'srvp_linear_attention_ws_bytes': ([C.c_char_p, c_i32], c_i64),
+    'srvp_linear_attention_fwd': ([C.c_char_p, c_vp], c_i32),
+    'srvp_linear_attention_bwd': ([C.c_char_p, c_vp], c_i32),
+    'srvp_linear_attention_step': ([C.c_char_p, c_vp], c_i32),
+    'srvp_rotary': ([C.c_char_p, c_vp], c_i32),
+    'srvp_rms_norm': ([C.c_char_p, c_vp], c_i32),
+    'srvp_rms_norm_bwd_ws_bytes': ([c_i64, c_i32, c_i32], c_i64),
+    'srvp_rms_norm_bwd': ([C.c_char_p, c_vp], c_i32),
+    'srvp_linear_int8': ([C.c_char_p, c_vp], c_i32),
     'srvp_skip_grad_reduce': ([c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp], c_i32),
 }
 

@@ -1,0 +1,697 @@
+// Linear attention with a decay for each head, over time-major tensors (T, B, H, D):
+//
+//     S_t = a_h S_{t-1} + k_t v_t^T          (Dk x Dv, fp32)          o_t = scale * q_t S_t
+//
+// Chunked form.  Within a chunk of C tokens (index i, decay a, state S in front of it)
+//
+//     o_i = scale * ( sum_{j <= i} a^(i-j) (q_i . k_j) v_j  +  a^(i+1) q_i S ),        S' = a^C S + sum_j a^(C-1-j) k_j v_j^T
+//
+// so a chunk is four matrix products on the matrix cores and the recurrence advances once a chunk.  The gradients are the same sum with its
+// operands exchanged and, for two of them, time reversed:
+//
+//     dq_i = scale * sum_{j <= i} a^(i-j) (do_i . v_j) k_j  +  scale a^(i+1) do_i S_0^T
+//     dv_j = scale * sum_{i >= j} a^(i-j) (k_j . q_i) do_i  +  a^(n-1-j) k_j dS_n          dk_j: (v, do, q) and dS_n^T
+//     dS_0 = scale * sum_i a^(i+1) q_i do_i^T + a^n dS_n
+//
+// One kernel (scan_kernel) therefore serves forward and backward: a "role" names its operands a, b, c, the output, the direction and where the
+// carried state comes from and goes to.  In reversed time the carry is taken after its decay (X_t = a R_t), which moves the two exponents by one
+// (`e` below) and leaves no division by a.  No power of a is ever formed with a negative exponent: a = 0 (log_decay = -inf) is an ordinary value.
+#include "common.h"
+#include "../../include/srvp_hip.h"
+
+namespace {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+
+struct Operand {
+    const void* p;
+    long long st, sb, sh;      // elements between tokens, sequences, heads
+    int d;                     // features
+    int vec;                   // 16-byte loads allowed
+};
+
+struct Role {
+    Operand a, b, c;
+    void* o;
+    long long ot, ob, oh;
+    int ovec;
+    int rev;                   // time runs backwards
+    const float* init;         // carry in front of the first token [b][h][...], or null
+    const float* prefix;       // carry in front of every segment [b][h][seg][...], or null (one segment)
+    float* fin;                // carry behind the last token, or null
+    int init_a, init_c;        // strides of all three (elements of a, of c)
+    float init_mul, fin_mul;
+};
+
+struct ScanArgs {
+    Role r[3];
+    int nroles;
+    const float* log_decay;
+    const long long* lengths;
+    int T, B, H, nseg, seg_len, ncb;
+    float scale;
+    float* part;               // state-only launch: segment sums [role][b][h][seg][da][dc]
+};
+
+__device__ __forceinline__ float dpow(float l2, int n) { return n <= 0 ? 1.f : exp2f(l2 * (float)n); }      // decay^n, n >= 0 (0^0 = 1)
+
+// ---- the two element types.  KS = contraction elements of one step; a fragment holds, for lane (g = lane >> 4, s = lane & 15), the KS/4 elements
+// whose index in the step is 4g .. 4g+3 (and 16 + 4g .. for bf16) of row / column s.  That order is the one in which a 16x16 accumulator tile holds its
+// rows, so a product's result is the next product's operand without leaving the registers.
+template <class E> struct Ty;
+template <> struct Ty<bf16_t> {
+    static constexpr int KS = 32, TPK = 2, C = 64, VE = 8, PAD = 8;
+    typedef s16x8_t frag;
+    static __device__ __forceinline__ frag rows(const bf16_t* t, int ld, int row, int k, int lane) {
+        const bf16_t* p = t + (row + (lane & 15)) * ld + k + (lane >> 4) * 4;
+        const s16x4_t lo = *reinterpret_cast<const s16x4_t*>(p), hi = *reinterpret_cast<const s16x4_t*>(p + 16);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    // ds_read_b64_tr_b16: lane s of a 16-lane group receives column s of the 4 x 16 block whose row j the lanes 4j .. 4j+3 address
+    static __device__ __forceinline__ frag cols(const bf16_t* t, int ld, int row, int col, int lane) {
+        typedef __attribute__((address_space(3))) s16x4_t lds_t;
+        const bf16_t* p = t + (row + (lane >> 4) * 4 + ((lane & 15) >> 2)) * ld + col + (lane & 3) * 4;
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p);
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + 16 * ld));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ frag pack(const f32x4_t* t) {
+        u32x4_t v;
+        v.x = pack2bf(t[0][0], t[0][1]); v.y = pack2bf(t[0][2], t[0][3]);
+        v.z = pack2bf(t[1][0], t[1][1]); v.w = pack2bf(t[1][2], t[1][3]);
+        return __builtin_bit_cast(frag, v);
+    }
+    static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, const f32x4_t& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
+    }
+    static constexpr int SPLIT = 3;
+    // x * w as a sum of three bf16 values (8 significant bits each: the fp32 product to its last bit)
+    static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) {
+        float f[8];
+        unpack8(__builtin_bit_cast(u32x4_t, x), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= w[i];
+#pragma unroll
+        for (int s = 0; s < SPLIT; ++s) {
+            const u32x4_t v = pack8(f);
+            out[s] = __builtin_bit_cast(frag, v);
+            float h[8];
+            unpack8(v, h);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] -= h[i];
+        }
+    }
+};
+template <> struct Ty<float> {
+    static constexpr int KS = 16, TPK = 1, C = 32, VE = 4, PAD = 4;
+    typedef f32x4_t frag;
+    static __device__ __forceinline__ frag rows(const float* t, int ld, int row, int k, int lane) {
+        return *reinterpret_cast<const f32x4_t*>(t + (row + (lane & 15)) * ld + k + (lane >> 4) * 4);
+    }
+    static __device__ __forceinline__ frag cols(const float* t, int ld, int row, int col, int lane) {
+        const float* p = t + (row + (lane >> 4) * 4) * ld + col + (lane & 15);
+        return frag{p[0], p[ld], p[2 * ld], p[3 * ld]};
+    }
+    static __device__ __forceinline__ frag pack(const f32x4_t* t) { return t[0]; }
+    static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, f32x4_t c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+        return c;
+    }
+    static constexpr int SPLIT = 1;
+    static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) { out[0] = frag{x[0] * w[0], x[1] * w[1], x[2] * w[2], x[3] * w[3]}; }
+};
+
+// ---- global -> registers -> LDS: C rows x W columns of one operand, zero outside the chunk's tokens and the operand's features.  Row i of the tile is
+// token c0 + i, or c0 + mm - 1 - i in reversed time: everything behind the loader sees time running forwards.
+template <class E, int W> struct Tile {
+    static constexpr int C = Ty<E>::C, VE = Ty<E>::VE, NV = C * W / VE / 256, LD = W + Ty<E>::PAD;
+    u32x4_t v[NV];
+    __device__ __forceinline__ void load(const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = i * 256 + tid, row = idx / (W / VE), col = (idx % (W / VE)) * VE;
+            u32x4_t x = {0, 0, 0, 0};
+            if (row < mm) {
+                const E* p = base + (long long)(c0 + (rev ? mm - 1 - row : row)) * s.st + col0 + col;
+                const int left = s.d - col0 - col;
+                if (s.vec) {
+                    if (left > 0) x = *reinterpret_cast<const u32x4_t*>(p);
+                } else {
+                    E e[VE];
+#pragma unroll
+                    for (int j = 0; j < VE; ++j) e[j] = j < left ? p[j] : E(0);
+                    __builtin_memcpy(&x, e, 16);
+                }
+            }
+            v[i] = x;
+        }
+    }
+    __device__ __forceinline__ void store(E* lds, int tid) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int idx = i * 256 + tid, row = idx / (W / VE), col = (idx % (W / VE)) * VE;
+            *reinterpret_cast<u32x4_t*>(lds + row * LD + col) = v[i];
+        }
+    }
+};
+
+__device__ __forceinline__ void put(bf16_t* p, float v) { *p = f2bf(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put4(bf16_t* p, const f32x4_t& v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3])); }
+__device__ __forceinline__ void put4(float* p, const f32x4_t& v) { *reinterpret_cast<f32x4_t*>(p) = v; }
+
+// One workgroup (4 waves) walks one segment of one (sequence, head) in scan order; wave w owns 16 * NCT columns of c, hence of the state (registers,
+// fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel).
+template <class E, int DA, int NCT, bool OUT>
+__global__ __launch_bounds__(256) void scan_kernel(const ScanArgs g) {
+    using Y = Ty<E>;
+    typedef typename Y::frag frag;
+    constexpr int C = Y::C, KS = Y::KS, TPK = Y::TPK, CB = 64 * NCT, ND = DA / KS, NJ = C / KS, NTA = DA / 16;
+    using TA = Tile<E, DA>;
+    using TC = Tile<E, CB>;
+    __shared__ __align__(16) E lds[(OUT ? C * TA::LD : 0) + C * TA::LD + C * TC::LD];
+    E* lb = lds;
+    E* lc = lb + C * TA::LD;
+    E* la = lc + C * TC::LD;
+
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, lg = lane >> 4, ls = lane & 15;
+    int id = blockIdx.x;
+    const int cb = id % g.ncb; id /= g.ncb;
+    const int h = id % g.H; id /= g.H;
+    const int seg = id % g.nseg; id /= g.nseg;
+    const int b = id % g.B, ro = id / g.B;
+    const Role& r = g.r[ro];
+    const long long bh = (long long)b * g.H + h;
+    const int da = r.a.d, dc = r.c.d, col0 = cb * CB, e = r.rev ? 0 : 1;
+    const float l2 = (float)((double)g.log_decay[h] * 1.4426950408889634);
+
+    int n = g.T;
+    if (g.lengths) { const long long x = g.lengths[b]; n = x < 0 ? 0 : x < g.T ? (int)x : g.T; }
+    const int t0 = seg * g.seg_len, te = min(t0 + g.seg_len, g.T), t1 = min(te, n);
+    const int m = max(0, t1 - t0), nch = (m + C - 1) / C;
+
+    const E* pa = (const E*)r.a.p + b * r.a.sb + h * r.a.sh;
+    const E* pb = (const E*)r.b.p + b * r.b.sb + h * r.b.sh;
+    const E* pc = (const E*)r.c.p + b * r.c.sb + h * r.c.sh;
+    E* po = (E*)r.o + b * r.ob + h * r.oh;
+
+    if (OUT) {
+        // rows behind the sequence's last token: zero
+        const int cw = min(CB, dc - col0);
+        for (int t = max(t0, n); t < te; ++t)
+            for (int c = tid; c < cw; c += 256) put(po + t * r.ot + col0 + c, 0.f);
+    }
+
+    // state: tile (ta, ct) holds rows 16 ta + 4 lg + {0..3}, column ccol + 16 ct
+    const int ccol = col0 + w * 16 * NCT + ls;
+    f32x4_t S[NTA][NCT];
+    {
+        const float* src = nullptr;
+        float mul = 1.f;
+        if (OUT) {
+            if (r.prefix) src = r.prefix + (bh * g.nseg + seg) * (long long)da * dc;
+            else if (r.init) { src = r.init + bh * (long long)da * dc; mul = r.init_mul; }
+        }
+#pragma unroll
+        for (int ta = 0; ta < NTA; ++ta)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int a = ta * 16 + lg * 4 + i, c = ccol + ct * 16;
+                    S[ta][ct][i] = (src && a < da && c < dc) ? mul * src[(long long)a * r.init_a + (long long)c * r.init_c] : 0.f;
+                }
+    }
+
+    TA ra, rb;
+    TC rc;
+    auto fetch = [&](int cc) {
+        const int ch = r.rev ? nch - 1 - cc : cc, c0 = t0 + ch * C, mm = min(C, t1 - c0);
+        if (OUT) ra.load(r.a, pa, c0, mm, r.rev, 0, tid);
+        rb.load(r.b, pb, c0, mm, r.rev, 0, tid);
+        rc.load(r.c, pc, c0, mm, r.rev, col0, tid);
+    };
+    if (nch > 0) fetch(0);
+    for (int cc = 0; cc < nch; ++cc) {
+        const int ch = r.rev ? nch - 1 - cc : cc, c0 = t0 + ch * C, mm = min(C, t1 - c0);
+        __syncthreads();                                  // (the previous chunk's tiles have been read)
+        if (OUT) ra.store(la, tid);
+        rb.store(lb, tid);
+        rc.store(lc, tid);
+        __syncthreads();
+        if (cc + 1 < nch) fetch(cc + 1);                  // in flight under this chunk's products
+
+        frag vf[NJ][NCT];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = Y::cols(lc, TC::LD, j * KS, (w * NCT + ct) * 16, lane);
+
+        if (OUT) {
+            frag sf[ND][NCT];
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int ct = 0; ct < NCT; ++ct) {
+                    f32x4_t t[TPK];
+#pragma unroll
+                    for (int x = 0; x < TPK; ++x) t[x] = S[d * TPK + x][ct];
+                    sf[d][ct] = Y::pack(t);               // bf16: the state is rounded once for the product with q (it is kept in fp32)
+                }
+            float near[4], next[4];                       // a^(i-j) inside a diagonal tile (0 above it); a^(16 + i - j) for the tile below
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int gap = ls - lg * 4 - x;
+                near[x] = gap >= 0 ? dpow(l2, gap) : 0.f;
+                next[x] = dpow(l2, 16 + gap);
+            }
+#pragma unroll
+            for (int ti = 0; ti < C / 16; ++ti) {
+                if (ti * 16 < mm) {
+                    frag af[ND];
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) af[d] = Y::rows(la, TA::LD, ti * 16, d * KS, lane);
+                    // output^T tiles: rows = columns of c (4 lg + ..), column = token ti * 16 + ls
+                    f32x4_t acc[NCT];
+#pragma unroll
+                    for (int ct = 0; ct < NCT; ++ct) {
+                        acc[ct] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) acc[ct] = Y::mfma(sf[d][ct], af[d], acc[ct]);
+                        acc[ct] *= dpow(l2, ti * 16 + ls + e);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if (j * KS <= ti * 16 + 15) {
+                            f32x4_t P[TPK];
+#pragma unroll
+                            for (int x = 0; x < TPK; ++x) {
+                                const int tj = j * TPK + x;
+                                P[x] = f32x4_t{0, 0, 0, 0};
+                                if (tj <= ti) {
+#pragma unroll
+                                    for (int d = 0; d < ND; ++d) P[x] = Y::mfma(Y::rows(lb, TA::LD, tj * 16, d * KS, lane), af[d], P[x]);
+                                    const float back = dpow(l2, 16 * (ti - tj - 1));
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) P[x][i] = tj == ti ? (ls >= lg * 4 + i ? P[x][i] * near[i] : 0.f) : P[x][i] * (next[i] * back);
+                                }
+                            }
+                            const frag pf = Y::pack(P);   // bf16: the scores are rounded once, like the state above
+#pragma unroll
+                            for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf, acc[ct]);
+                        }
+                    }
+                    const int i = ti * 16 + ls;
+                    if (i < mm) {
+                        E* q = po + (long long)(c0 + (r.rev ? mm - 1 - i : i)) * r.ot;
+#pragma unroll
+                        for (int ct = 0; ct < NCT; ++ct) {
+                            const int c = col0 + (w * NCT + ct) * 16 + lg * 4;
+                            acc[ct] *= g.scale;
+                            if (r.ovec) {
+                                if (c < dc) put4(q + c, acc[ct]);
+                            } else {
+#pragma unroll
+                                for (int x = 0; x < 4; ++x)
+                                    if (c + x < dc) put(q + c + x, acc[ct][x]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        // state update
+        const float all = dpow(l2, mm);
+#pragma unroll
+        for (int ta = 0; ta < NTA; ++ta)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) S[ta][ct] *= all;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if (j * KS < mm) {
+                float wt[KS / 4];
+#pragma unroll
+                for (int x = 0; x < KS / 4; ++x) wt[x] = dpow(l2, mm - e - (j * KS + (x >> 2) * 16 + lg * 4 + (x & 3)));
+                frag wv[NCT][Y::SPLIT];
+#pragma unroll
+                for (int ct = 0; ct < NCT; ++ct) Y::weigh(vf[j][ct], wt, wv[ct]);
+#pragma unroll
+                for (int ta = 0; ta < NTA; ++ta) {
+                    const frag kf = Y::cols(lb, TA::LD, j * KS, ta * 16, lane);
+#pragma unroll
+                    for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                        for (int s = 0; s < Y::SPLIT; ++s) S[ta][ct] = Y::mfma(kf, wv[ct][s], S[ta][ct]);
+                }
+            }
+        }
+    }
+
+    float* dst = nullptr;
+    float mul = 1.f;
+    if (!OUT) {
+        dst = g.part + (((long long)ro * g.B * g.H + bh) * g.nseg + seg) * (long long)da * dc;
+    } else if (r.fin) {
+        const int last = r.rev ? 0 : n > 0 ? (n - 1) / g.seg_len : 0;
+        if (seg == last) { dst = r.fin + bh * (long long)da * dc; mul = r.fin_mul; }
+    }
+    if (dst) {
+#pragma unroll
+        for (int ta = 0; ta < NTA; ++ta)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int a = ta * 16 + lg * 4 + i, c = ccol + ct * 16;
+                    if (a < da && c < dc) dst[(long long)a * r.init_a + (long long)c * r.init_c] = mul * S[ta][ct][i];
+                }
+    }
+}
+
+// Segment sums -> the carry in front of every segment, in place.  One thread owns one element of the state and walks the segments in scan order.
+struct JoinArgs {
+    float* part;
+    const float* init[2];
+    float init_mul[2];
+    int rev[2];
+    const float* log_decay;
+    const long long* lengths;
+    int T, B, H, nseg, seg_len, n;      // n = elements of a state
+};
+__global__ __launch_bounds__(256) void join_kernel(const JoinArgs g) {
+    const int el = blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y, set = blockIdx.z;
+    if (el >= g.n) return;
+    const int b = bh / g.H;
+    const float l2 = (float)((double)g.log_decay[bh % g.H] * 1.4426950408889634);
+    int n = g.T;
+    if (g.lengths) { const long long x = g.lengths[b]; n = x < 0 ? 0 : x < g.T ? (int)x : g.T; }
+    float* p = g.part + ((long long)set * g.B * g.H + bh) * g.nseg * (long long)g.n + el;
+    float carry = g.init[set] ? g.init_mul[set] * g.init[set][(long long)bh * g.n + el] : 0.f;
+    for (int i = 0; i < g.nseg; ++i) {
+        const int s = g.rev[set] ? g.nseg - 1 - i : i;
+        const int m = min(max(n - s * g.seg_len, 0), g.seg_len);
+        const float x = p[(long long)s * g.n];
+        p[(long long)s * g.n] = carry;
+        carry = m > 0 ? dpow(l2, m) * carry + x : carry;
+    }
+}
+
+// ---- recurrent form: one token a row, states updated in place.  A workgroup owns one (row, head): the state passes through the registers once
+// (read + written: 8 Dk Dv bytes are the whole cost), columns across the lanes, rows of the state across the rest of the workgroup.
+// Rows that name the same slot are successive tokens of that sequence, in row order: the first of them does the others' work as well.
+struct StepArgs {
+    const void *q, *k, *v;
+    void* o;
+    long long qs[2], ks[2], vs[2], os[2];
+    const float* log_decay;
+    float* state;
+    const long long* slots;
+    int B, H, Dk, Dv, nslots;
+    float scale;
+};
+template <class E> __device__ __forceinline__ float get(const E* p);
+template <> __device__ __forceinline__ float get<bf16_t>(const bf16_t* p) { return bf2f(*p); }
+template <> __device__ __forceinline__ float get<float>(const float* p) { return *p; }
+
+template <class E>
+__global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
+    __shared__ float sq[256], sk[256], red[256][4];
+    __shared__ int first, next;
+    const int tid = threadIdx.x, h = blockIdx.x % g.H;
+    int b = blockIdx.x / g.H;
+    long long slot = b;
+    if (g.slots) {
+        slot = g.slots[b];
+        if (slot < 0 || slot >= g.nslots) {               // a padded row: no state, output zero
+            E* o = (E*)g.o + b * g.os[0] + h * g.os[1];
+            for (int c = tid; c < g.Dv; c += 256) put(o + c, 0.f);
+            return;
+        }
+        if (tid == 0) { first = 1; next = g.B; }
+        __syncthreads();
+        int mine = g.B;
+        for (int x = tid; x < g.B; x += 256)
+            if (x != b && g.slots[x] == slot) {
+                if (x < b) first = 0;
+                else mine = min(mine, x);
+            }
+        if (mine < g.B) atomicMin(&next, mine);
+        __syncthreads();
+        if (!first) return;
+    }
+    const float a = expf(g.log_decay[h]);
+    float* st = g.state + (slot * g.H + h) * (long long)g.Dk * g.Dv;
+    const int nc = (g.Dv + 3) / 4;                        // columns in fours (at most 64 of them); 256 / nct rows of the state at a time
+    int nct = 1;
+    while (nct < nc) nct <<= 1;
+    const int rows = 256 / nct, c4 = tid % nct, r0 = tid / nct;
+    const bool vec = (g.Dv & 3) == 0;
+    while (true) {
+        const E* q = (const E*)g.q + b * g.qs[0] + h * g.qs[1];
+        const E* k = (const E*)g.k + b * g.ks[0] + h * g.ks[1];
+        const E* v = (const E*)g.v + b * g.vs[0] + h * g.vs[1];
+        E* o = (E*)g.o + b * g.os[0] + h * g.os[1];
+        for (int i = tid; i < g.Dk; i += 256) { sq[i] = g.scale * get(q + i); sk[i] = get(k + i); }
+        __syncthreads();
+        const int c = c4 * 4;
+        float vv[4], acc[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vv[x] = c + x < g.Dv ? get(v + c + x) : 0.f;
+        if (vec) {
+            if (c < g.Dv) {
+#pragma unroll 4
+                for (int i = r0; i < g.Dk; i += rows) {
+                    f32x4_t s = *reinterpret_cast<f32x4_t*>(st + (long long)i * g.Dv + c);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) { s[x] = a * s[x] + sk[i] * vv[x]; acc[x] += sq[i] * s[x]; }
+                    *reinterpret_cast<f32x4_t*>(st + (long long)i * g.Dv + c) = s;
+                }
+            }
+        } else {
+            for (int i = r0; i < g.Dk; i += rows)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (c + x < g.Dv) {
+                        float* p = st + (long long)i * g.Dv + c + x;
+                        const float s = a * *p + sk[i] * vv[x];
+                        *p = s;
+                        acc[x] += sq[i] * s;
+                    }
+        }
+        // sum over the row groups, in a fixed order
+#pragma unroll
+        for (int x = 0; x < 4; ++x) red[tid][x] = acc[x];
+        __syncthreads();
+        if (r0 == 0) {
+            for (int x = 0; x < 4; ++x) {
+                float s = 0.f;
+                for (int y = 0; y < rows; ++y) s += red[y * nct + c4][x];
+                if (c + x < g.Dv) put(o + c + x, s);
+            }
+        }
+        __syncthreads();
+        if (!g.slots) return;
+        b = next;
+        if (b >= g.B) return;
+        __syncthreads();
+        if (tid == 0) next = g.B;
+        __syncthreads();
+        int mine = g.B;
+        for (int x = b + 1 + tid; x < g.B; x += 256)
+            if (g.slots[x] == slot) mine = min(mine, x);
+        if (mine < g.B) atomicMin(&next, mine);
+        __syncthreads();
+    }
+}
+
+bool aligned(const void* p, long long s0, long long s1, long long s2, int d, int e, int bytes) {
+    const int n = bytes / e;
+    return ((uintptr_t)p % bytes) == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0 && d % n == 0;
+}
+Operand operand(const void* p, const int64_t* s, int d, int f32) {
+    return Operand{p, s[0], s[1], s[2], d, aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, 16) ? 1 : 0};
+}
+void output(Role& r, void* p, const int64_t* s, int d, int f32) {
+    r.o = p; r.ot = s[0]; r.ob = s[1]; r.oh = s[2];
+    r.ovec = aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, f32 ? 16 : 8);
+}
+
+template <class E, int DA, int NCT>
+void launch_one(ScanArgs& g, bool out, hipStream_t st) {
+    const unsigned grid = (unsigned)g.nroles * g.B * g.nseg * g.H * g.ncb;
+    if (out) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true>), dim3(grid), dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false>), dim3(grid), dim3(256), 0, st, g);
+}
+int da_class(int da) { return da <= 64 ? 64 : da <= 128 ? 128 : 256; }
+int nct_of(int da, int dc) { return da <= 128 && dc > 64 ? 2 : 1; }       // (256 features of a: 64 columns a workgroup, or the state would not fit its registers)
+
+// launches `n` roles; those that take the same kernel share a launch
+template <class E>
+void launch(const ScanArgs& base, const Role* roles, int n, bool out, float* part, hipStream_t st) {
+    bool done[3] = {false, false, false};
+    for (int i = 0; i < n; ++i) {
+        if (done[i]) continue;
+        ScanArgs g = base;
+        g.nroles = 0;
+        const int da = da_class(roles[i].a.d), nct = nct_of(roles[i].a.d, roles[i].c.d), ncb = (roles[i].c.d + 64 * nct - 1) / (64 * nct);
+        for (int j = i; j < n; ++j)
+            if (!done[j] && da_class(roles[j].a.d) == da && nct_of(roles[j].a.d, roles[j].c.d) == nct && (roles[j].c.d + 64 * nct - 1) / (64 * nct) == ncb
+                && (out || roles[j].a.d == roles[i].a.d)) {
+                g.r[g.nroles++] = roles[j];
+                done[j] = true;
+            }
+        g.ncb = ncb;
+        g.part = part + (out ? 0 : (long long)i * g.B * g.H * g.nseg * roles[i].a.d * roles[i].c.d);
+        if (da == 64) { if (nct == 2) launch_one<E, 64, 2>(g, out, st); else launch_one<E, 64, 1>(g, out, st); }
+        else if (da == 128) { if (nct == 2) launch_one<E, 128, 2>(g, out, st); else launch_one<E, 128, 1>(g, out, st); }
+        else launch_one<E, 256, 1>(g, out, st);
+    }
+}
+
+// Segments: with fewer (sequence, head) pairs than the chip has room for, a sequence is cut and its segments walked side by side.
+void segments(const srvp_linear_attention_desc* d, int roles, int* nseg, int* seg_len) {
+    const int C = d->elem_f32 ? 32 : 64;
+    const long long ncb = (d->Dv + 127) / 128, base = (long long)d->B * d->H * ncb * roles;
+    const long long chunks = (d->T + C - 1) / C;
+    long long n = base >= 256 || base == 0 ? 1 : (512 + base - 1) / base;
+    if (n > (chunks + 3) / 4) n = (chunks + 3) / 4;
+    if (n < 1) n = 1;
+    const long long per = chunks > n ? (chunks + n - 1) / n : 1;
+    *seg_len = (int)(per * C);
+    *nseg = (int)((chunks + per - 1) / per);
+    if (*nseg < 1) *nseg = 1;
+}
+
+int check(const srvp_linear_attention_desc* d, const char* who) {
+    SRVP_REQUIRE(d, "%s: null descriptor", who);
+    SRVP_REQUIRE(d->T >= 0 && d->B >= 0 && d->H >= 0, "%s: negative size", who);
+    SRVP_REQUIRE(d->Dk >= 1 && d->Dk <= 256 && d->Dv >= 1 && d->Dv <= 256, "%s: heads of 1 to 256 features (got %d, %d)", who, d->Dk, d->Dv);
+    SRVP_REQUIRE(d->T < (1 << 30) && (long long)d->B * d->H < (1 << 20), "%s: more than 2^30 tokens or 2^20 (sequence, head) pairs", who);
+    SRVP_REQUIRE(d->scale != 0.f && d->scale - d->scale == 0.f, "%s: scale must be finite and not zero", who);
+    return SRVP_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t srvp_linear_attention_ws_bytes(const srvp_linear_attention_desc* d, int32_t backward) {
+    if (check(d, "srvp_linear_attention_ws_bytes")) return -1;
+    int nseg, len;
+    segments(d, backward ? 3 : 1, &nseg, &len);
+    return nseg <= 1 ? 0 : (int64_t)(backward ? 2 : 1) * d->B * d->H * nseg * d->Dk * d->Dv * 4;
+}
+
+static int run_join(const ScanArgs& base, const srvp_linear_attention_desc* d, int sets, const float* const* init, const float* mul, float* part, hipStream_t st) {
+    JoinArgs j;
+    memset(&j, 0, sizeof(j));
+    j.part = part; j.log_decay = d->log_decay; j.lengths = base.lengths;
+    for (int i = 0; i < sets; ++i) { j.init[i] = init[i]; j.init_mul[i] = mul[i]; j.rev[i] = i; }
+    j.T = d->T; j.B = d->B; j.H = d->H; j.nseg = base.nseg; j.seg_len = base.seg_len; j.n = d->Dk * d->Dv;
+    // (grid.y: a sequence is cut where there are fewer than 256 pairs)
+    hipLaunchKernelGGL(join_kernel, dim3((j.n + 255) / 256, d->B * d->H, sets), dim3(256), 0, st, j);
+    SRVP_CHECK_LAUNCH("srvp_linear_attention(join)");
+    return SRVP_OK;
+}
+
+static void base_args(ScanArgs& g, const srvp_linear_attention_desc* d, int roles) {
+    memset(&g, 0, sizeof(g));
+    g.log_decay = d->log_decay; g.lengths = (const long long*)d->lengths;
+    g.T = d->T; g.B = d->B; g.H = d->H; g.scale = d->scale;
+    segments(d, roles, &g.nseg, &g.seg_len);
+}
+
+extern "C" int srvp_linear_attention_fwd(const srvp_linear_attention_desc* d, void* stream) {
+    if (int rc = check(d, "srvp_linear_attention_fwd")) return rc;
+    if (d->B == 0 || d->H == 0) return SRVP_OK;
+    SRVP_REQUIRE(d->log_decay && (d->T == 0 || (d->q && d->k && d->v && d->o)), "srvp_linear_attention_fwd: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    ScanArgs g;
+    base_args(g, d, 1);
+    const int64_t need = srvp_linear_attention_ws_bytes(d, 0);
+    SRVP_REQUIRE(need == 0 || (d->ws && d->ws_bytes >= need), "srvp_linear_attention_fwd: workspace of %lld bytes needed", (long long)need);
+    Role r;
+    memset(&r, 0, sizeof(r));
+    r.a = operand(d->q, d->qs, d->Dk, d->elem_f32);
+    r.b = operand(d->k, d->ks, d->Dk, d->elem_f32);
+    r.c = operand(d->v, d->vs, d->Dv, d->elem_f32);
+    output(r, d->o, d->os, d->Dv, d->elem_f32);
+    r.init = d->state_in; r.init_mul = 1.f; r.fin = d->state_out; r.fin_mul = 1.f;
+    r.init_a = d->Dv; r.init_c = 1;
+    if (g.nseg > 1) {
+        float* part = (float*)d->ws;
+        if (d->elem_f32) launch<float>(g, &r, 1, false, part, st); else launch<bf16_t>(g, &r, 1, false, part, st);
+        SRVP_CHECK_LAUNCH("srvp_linear_attention_fwd(segments)");
+        const float* init[1] = {d->state_in};
+        const float mul[1] = {1.f};
+        if (int rc = run_join(g, d, 1, init, mul, part, st)) return rc;
+        r.prefix = part;
+    }
+    if (d->elem_f32) launch<float>(g, &r, 1, true, nullptr, st); else launch<bf16_t>(g, &r, 1, true, nullptr, st);
+    SRVP_CHECK_LAUNCH("srvp_linear_attention_fwd");
+    return SRVP_OK;
+}
+
+extern "C" int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* bd, void* stream) {
+    SRVP_REQUIRE(bd, "srvp_linear_attention_bwd: null descriptor");
+    const srvp_linear_attention_desc* d = &bd->f;
+    if (int rc = check(d, "srvp_linear_attention_bwd")) return rc;
+    if (d->B == 0 || d->H == 0) return SRVP_OK;
+    SRVP_REQUIRE(d->log_decay && (d->T == 0 || (d->q && d->k && d->v && bd->d_o && bd->dq && bd->dk && bd->dv)), "srvp_linear_attention_bwd: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    ScanArgs g;
+    base_args(g, d, 3);
+    const int64_t need = srvp_linear_attention_ws_bytes(d, 1);
+    SRVP_REQUIRE(need == 0 || (d->ws && d->ws_bytes >= need), "srvp_linear_attention_bwd: workspace of %lld bytes needed", (long long)need);
+    const int f32 = d->elem_f32, Dk = d->Dk, Dv = d->Dv;
+    const Operand q = operand(d->q, d->qs, Dk, f32), k = operand(d->k, d->ks, Dk, f32), v = operand(d->v, d->vs, Dv, f32), go = operand(bd->d_o, bd->d_os, Dv, f32);
+    Role r[3];
+    memset(r, 0, sizeof(r));
+    // dv: (k, q, do), reversed, carry X (Dk x Dv)
+    r[0].a = k; r[0].b = q; r[0].c = go; output(r[0], bd->dv, bd->dvs, Dv, f32);
+    r[0].rev = 1; r[0].init = bd->d_state_out; r[0].init_mul = 1.f / d->scale; r[0].fin = bd->d_state_in; r[0].fin_mul = d->scale;
+    r[0].init_a = Dv; r[0].init_c = 1;
+    // dk: (v, do, q), reversed, carry X^T
+    r[1].a = v; r[1].b = go; r[1].c = q; output(r[1], bd->dk, bd->dks, Dk, f32);
+    r[1].rev = 1; r[1].init = bd->d_state_out; r[1].init_mul = 1.f / d->scale; r[1].init_a = 1; r[1].init_c = Dv;
+    // dq: (do, v, k), forwards, carry S^T
+    r[2].a = go; r[2].b = v; r[2].c = k; output(r[2], bd->dq, bd->dqs, Dk, f32);
+    r[2].init = d->state_in; r[2].init_mul = 1.f; r[2].init_a = 1; r[2].init_c = Dv;
+    if (g.nseg > 1) {
+        float* part = (float*)d->ws;
+        const long long set = (long long)d->B * d->H * g.nseg * Dk * Dv;
+        Role p[2];                                        // segment sums of S (k, v) and of X (q, do)
+        memset(p, 0, sizeof(p));
+        p[0].a = k; p[0].b = k; p[0].c = v; p[0].init_a = Dv; p[0].init_c = 1;
+        p[1].a = q; p[1].b = q; p[1].c = go; p[1].init_a = Dv; p[1].init_c = 1; p[1].rev = 1;
+        if (f32) launch<float>(g, p, 2, false, part, st); else launch<bf16_t>(g, p, 2, false, part, st);
+        SRVP_CHECK_LAUNCH("srvp_linear_attention_bwd(segments)");
+        const float* init[2] = {d->state_in, bd->d_state_out};
+        const float mul[2] = {1.f, 1.f / d->scale};
+        if (int rc = run_join(g, d, 2, init, mul, part, st)) return rc;
+        r[0].prefix = r[1].prefix = part + set;
+        r[2].prefix = part;
+    }
+    if (f32) launch<float>(g, r, 3, true, nullptr, st); else launch<bf16_t>(g, r, 3, true, nullptr, st);
+    SRVP_CHECK_LAUNCH("srvp_linear_attention_bwd");
+    return SRVP_OK;
+}
+
+extern "C" int srvp_linear_attention_step(const srvp_linear_attention_step_desc* d, void* stream) {
+    SRVP_REQUIRE(d, "srvp_linear_attention_step: null descriptor");
+    SRVP_REQUIRE(d->B >= 0 && d->H >= 0 && d->nslots >= 0 && (long long)d->B * d->H < (1 << 30), "srvp_linear_attention_step: bad sizes");
+    SRVP_REQUIRE(d->Dk >= 1 && d->Dk <= 256 && d->Dv >= 1 && d->Dv <= 256, "srvp_linear_attention_step: heads of 1 to 256 features (got %d, %d)", d->Dk, d->Dv);
+    if (d->B == 0 || d->H == 0) return SRVP_OK;
+    SRVP_REQUIRE(d->q && d->k && d->v && d->o && d->log_decay && (d->state || d->nslots == 0), "srvp_linear_attention_step: null pointer");
+    SRVP_REQUIRE(d->slots || d->B <= d->nslots, "srvp_linear_attention_step: %d rows for %d states", d->B, d->nslots);
+    SRVP_REQUIRE((uintptr_t)d->state % 16 == 0, "srvp_linear_attention_step: state must be 16-byte aligned");
+    StepArgs g;
+    g.q = d->q; g.k = d->k; g.v = d->v; g.o = d->o;
+    for (int i = 0; i < 2; ++i) { g.qs[i] = d->qs[i]; g.ks[i] = d->ks[i]; g.vs[i] = d->vs[i]; g.os[i] = d->os[i]; }
+    g.log_decay = d->log_decay; g.state = d->state; g.slots = (const long long*)d->slots;
+    g.B = d->B; g.H = d->H; g.Dk = d->Dk; g.Dv = d->Dv; g.nslots = d->nslots; g.scale = d->scale;
+    if (d->elem_f32) hipLaunchKernelGGL(step_kernel<float>, dim3(d->B * d->H), dim3(256), 0, (hipStream_t)stream, g);
+    else hipLaunchKernelGGL(step_kernel<bf16_t>, dim3(d->B * d->H), dim3(256), 0, (hipStream_t)stream, g);
+    SRVP_CHECK_LAUNCH("srvp_linear_attention_step");
+    return SRVP_OK;
+}
