@@ -59,23 +59,19 @@ __device__ __forceinline__ float dpow(float l2, int n) { return n <= 0 ? 1.f : e
 // ---- the two element types.  KS = contraction elements of one step; a fragment holds, for lane (g = lane >> 4, s = lane & 15), the KS/4 elements
 // whose index in the step is 4g .. 4g+3 (and 16 + 4g .. for bf16) of row / column s.  That order is the one in which a 16x16 accumulator tile holds its
 // rows, so a product's result is the next product's operand without leaving the registers.
+//
+// View<E, W>: a tile of W features a row in LDS, read as fragments along its rows (contraction over features) and across them (over tokens).
+// bf16: 8-byte chunks, exchanged within every 128 bytes of a row by chunk ^= swz(row).  A wave reads 16 rows of one chunk, or (ds_read_b64_tr_b16) 4 rows of 4
+// chunks, 16 lanes at a time: both touch each pair of the 32 banks once.  (Rows padded by 16 bytes instead: two-way conflicts in both, 43 % of the LDS time.)
+// fp32: rows padded by 16 bytes.
 template <class E> struct Ty;
+template <class E, int W> struct View;
+
+__device__ __forceinline__ int swz(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+
 template <> struct Ty<bf16_t> {
-    static constexpr int KS = 32, TPK = 2, C = 64, VE = 8, PAD = 8;
+    static constexpr int KS = 32, TPK = 2, C = 64, VE = 8;
     typedef s16x8_t frag;
-    static __device__ __forceinline__ frag rows(const bf16_t* t, int ld, int row, int k, int lane) {
-        const bf16_t* p = t + (row + (lane & 15)) * ld + k + (lane >> 4) * 4;
-        const s16x4_t lo = *reinterpret_cast<const s16x4_t*>(p), hi = *reinterpret_cast<const s16x4_t*>(p + 16);
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    // ds_read_b64_tr_b16: lane s of a 16-lane group receives column s of the 4 x 16 block whose row j the lanes 4j .. 4j+3 address
-    static __device__ __forceinline__ frag cols(const bf16_t* t, int ld, int row, int col, int lane) {
-        typedef __attribute__((address_space(3))) s16x4_t lds_t;
-        const bf16_t* p = t + (row + (lane >> 4) * 4 + ((lane & 15) >> 2)) * ld + col + (lane & 3) * 4;
-        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p);
-        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + 16 * ld));
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
     static __device__ __forceinline__ frag pack(const f32x4_t* t) {
         u32x4_t v;
         v.x = pack2bf(t[0][0], t[0][1]); v.y = pack2bf(t[0][2], t[0][3]);
@@ -85,8 +81,9 @@ template <> struct Ty<bf16_t> {
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, const f32x4_t& c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
     }
+    // x * w as a sum of three bf16 values of 8 significant bits each: the fp32 product to its last bit, so the state (a result of its own) has fp32's
+    // accuracy.  Two terms (2^-17) would save 5 % of a long sequence's time, but outputs would then depend on whether the state was asked for.
     static constexpr int SPLIT = 3;
-    // x * w as a sum of three bf16 values (8 significant bits each: the fp32 product to its last bit)
     static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) {
         float f[8];
         unpack8(__builtin_bit_cast(u32x4_t, x), f);
@@ -103,16 +100,51 @@ template <> struct Ty<bf16_t> {
         }
     }
 };
+template <int W> struct View<bf16_t, W> {
+    typedef __attribute__((address_space(3))) s16x4_t lds_t;
+    typedef s16x8_t frag;
+    static constexpr int RB = W * 2;                       // bytes of a row
+    static constexpr int elems(int rows) { return rows * W; }
+    static __device__ __forceinline__ int at(int row, int col) { return row * W + ((((col >> 2) ^ swz(row)) << 2) | (col & 3)); }      // (the low 4 bits of the chunk)
+    int r[4], t[4];                                        // byte offsets of the lane's chunks 4x: row s; row 4g + (s >> 2), chunk s & 3
+    __device__ __forceinline__ explicit View(int lane) {
+        const int g = lane >> 4, s = lane & 15, q = 4 * g + (s >> 2);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            r[x] = s * RB + (((4 * x + g) ^ swz(s)) << 3);
+            t[x] = q * RB + (((4 * x + (s & 3)) ^ swz(q)) << 3);
+        }
+    }
+    // rows row0 + s, step d of the features
+    __device__ __forceinline__ frag rows(const bf16_t* base, int row0, int d) const {
+        const char* p = (const char*)base + row0 * RB;
+        const s16x4_t lo = *reinterpret_cast<const s16x4_t*>(p + ((2 * d) >> 2) * 128 + r[(2 * d) & 3]);
+        const s16x4_t hi = *reinterpret_cast<const s16x4_t*>(p + ((2 * d + 1) >> 2) * 128 + r[(2 * d + 1) & 3]);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    // byte offset of the lane's chunk of columns 16 c ..
+    static __device__ __forceinline__ int column(int lane, int c) {
+        const int s = lane & 15, q = 4 * (lane >> 4) + (s >> 2);
+        return q * RB + (((4 * c + (s & 3)) ^ swz(q)) << 3);
+    }
+    // columns 16 c + s, tokens row0 .. row0 + 31.  ds_read_b64_tr_b16: lane s of a 16-lane group receives column s of the 4 x 16 block whose row j the lanes
+    // 4j .. 4j+3 address
+    __device__ __forceinline__ frag cols(const bf16_t* base, int row0, int c) const { return at_column(base, row0, (c >> 2) * 128 + t[c & 3]); }
+    static __device__ __forceinline__ frag at_column(const bf16_t* base, int row0, int off) {
+        const char* p = (const char*)base + row0 * RB + off;
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p);
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + 16 * RB));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ void put16(bf16_t* base, int row, int col, const u32x4_t& v) {
+        *reinterpret_cast<uint2*>(base + at(row, col)) = make_uint2(v.x, v.y);
+        *reinterpret_cast<uint2*>(base + at(row, col + 4)) = make_uint2(v.z, v.w);
+    }
+};
+
 template <> struct Ty<float> {
-    static constexpr int KS = 16, TPK = 1, C = 32, VE = 4, PAD = 4;
+    static constexpr int KS = 16, TPK = 1, C = 32, VE = 4;
     typedef f32x4_t frag;
-    static __device__ __forceinline__ frag rows(const float* t, int ld, int row, int k, int lane) {
-        return *reinterpret_cast<const f32x4_t*>(t + (row + (lane & 15)) * ld + k + (lane >> 4) * 4);
-    }
-    static __device__ __forceinline__ frag cols(const float* t, int ld, int row, int col, int lane) {
-        const float* p = t + (row + (lane >> 4) * 4) * ld + col + (lane & 15);
-        return frag{p[0], p[ld], p[2 * ld], p[3 * ld]};
-    }
     static __device__ __forceinline__ frag pack(const f32x4_t* t) { return t[0]; }
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, f32x4_t c) {
 #pragma unroll
@@ -122,39 +154,21 @@ template <> struct Ty<float> {
     static constexpr int SPLIT = 1;
     static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) { out[0] = frag{x[0] * w[0], x[1] * w[1], x[2] * w[2], x[3] * w[3]}; }
 };
-
-// ---- global -> registers -> LDS: C rows x W columns of one operand, zero outside the chunk's tokens and the operand's features.  Row i of the tile is
-// token c0 + i, or c0 + mm - 1 - i in reversed time: everything behind the loader sees time running forwards.
-template <class E, int W> struct Tile {
-    static constexpr int C = Ty<E>::C, VE = Ty<E>::VE, NV = C * W / VE / 256, LD = W + Ty<E>::PAD;
-    u32x4_t v[NV];
-    __device__ __forceinline__ void load(const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int idx = i * 256 + tid, row = idx / (W / VE), col = (idx % (W / VE)) * VE;
-            u32x4_t x = {0, 0, 0, 0};
-            if (row < mm) {
-                const E* p = base + (long long)(c0 + (rev ? mm - 1 - row : row)) * s.st + col0 + col;
-                const int left = s.d - col0 - col;
-                if (s.vec) {
-                    if (left > 0) x = *reinterpret_cast<const u32x4_t*>(p);
-                } else {
-                    E e[VE];
-#pragma unroll
-                    for (int j = 0; j < VE; ++j) e[j] = j < left ? p[j] : E(0);
-                    __builtin_memcpy(&x, e, 16);
-                }
-            }
-            v[i] = x;
-        }
+template <int W> struct View<float, W> {
+    typedef f32x4_t frag;
+    static constexpr int LD = W + 4;
+    static constexpr int elems(int rows) { return rows * LD; }
+    static __device__ __forceinline__ int at(int row, int col) { return row * LD + col; }
+    int r, t;
+    __device__ __forceinline__ explicit View(int lane) : r((lane & 15) * LD + (lane >> 4) * 4), t((lane >> 4) * 4 * LD + (lane & 15)) {}
+    __device__ __forceinline__ frag rows(const float* base, int row0, int d) const { return *reinterpret_cast<const f32x4_t*>(base + row0 * LD + d * 16 + r); }
+    static __device__ __forceinline__ int column(int lane, int c) { return (lane >> 4) * 4 * LD + (lane & 15) + c * 16; }
+    __device__ __forceinline__ frag cols(const float* base, int row0, int c) const { return at_column(base, row0, t + c * 16); }
+    static __device__ __forceinline__ frag at_column(const float* base, int row0, int off) {
+        const float* p = base + row0 * LD + off;
+        return frag{p[0], p[LD], p[2 * LD], p[3 * LD]};
     }
-    __device__ __forceinline__ void store(E* lds, int tid) const {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int idx = i * 256 + tid, row = idx / (W / VE), col = (idx % (W / VE)) * VE;
-            *reinterpret_cast<u32x4_t*>(lds + row * LD + col) = v[i];
-        }
-    }
+    static __device__ __forceinline__ void put16(float* base, int row, int col, const u32x4_t& v) { *reinterpret_cast<u32x4_t*>(base + at(row, col)) = v; }
 };
 
 __device__ __forceinline__ void put(bf16_t* p, float v) { *p = f2bf(v); }
@@ -162,21 +176,64 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put4(bf16_t* p, const f32x4_t& v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3])); }
 __device__ __forceinline__ void put4(float* p, const f32x4_t& v) { *reinterpret_cast<f32x4_t*>(p) = v; }
 
+// ---- global -> registers -> LDS: C rows x W columns of one operand, zero outside the chunk's tokens and the operand's features.  Row i of the tile is
+// token c0 + i, or c0 + mm - 1 - i in reversed time: everything behind the loader sees time running forwards.
+// VEC: 16 bytes at a time.  The loads carry no condition (rows and columns are clamped to valid ones and zeroed on the way into LDS): a load under a branch
+// makes the compiler wait for every load in flight where the paths meet, three memory latencies a chunk.  Otherwise the elements go straight to LDS in `store`.
+template <class E, int W, bool VEC> struct Tile {
+    using V = View<E, W>;
+    static constexpr int C = Ty<E>::C, VE = Ty<E>::VE, NV = C * W / VE / 256, ROWS = 256 / (W / VE);
+    u32x4_t v[NV];
+    __device__ __forceinline__ void load(const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) {
+        if constexpr (VEC) {
+            const char* p = (const char*)(base + (long long)c0 * s.st);
+            const unsigned step = (unsigned)s.st * sizeof(E), row = tid / (W / VE), col = min(col0 + (int)(tid % (W / VE)) * VE, s.d - VE) * sizeof(E);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const unsigned at = min((int)row + i * ROWS, mm - 1);
+                v[i] = *reinterpret_cast<const u32x4_t*>(p + (size_t)((rev ? mm - 1 - at : at) * step + col));      // (64 tokens are less than 2^31 bytes apart)
+            }
+        }
+    }
+    __device__ __forceinline__ void store(E* lds, const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) const {
+        if constexpr (VEC) {
+            const int row = tid / (W / VE), col = (tid % (W / VE)) * VE;
+            if (mm == C && s.d - col0 >= W) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) V::put16(lds, row + i * ROWS, col, v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const bool in = row + i * ROWS < mm && col0 + col < s.d;
+                    V::put16(lds, row + i * ROWS, col, in ? v[i] : u32x4_t{0, 0, 0, 0});
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int i = tid; i < C * W; i += 256) {
+                const int row = i / W, col = i % W;
+                lds[V::at(row, col)] = row < mm && col0 + col < s.d ? base[(long long)(c0 + (rev ? mm - 1 - row : row)) * s.st + col0 + col] : E(0);
+            }
+        }
+    }
+};
+
 // One workgroup (4 waves) walks one segment of one (sequence, head) in scan order; wave w owns 16 * NCT columns of c, hence of the state (registers,
 // fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel).
-template <class E, int DA, int NCT, bool OUT>
-__global__ __launch_bounds__(256) void scan_kernel(const ScanArgs g) {
+// A chunk: the three tiles go to LDS (the next chunk's loads are in flight meanwhile); the lower-triangular 16 x 16 tiles of the scores are dealt to the
+// waves and exchanged through LDS; then every wave forms its columns of the output and of the state.
+template <class E, int DA, int NCT, bool OUT, bool VEC>
+__global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanArgs g) {
     using Y = Ty<E>;
     typedef typename Y::frag frag;
-    constexpr int C = Y::C, KS = Y::KS, TPK = Y::TPK, CB = 64 * NCT, ND = DA / KS, NJ = C / KS, NTA = DA / 16;
-    using TA = Tile<E, DA>;
-    using TC = Tile<E, CB>;
-    __shared__ __align__(16) E lds[(OUT ? C * TA::LD : 0) + C * TA::LD + C * TC::LD];
-    E* lb = lds;
-    E* lc = lb + C * TA::LD;
-    E* la = lc + C * TC::LD;
+    constexpr int C = Y::C, KS = Y::KS, TPK = Y::TPK, SPLIT = Y::SPLIT, CB = 64 * NCT, ND = DA / KS, NJ = C / KS, NTA = DA / 16, NTI = C / 16;
+    using VA = View<E, DA>;
+    using VC = View<E, CB>;
+    using VP = View<E, C>;
+    __shared__ __align__(16) E lb[VA::elems(C)], lc[VC::elems(C)], la[OUT ? VA::elems(C) : 1], lp[OUT ? VP::elems(C) : 1];      // lp: scores [i][j]
+    __shared__ float pw[C + 1];                              // a^n
 
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, lg = lane >> 4, ls = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
     int id = blockIdx.x;
     const int cb = id % g.ncb; id /= g.ncb;
     const int h = id % g.H; id /= g.H;
@@ -184,7 +241,7 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanArgs g) {
     const int b = id % g.B, ro = id / g.B;
     const Role& r = g.r[ro];
     const long long bh = (long long)b * g.H + h;
-    const int da = r.a.d, dc = r.c.d, col0 = cb * CB, e = r.rev ? 0 : 1;
+    const int da = r.a.d, dc = r.c.d, col0 = cb * CB, rev = r.rev, e = rev ? 0 : 1;
     const float l2 = (float)((double)g.log_decay[h] * 1.4426950408889634);
 
     int n = g.T;
@@ -197,16 +254,29 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanArgs g) {
     const E* pc = (const E*)r.c.p + b * r.c.sb + h * r.c.sh;
     E* po = (E*)r.o + b * r.ob + h * r.oh;
 
+    Tile<E, DA, VEC> ra, rb;
+    Tile<E, CB, VEC> rc;
+    auto fetch = [&](int cc) {
+        const int c0 = t0 + (rev ? nch - 1 - cc : cc) * C, mm = min(C, t1 - c0);
+        if (OUT) ra.load(r.a, pa, c0, mm, rev, 0, tid);
+        rb.load(r.b, pb, c0, mm, rev, 0, tid);
+        rc.load(r.c, pc, c0, mm, rev, col0, tid);
+    };
+    if (nch > 0) fetch(0);
+
+    if (tid <= C) pw[tid] = dpow(l2, tid);
     if (OUT) {
         // rows behind the sequence's last token: zero
         const int cw = min(CB, dc - col0);
         for (int t = max(t0, n); t < te; ++t)
             for (int c = tid; c < cw; c += 256) put(po + t * r.ot + col0 + c, 0.f);
+        // scores above the diagonal tiles: zero, once
+        for (int i = tid; i < VP::elems(C); i += 256) lp[i] = E(0);
     }
 
     // state: tile (ta, ct) holds rows 16 ta + 4 lg + {0..3}, column ccol + 16 ct
     const int ccol = col0 + w * 16 * NCT + ls;
-    f32x4_t S[NTA][NCT];
+    f32x4_t S[NCT][NTA];
     {
         const float* src = nullptr;
         float mul = 1.f;
@@ -215,102 +285,97 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanArgs g) {
             else if (r.init) { src = r.init + bh * (long long)da * dc; mul = r.init_mul; }
         }
 #pragma unroll
-        for (int ta = 0; ta < NTA; ++ta)
+        for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct)
+            for (int ta = 0; ta < NTA; ++ta)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int a = ta * 16 + lg * 4 + i, c = ccol + ct * 16;
-                    S[ta][ct][i] = (src && a < da && c < dc) ? mul * src[(long long)a * r.init_a + (long long)c * r.init_c] : 0.f;
+                    S[ct][ta][i] = (src && a < da && c < dc) ? mul * src[(long long)a * r.init_a + (long long)c * r.init_c] : 0.f;
                 }
     }
+    float near[4], next[4];                               // a^(i-j) inside a diagonal tile (0 above it); a^(16 + i - j) for the tile left of it
+    if (OUT) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int gap = ls - lg * 4 - x;
+            near[x] = gap >= 0 ? dpow(l2, gap) : 0.f;
+            next[x] = dpow(l2, 16 + gap);
+        }
+    }
+    const VA va(lane);
+    int vcol[NCT];
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) vcol[ct] = VC::column(lane, w * NCT + ct);
+    const VP vp(lane);
 
-    TA ra, rb;
-    TC rc;
-    auto fetch = [&](int cc) {
-        const int ch = r.rev ? nch - 1 - cc : cc, c0 = t0 + ch * C, mm = min(C, t1 - c0);
-        if (OUT) ra.load(r.a, pa, c0, mm, r.rev, 0, tid);
-        rb.load(r.b, pb, c0, mm, r.rev, 0, tid);
-        rc.load(r.c, pc, c0, mm, r.rev, col0, tid);
-    };
-    if (nch > 0) fetch(0);
-    for (int cc = 0; cc < nch; ++cc) {
-        const int ch = r.rev ? nch - 1 - cc : cc, c0 = t0 + ch * C, mm = min(C, t1 - c0);
-        __syncthreads();                                  // (the previous chunk's tiles have been read)
-        if (OUT) ra.store(la, tid);
-        rb.store(lb, tid);
-        rc.store(lc, tid);
-        __syncthreads();
-        if (cc + 1 < nch) fetch(cc + 1);                  // in flight under this chunk's products
-
+    auto chunk = [&](int c0, int mm) {
+        if (OUT) {
+            // tiles (ti, tj <= ti), dealt in turn
+            int ti = 0, tj = w;
+            while (tj > ti) { tj -= ti + 1; ++ti; }
+            while (ti < NTI && (ti * 16 < mm)) {
+                f32x4_t P = {0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < ND; ++d) P = Y::mfma(va.rows(lb, tj * 16, d), va.rows(la, ti * 16, d), P);
+                if (tj == ti) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) P[x] = ls >= lg * 4 + x ? P[x] * near[x] : 0.f;
+                } else {
+                    const float back = pw[16 * (ti - tj - 1)];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) P[x] *= next[x] * back;
+                }
+                put4(lp + VP::at(ti * 16 + ls, tj * 16 + lg * 4), P);      // bf16: the scores are rounded once
+                tj += 4;
+                while (tj > ti) { tj -= ti + 1; ++ti; }
+            }
+        }
         frag vf[NJ][NCT];
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = Y::cols(lc, TC::LD, j * KS, (w * NCT + ct) * 16, lane);
+            for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = VC::at_column(lc, j * KS, vcol[ct]);
 
         if (OUT) {
-            frag sf[ND][NCT];
+            frag sf[ND][NCT];                             // bf16: the state is rounded once for the product with a (it is kept in fp32)
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int ct = 0; ct < NCT; ++ct) {
-                    f32x4_t t[TPK];
+                for (int ct = 0; ct < NCT; ++ct) sf[d][ct] = Y::pack(S[ct] + d * TPK);
+            __syncthreads();                              // the scores are complete
 #pragma unroll
-                    for (int x = 0; x < TPK; ++x) t[x] = S[d * TPK + x][ct];
-                    sf[d][ct] = Y::pack(t);               // bf16: the state is rounded once for the product with q (it is kept in fp32)
-                }
-            float near[4], next[4];                       // a^(i-j) inside a diagonal tile (0 above it); a^(16 + i - j) for the tile below
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int gap = ls - lg * 4 - x;
-                near[x] = gap >= 0 ? dpow(l2, gap) : 0.f;
-                next[x] = dpow(l2, 16 + gap);
-            }
-#pragma unroll
-            for (int ti = 0; ti < C / 16; ++ti) {
+            for (int ti = 0; ti < NTI; ++ti) {
                 if (ti * 16 < mm) {
-                    frag af[ND];
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) af[d] = Y::rows(la, TA::LD, ti * 16, d * KS, lane);
                     // output^T tiles: rows = columns of c (4 lg + ..), column = token ti * 16 + ls
                     f32x4_t acc[NCT];
 #pragma unroll
-                    for (int ct = 0; ct < NCT; ++ct) {
-                        acc[ct] = f32x4_t{0, 0, 0, 0};
+                    for (int ct = 0; ct < NCT; ++ct) acc[ct] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-                        for (int d = 0; d < ND; ++d) acc[ct] = Y::mfma(sf[d][ct], af[d], acc[ct]);
-                        acc[ct] *= dpow(l2, ti * 16 + ls + e);
+                    for (int d = 0; d < ND; ++d) {
+                        const frag af = va.rows(la, ti * 16, d);
+#pragma unroll
+                        for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(sf[d][ct], af, acc[ct]);
                     }
+                    const float past = pw[ti * 16 + ls + e];
+#pragma unroll
+                    for (int ct = 0; ct < NCT; ++ct) acc[ct] *= past;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
                         if (j * KS <= ti * 16 + 15) {
-                            f32x4_t P[TPK];
-#pragma unroll
-                            for (int x = 0; x < TPK; ++x) {
-                                const int tj = j * TPK + x;
-                                P[x] = f32x4_t{0, 0, 0, 0};
-                                if (tj <= ti) {
-#pragma unroll
-                                    for (int d = 0; d < ND; ++d) P[x] = Y::mfma(Y::rows(lb, TA::LD, tj * 16, d * KS, lane), af[d], P[x]);
-                                    const float back = dpow(l2, 16 * (ti - tj - 1));
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) P[x][i] = tj == ti ? (ls >= lg * 4 + i ? P[x][i] * near[i] : 0.f) : P[x][i] * (next[i] * back);
-                                }
-                            }
-                            const frag pf = Y::pack(P);   // bf16: the scores are rounded once, like the state above
+                            const frag pf = vp.rows(lp, ti * 16, j);
 #pragma unroll
                             for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf, acc[ct]);
                         }
                     }
                     const int i = ti * 16 + ls;
                     if (i < mm) {
-                        E* q = po + (long long)(c0 + (r.rev ? mm - 1 - i : i)) * r.ot;
+                        E* q = po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot;
 #pragma unroll
                         for (int ct = 0; ct < NCT; ++ct) {
                             const int c = col0 + (w * NCT + ct) * 16 + lg * 4;
                             acc[ct] *= g.scale;
-                            if (r.ovec) {
+                            if (VEC) {
                                 if (c < dc) put4(q + c, acc[ct]);
                             } else {
 #pragma unroll
@@ -323,30 +388,41 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanArgs g) {
             }
         }
         // state update
-        const float all = dpow(l2, mm);
+        const float all = pw[mm];
 #pragma unroll
-        for (int ta = 0; ta < NTA; ++ta)
+        for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) S[ta][ct] *= all;
+            for (int ta = 0; ta < NTA; ++ta) S[ct][ta] *= all;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             if (j * KS < mm) {
                 float wt[KS / 4];
 #pragma unroll
-                for (int x = 0; x < KS / 4; ++x) wt[x] = dpow(l2, mm - e - (j * KS + (x >> 2) * 16 + lg * 4 + (x & 3)));
-                frag wv[NCT][Y::SPLIT];
+                for (int x = 0; x < KS / 4; ++x) wt[x] = pw[max(0, mm - e - (j * KS + (x >> 2) * 16 + lg * 4 + (x & 3)))];     // (rows behind mm are zero)
+                frag wv[NCT][SPLIT];
 #pragma unroll
                 for (int ct = 0; ct < NCT; ++ct) Y::weigh(vf[j][ct], wt, wv[ct]);
 #pragma unroll
                 for (int ta = 0; ta < NTA; ++ta) {
-                    const frag kf = Y::cols(lb, TA::LD, j * KS, ta * 16, lane);
+                    const frag kf = va.cols(lb, j * KS, ta);
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-                        for (int s = 0; s < Y::SPLIT; ++s) S[ta][ct] = Y::mfma(kf, wv[ct][s], S[ta][ct]);
+                        for (int x = 0; x < SPLIT; ++x) S[ct][ta] = Y::mfma(kf, wv[ct][x], S[ct][ta]);
                 }
             }
         }
+    };
+
+    for (int cc = 0; cc < nch; ++cc) {
+        const int c0 = t0 + (rev ? nch - 1 - cc : cc) * C, mm = min(C, t1 - c0);
+        __syncthreads();                                  // (the previous chunk's tiles have been read)
+        if (OUT) ra.store(la, r.a, pa, c0, mm, rev, 0, tid);
+        rb.store(lb, r.b, pb, c0, mm, rev, 0, tid);
+        rc.store(lc, r.c, pc, c0, mm, rev, col0, tid);
+        __syncthreads();
+        if (cc + 1 < nch) fetch(cc + 1);                  // in flight under this chunk's products
+        chunk(c0, mm);
     }
 
     float* dst = nullptr;
@@ -354,18 +430,18 @@ __global__ __launch_bounds__(256) void scan_kernel(const ScanArgs g) {
     if (!OUT) {
         dst = g.part + (((long long)ro * g.B * g.H + bh) * g.nseg + seg) * (long long)da * dc;
     } else if (r.fin) {
-        const int last = r.rev ? 0 : n > 0 ? (n - 1) / g.seg_len : 0;
+        const int last = rev ? 0 : n > 0 ? (n - 1) / g.seg_len : 0;
         if (seg == last) { dst = r.fin + bh * (long long)da * dc; mul = r.fin_mul; }
     }
     if (dst) {
 #pragma unroll
-        for (int ta = 0; ta < NTA; ++ta)
+        for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct)
+            for (int ta = 0; ta < NTA; ++ta)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int a = ta * 16 + lg * 4 + i, c = ccol + ct * 16;
-                    if (a < da && c < dc) dst[(long long)a * r.init_a + (long long)c * r.init_c] = mul * S[ta][ct][i];
+                    if (a < da && c < dc) dst[(long long)a * r.init_a + (long long)c * r.init_c] = mul * S[ct][ta][i];
                 }
     }
 }
@@ -389,12 +465,22 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs g) {
     if (g.lengths) { const long long x = g.lengths[b]; n = x < 0 ? 0 : x < g.T ? (int)x : g.T; }
     float* p = g.part + ((long long)set * g.B * g.H + bh) * g.nseg * (long long)g.n + el;
     float carry = g.init[set] ? g.init_mul[set] * g.init[set][(long long)bh * g.n + el] : 0.f;
-    for (int i = 0; i < g.nseg; ++i) {
-        const int s = g.rev[set] ? g.nseg - 1 - i : i;
-        const int m = min(max(n - s * g.seg_len, 0), g.seg_len);
-        const float x = p[(long long)s * g.n];
-        p[(long long)s * g.n] = carry;
-        carry = m > 0 ? dpow(l2, m) * carry + x : carry;
+    for (int i0 = 0; i0 < g.nseg; i0 += 8) {
+        float x[8];                                       // (eight loads in flight; the stores go to the same places)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = min(i0 + k, g.nseg - 1);
+            x[k] = p[(long long)(g.rev[set] ? g.nseg - 1 - i : i) * g.n];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k, s = g.rev[set] ? g.nseg - 1 - i : i;
+            if (i < g.nseg) {
+                const int m = min(max(n - s * g.seg_len, 0), g.seg_len);
+                p[(long long)s * g.n] = carry;
+                carry = m > 0 ? dpow(l2, m) * carry + x[k] : carry;
+            }
+        }
     }
 }
 
@@ -511,7 +597,7 @@ bool aligned(const void* p, long long s0, long long s1, long long s2, int d, int
     return ((uintptr_t)p % bytes) == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0 && d % n == 0;
 }
 Operand operand(const void* p, const int64_t* s, int d, int f32) {
-    return Operand{p, s[0], s[1], s[2], d, aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, 16) ? 1 : 0};
+    return Operand{p, s[0], s[1], s[2], d, aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, 16) && s[0] >= 0 && s[0] < (1 << 23) ? 1 : 0};
 }
 void output(Role& r, void* p, const int64_t* s, int d, int f32) {
     r.o = p; r.ot = s[0]; r.ob = s[1]; r.oh = s[2];
@@ -519,15 +605,20 @@ void output(Role& r, void* p, const int64_t* s, int d, int f32) {
 }
 
 template <class E, int DA, int NCT>
-void launch_one(ScanArgs& g, bool out, hipStream_t st) {
-    const unsigned grid = (unsigned)g.nroles * g.B * g.nseg * g.H * g.ncb;
-    if (out) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true>), dim3(grid), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false>), dim3(grid), dim3(256), 0, st, g);
+void launch_one(const ScanArgs& g, bool out, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)g.nroles * g.B * g.nseg * g.H * g.ncb), wg(256);
+    if (out) {
+        if (vec) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, true>), grid, wg, 0, st, g);
+        else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, false>), grid, wg, 0, st, g);
+    } else {
+        if (vec) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false, true>), grid, wg, 0, st, g);
+        else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false, false>), grid, wg, 0, st, g);
+    }
 }
 int da_class(int da) { return da <= 64 ? 64 : da <= 128 ? 128 : 256; }
 int nct_of(int da, int dc) { return da <= 128 && dc > 64 ? 2 : 1; }       // (256 features of a: 64 columns a workgroup, or the state would not fit its registers)
 
-// launches `n` roles; those that take the same kernel share a launch
+// Launches `n` roles; those that take the same kernel share a launch.
 template <class E>
 void launch(const ScanArgs& base, const Role* roles, int n, bool out, float* part, hipStream_t st) {
     bool done[3] = {false, false, false};
@@ -543,10 +634,12 @@ void launch(const ScanArgs& base, const Role* roles, int n, bool out, float* par
                 done[j] = true;
             }
         g.ncb = ncb;
+        bool vec = true;                                  // 16-byte rows in and out
+        for (int j = 0; j < g.nroles; ++j) vec = vec && g.r[j].b.vec && g.r[j].c.vec && (!out || (g.r[j].a.vec && g.r[j].ovec));
         g.part = part + (out ? 0 : (long long)i * g.B * g.H * g.nseg * roles[i].a.d * roles[i].c.d);
-        if (da == 64) { if (nct == 2) launch_one<E, 64, 2>(g, out, st); else launch_one<E, 64, 1>(g, out, st); }
-        else if (da == 128) { if (nct == 2) launch_one<E, 128, 2>(g, out, st); else launch_one<E, 128, 1>(g, out, st); }
-        else launch_one<E, 256, 1>(g, out, st);
+        if (da == 64) { if (nct == 2) launch_one<E, 64, 2>(g, out, vec, st); else launch_one<E, 64, 1>(g, out, vec, st); }
+        else if (da == 128) { if (nct == 2) launch_one<E, 128, 2>(g, out, vec, st); else launch_one<E, 128, 1>(g, out, vec, st); }
+        else launch_one<E, 256, 1>(g, out, vec, st);
     }
 }
 
