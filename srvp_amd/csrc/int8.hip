@@ -31,67 +31,275 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put4(bf16_t* p, const f32x4_t& v) { *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3])); }
 __device__ __forceinline__ void put4(float* p, const f32x4_t& v) { *reinterpret_cast<f32x4_t*>(p) = v; }
 
-// 128 x 128 outputs a workgroup, 4 waves of 64 x 64; W is the left operand, so that a lane holds 4 neighbouring columns of one row of y.
-template <class E>
-__global__ __launch_bounds__(256) void int8_tile_kernel(const Int8Args g) {
-    constexpr int BK = 64, LD = BK + 16;
-    __shared__ __align__(16) signed char lx[128 * LD], lw[128 * LD];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, lg = lane >> 4, ls = lane & 15;
-    const int m0 = blockIdx.y * 128, n0 = blockIdx.x * 128, wm = (wv & 1) * 64, wn = (wv >> 1) * 64;
-    i32x4_t acc[4][4];
+// W is the left operand of every product, so that a lane holds 4 neighbouring columns of one row of y.
+template <class E> __device__ __forceinline__ void finish(const Int8Args& g, int m, int n, const int* acc) {
+    if (m >= g.M) return;
+    const float xs = g.xs[m];
+    E* y = (E*)g.y + (long long)m * g.ldy + n;
+    f32x4_t o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int r = 0; r < 4; ++r) o[r] = n + r < g.N ? (float)acc[r] * xs * g.ws[n + r] + (g.bias ? g.bias[n + r] : 0.f) : 0.f;
+    if (g.vecy) {
+        if (n < g.N) put4(y, o);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
-    for (int k0 = 0; k0 < g.K; k0 += BK) {
-        u32x4_t vx[2], vw[2];
+        for (int r = 0; r < 4; ++r)
+            if (n + r < g.N) put(y + r, o[r]);
+    }
+}
+
+// workgroup -> tile: every XCD owns a contiguous range of tiles (xcd_remap), which walks bands of 8 row tiles down the columns: the 32 tiles in flight on an
+// XCD are 8 x 4, and share their operands' rows in its L2
+__device__ __forceinline__ void tile_of(unsigned id, unsigned tm, unsigned tn, unsigned& im, unsigned& in) {
+    id = xcd_remap(id, tm * tn);
+    const unsigned band = id / (8 * tn), rows = min(8u, tm - band * 8), in_band = id - band * 8 * tn;
+    im = band * 8 + in_band % rows;
+    in = in_band / rows;
+}
+
+__device__ __align__(16) signed char zero16[16];
+
+// BM x BN outputs a workgroup of WM x WN waves; rows 16-byte aligned, K a multiple of 16.  Four LDS stages of 64 bytes of k are filled by LDS-DMA three ahead
+// of the products; 16-byte chunks are exchanged (chunk ^= (row >> 1) & 3, on the global side: the LDS side of a DMA is linear) so that 8 rows of one chunk lie
+// on all 32 banks.  One barrier a stage: behind it every wave has both stage i (its own loads waited for) and left the buffer of stage i + 3.
+template <class E, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void int8_dma_kernel(const Int8Args g) {
+    constexpr int NT = WM * WN * 64, BK = 64, STAGES = 4, MT = BM / WM / 32, NTL = BN / WN / 32, LA = BM * 4 / NT, LW = BN * 4 / NT;
+    typedef int i32x16_t __attribute__((ext_vector_type(16)));
+    typedef __attribute__((address_space(1))) const void* gptr_t;
+    typedef __attribute__((address_space(3))) void* lptr_t;
+    extern __shared__ __align__(16) signed char lds[];       // [stage][BM + BN rows][BK]
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l32 = lane & 31;
+    const int wm = (wid % WM) * (BM / WM), wn = (wid / WM) * (BN / WN);
+    unsigned im, in;
+    tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
+    const int m0 = im * BM, n0 = in * BN;
+    // this thread's rows and chunk (the same in every stage)
+    const signed char *px[LA], *pw[LW];
+    const int chunk = tid & 3;
+    int kx[LA], kw[LW];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int idx = i * 256 + tid, row = idx >> 2, k = k0 + (idx & 3) * 16;
-            vx[i] = m0 + row < g.M ? bytes16(g.x + (long long)(m0 + row) * g.ldx, k, g.K) : u32x4_t{0, 0, 0, 0};
-            vw[i] = n0 + row < g.N ? bytes16(g.w + (long long)(n0 + row) * g.ldw, k, g.K) : u32x4_t{0, 0, 0, 0};
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int idx = i * 256 + tid, row = idx >> 2, k = (idx & 3) * 16;
-            *reinterpret_cast<u32x4_t*>(lx + row * LD + k) = vx[i];
-            *reinterpret_cast<u32x4_t*>(lw + row * LD + k) = vw[i];
-        }
-        __syncthreads();
-        i32x4_t fx[4], fw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            fx[i] = *reinterpret_cast<const i32x4_t*>(lx + (wm + i * 16 + ls) * LD + lg * 16);
-            fw[i] = *reinterpret_cast<const i32x4_t*>(lw + (wn + i * 16 + ls) * LD + lg * 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
+    for (int i = 0; i < LA; ++i) {
+        const int row = (i * NT + tid) >> 2;
+        kx[i] = (chunk ^ ((row >> 1) & 3)) * 16;
+        px[i] = g.x + (long long)min(m0 + row, g.M - 1) * g.ldx + kx[i];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int m = m0 + wm + i * 16 + ls;
-        if (m < g.M) {
-            const float xs = g.xs[m];
-            E* y = (E*)g.y + (long long)m * g.ldy;
+    for (int i = 0; i < LW; ++i) {
+        const int row = (i * NT + tid) >> 2;
+        kw[i] = (chunk ^ ((row >> 1) & 3)) * 16;
+        pw[i] = g.w + (long long)min(n0 + row, g.N - 1) * g.ldw + kw[i];
+    }
+    const int steps = (g.K + BK - 1) / BK;
+    auto issue = [&](int s) {
+        const int k0 = s * BK;
+        signed char* lx = lds + (s & (STAGES - 1)) * (BM + BN) * BK;
+        signed char* lw = lx + BM * BK;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + wn + j * 16 + lg * 4;
-                f32x4_t o;
+        for (int i = 0; i < LA; ++i)
+            __builtin_amdgcn_global_load_lds((gptr_t)(k0 + kx[i] < g.K ? px[i] + k0 : zero16), (lptr_t)(lx + (i * NT + wid * 64) * 16), 16, 0, 0);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] = n + r < g.N ? (float)acc[i][j][r] * xs * g.ws[n + r] + (g.bias ? g.bias[n + r] : 0.f) : 0.f;
-                if (g.vecy) {
-                    if (n < g.N) put4(y + n, o);
-                } else {
+        for (int i = 0; i < LW; ++i)
+            __builtin_amdgcn_global_load_lds((gptr_t)(k0 + kw[i] < g.K ? pw[i] + k0 : zero16), (lptr_t)(lw + (i * NT + wid * 64) * 16), 16, 0, 0);
+    };
+    i32x16_t acc[MT][NTL];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < g.N) put(y + n + r, o[r]);
-                }
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    // byte offset of the lane's chunk of k step ks in row l32 (+ 32 t: the same exchange)
+    const int sw = (l32 >> 1) & 3;
+    const int off[2] = {l32 * BK + ((half ^ sw) << 4), l32 * BK + (((2 + half) ^ sw) << 4)};
+    issue(0);
+    if (steps > 1) issue(1);
+    if (steps > 2) issue(2);
+    for (int s = 0; s < steps; ++s) {
+        // stage s has landed: all but the loads of the stages behind it (at most two)
+        const int behind = min(steps - 1 - s, 2);
+        // (lgkmcnt: this wave's reads of the stage before it are back, so its buffer may be filled again)
+        if (behind == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * (LA + LW)) : "memory");
+        else if (behind == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LA + LW) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + 3 < steps) issue(s + 3);
+        const signed char* lx = lds + (s & (STAGES - 1)) * (BM + BN) * BK;
+        const signed char* lw = lx + BM * BK;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            i32x4_t fx[MT], fw[NTL];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fx[i] = *reinterpret_cast<const i32x4_t*>(lx + (wm + i * 32) * BK + off[ks]);
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) fw[j] = *reinterpret_cast<const i32x4_t*>(lw + (wn + j * 32) * BK + off[ks]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int a[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                finish<E>(g, m0 + wm + i * 32 + l32, n0 + wn + j * 32 + 8 * q + 4 * half, a);
+            }
+}
+
+// BM x BN outputs a workgroup of 2 x 2 waves, rows at any byte: 64 bytes of k pass through registers, the next ones under the products.
+template <class E, int BM, int BN>
+__global__ __launch_bounds__(256, 2) void int8_tile_kernel(const Int8Args g) {
+    constexpr int BK = 64, LD = BK + 16, MT = BM / 32, NTL = BN / 32, LA = BM * 4 / 256, LW = BN * 4 / 256;
+    __shared__ __align__(16) signed char lx[BM * LD], lw[BN * LD];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, lg = lane >> 4, ls = lane & 15;
+    unsigned im, in;
+    tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
+    const int m0 = im * BM, n0 = in * BN, wm = (wv & 1) * (BM / 2), wn = (wv >> 1) * (BN / 2);
+    i32x4_t acc[MT][NTL];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+    u32x4_t vx[LA], vw[LW];
+    const signed char *px[LA], *pw[LW];
+    const int kc = (tid & 3) * 16;
+#pragma unroll
+    for (int i = 0; i < LA; ++i) px[i] = g.x + (long long)min(m0 + ((i * 256 + tid) >> 2), g.M - 1) * g.ldx;      // (rows behind the last: not written)
+#pragma unroll
+    for (int i = 0; i < LW; ++i) pw[i] = g.w + (long long)min(n0 + ((i * 256 + tid) >> 2), g.N - 1) * g.ldw;
+    auto fetch = [&](int k0) {
+        if (k0 + BK <= g.K) {
+#pragma unroll
+            for (int i = 0; i < LA; ++i) __builtin_memcpy(&vx[i], px[i] + k0 + kc, 16);
+#pragma unroll
+            for (int i = 0; i < LW; ++i) __builtin_memcpy(&vw[i], pw[i] + k0 + kc, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LA; ++i) vx[i] = bytes16(px[i], k0 + kc, g.K);
+#pragma unroll
+            for (int i = 0; i < LW; ++i) vw[i] = bytes16(pw[i], k0 + kc, g.K);
+        }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < g.K; k0 += BK) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < LA; ++i) *reinterpret_cast<u32x4_t*>(lx + ((i * 256 + tid) >> 2) * LD + kc) = vx[i];
+#pragma unroll
+        for (int i = 0; i < LW; ++i) *reinterpret_cast<u32x4_t*>(lw + ((i * 256 + tid) >> 2) * LD + kc) = vw[i];
+        __syncthreads();
+        if (k0 + BK < g.K) fetch(k0 + BK);
+        i32x4_t fx[MT], fw[NTL];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fx[i] = *reinterpret_cast<const i32x4_t*>(lx + (wm + i * 16 + ls) * LD + lg * 16);
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) fw[j] = *reinterpret_cast<const i32x4_t*>(lw + (wn + j * 16 + ls) * LD + lg * 16);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) {
+            const int a[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+            finish<E>(g, m0 + wm + i * 16 + ls, n0 + wn + j * 16 + lg * 4, a);
+        }
+}
+
+// Few rows (M <= 16 MT): the weight's bytes are the cost.  A workgroup owns 16 rows of w and all rows of x; its 8 waves deal the steps of 64 bytes of k among
+// them, w straight from memory into the fragments, UNROLL steps in flight; the partial sums (whole numbers: any order) meet in LDS.
+template <class E, int MT, bool ALIGNED>
+__global__ __launch_bounds__(512) void int8_rows_kernel(const Int8Args g) {
+    constexpr int UNROLL = MT == 1 ? 8 : 4;
+    __shared__ int red[8][MT * 4 * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
+    const int n0 = blockIdx.x * 16;
+    const signed char* w = g.w + (long long)min(n0 + ls, g.N - 1) * g.ldw;
+    const signed char* x[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = g.x + (long long)min(i * 16 + ls, g.M - 1) * g.ldx;
+    i32x4_t acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = i32x4_t{0, 0, 0, 0};
+    const int steps = (g.K + 63) / 64;
+    for (int s0 = wid; s0 < steps; s0 += 8 * UNROLL) {
+        u32x4_t fw[UNROLL], fx[UNROLL][MT];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = (s0 + u * 8) * 64 + lg * 16;
+            if (ALIGNED) {
+                const bool in = k < g.K;
+                const int at = in ? k : 0;
+                fw[u] = *reinterpret_cast<const u32x4_t*>(w + at);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) fx[u][i] = *reinterpret_cast<const u32x4_t*>(x[i] + at);
+                if (!in) fw[u] = u32x4_t{0, 0, 0, 0};
+            } else {
+                fw[u] = bytes16(w, k, g.K);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) fx[u][i] = bytes16(x[i], k, g.K);
             }
         }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, fw[u]), __builtin_bit_cast(i32x4_t, fx[u][i]), acc[i], 0, 0, 0);
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) red[wid][(i * 4 + r) * 64 + lane] = acc[i][r];
+    __syncthreads();
+    for (int i = wid; i < MT; i += 8) {
+        int a[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            a[r] = 0;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) a[r] += red[v][(i * 4 + r) * 64 + lane];
+        }
+        finish<E>(g, i * 16 + ls, n0 + lg * 4, a);
+    }
+}
+
+template <class E, int BM, int BN, int WM, int WN>
+hipError_t dma_launch(const Int8Args& g, hipStream_t st) {
+    constexpr int bytes = 4 * (BM + BN) * 64;
+    const auto kern = int8_dma_kernel<E, BM, BN, WM, WN>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kern, dim3(((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN)), dim3(WM * WN * 64), bytes, st, g);
+    return hipSuccess;
+}
+template <class E>
+hipError_t launch(const Int8Args& g, bool aligned, hipStream_t st) {
+    const long long t256 = (long long)((g.M + 255) / 256) * ((g.N + 255) / 256), t128 = (long long)((g.M + 127) / 128) * ((g.N + 127) / 128);
+    if (g.M <= 64) {
+        const dim3 grid((g.N + 15) / 16);
+#define ROWS(MT)                                                                                                   \
+    do {                                                                                                           \
+        if (aligned) hipLaunchKernelGGL((int8_rows_kernel<E, MT, true>), grid, dim3(512), 0, st, g);               \
+        else hipLaunchKernelGGL((int8_rows_kernel<E, MT, false>), grid, dim3(512), 0, st, g);                      \
+    } while (0)
+        if (g.M <= 16) ROWS(1);
+        else if (g.M <= 32) ROWS(2);
+        else ROWS(4);
+#undef ROWS
+        return hipSuccess;
+    }
+    if (aligned && t256 >= 192) return dma_launch<E, 256, 256, 2, 4>(g, st);
+    if (aligned && t128 >= 128) return dma_launch<E, 128, 128, 2, 2>(g, st);
+    if (!aligned && t128 >= 512) hipLaunchKernelGGL((int8_tile_kernel<E, 128, 128>), dim3((unsigned)t128), dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((int8_tile_kernel<E, 64, 64>), dim3((unsigned)(((g.M + 63) / 64) * ((g.N + 63) / 64))), dim3(256), 0, st, g);
+    return hipSuccess;
 }
 
 }  // namespace
@@ -101,16 +309,20 @@ extern "C" int srvp_linear_int8(const srvp_linear_int8_desc* d, void* stream) {
     SRVP_REQUIRE(d->M >= 0 && d->N >= 0 && d->K >= 0, "srvp_linear_int8: negative size");
     SRVP_REQUIRE(d->K <= 131071, "srvp_linear_int8: more than 131071 products could pass 32 bits (K = %d)", d->K);
     if (d->M == 0 || d->N == 0) return SRVP_OK;
-    SRVP_REQUIRE((d->K == 0 || (d->x && d->w)) && d->x_scale && d->w_scale && d->y, "srvp_linear_int8: null pointer");
+    SRVP_REQUIRE(d->K > 0, "srvp_linear_int8: K must be positive");
+    SRVP_REQUIRE(d->x && d->w && d->x_scale && d->w_scale && d->y, "srvp_linear_int8: null pointer");
     const int e = d->out_f32 ? 4 : 2;
     Int8Args g;
     g.x = (const signed char*)d->x; g.w = (const signed char*)d->w; g.xs = d->x_scale; g.ws = d->w_scale; g.bias = d->bias; g.y = d->y;
     g.ldx = d->ldx; g.ldw = d->ldw; g.ldy = d->ldy; g.M = d->M; g.N = d->N; g.K = d->K;
     g.vecy = (uintptr_t)d->y % (4 * e) == 0 && d->ldy % 4 == 0 && d->N % 4 == 0;
-    SRVP_REQUIRE((d->M + 127) / 128 < 65536, "srvp_linear_int8: too many rows (M = %d)", d->M);
-    const dim3 grid((d->N + 127) / 128, (d->M + 127) / 128);
-    if (d->out_f32) hipLaunchKernelGGL(int8_tile_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, g);
-    else hipLaunchKernelGGL(int8_tile_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, g);
+    SRVP_REQUIRE((long long)((d->M + 63) / 64) * ((d->N + 63) / 64) < (1LL << 30), "srvp_linear_int8: too many outputs (%d x %d)", d->M, d->N);
+    const bool aligned = d->K % 16 == 0 && d->ldx % 16 == 0 && d->ldw % 16 == 0 && (uintptr_t)d->x % 16 == 0 && (uintptr_t)d->w % 16 == 0;
+    const hipError_t err = d->out_f32 ? launch<float>(g, aligned, (hipStream_t)stream) : launch<bf16_t>(g, aligned, (hipStream_t)stream);
+    if (err != hipSuccess) {
+        srvp_set_error("srvp_linear_int8: %s", hipGetErrorString(err));
+        return SRVP_ERR_LAUNCH;
+    }
     SRVP_CHECK_LAUNCH("srvp_linear_int8");
     return SRVP_OK;
 }

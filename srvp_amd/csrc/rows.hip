@@ -8,6 +8,18 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------- rotary
 // Pair p of a head is turned by positions[t][b] * freq[p] radians.  The angle is formed in 64 bits as a number of whole turns, of which only the
 // fraction matters; its sine and cosine are computed once a (row, pair) for all heads of q and k, in LDS.
+struct Div {                               // n / d for n < 2^31 as one high product: m = ceil(2^(32 + s) / d), s = ceil(log2 d) - 1
+    unsigned d, m, s;
+    __device__ __forceinline__ unsigned of(unsigned n) const { return d == 1 ? n : __umulhi(n, m) >> s; }
+};
+Div divide(unsigned d) {
+    Div r{d, 0, 0};
+    if (d > 1) {
+        while ((2ull << r.s) < d) ++r.s;
+        r.m = (unsigned)(((1ull << (32 + r.s)) + d - 1) / d);
+    }
+    return r;
+}
 struct RotArgs {
     const void *x[2];
     void *o[2];
@@ -16,19 +28,21 @@ struct RotArgs {
     long long pt, pb;
     const double* freq;
     int T, B, H0, H1, D, n, inter, R;      // n pairs; R rows a workgroup
+    Div dB, dn, dH, ditems;
     float sign, mult;
 };
 constexpr int ROT_TAB = 2048;
+enum { SINGLE, HALVES, PAIRS };            // single pairs and elements; 16-byte vectors of the halves layout; 16-byte vectors of adjacent pairs
 
-template <class E, int VE, bool VEC>
+// A head is `first` items that turn (HALVES: two vectors each) and the rest of the head, copied.  A thread has U items' loads in flight.
+template <class E, int VE, int MODE>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
-    __shared__ float tc[ROT_TAB], ts[ROT_TAB];
+    __shared__ __align__(16) float tc[ROT_TAB], ts[ROT_TAB];
     const int tid = threadIdx.x;
     const long long rows = (long long)g.T * g.B, row0 = (long long)blockIdx.x * g.R;
     const int R = (int)min((long long)g.R, rows - row0);
     for (int i = tid; i < R * g.n; i += 256) {
-        const int r = i / g.n, p = i - r * g.n;
-        const long long row = row0 + r, t = row / g.B, b = row - t * g.B;
+        const unsigned r = g.dn.of(i), p = i - r * g.n, row = (unsigned)row0 + r, t = g.dB.of(row), b = row - t * g.B;
         double turns = (double)g.pos[t * g.pt + b * g.pb] * (g.freq[p] * 0.15915494309189535);
         turns -= rint(turns);
         float s, c;
@@ -37,58 +51,69 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
         ts[i] = s * g.mult * g.sign;
     }
     __syncthreads();
-    const int H = g.H0 + g.H1;
-    // items of a head: VEC, halves layout: n / VE pairs of vectors, then the rest of the head in vectors; VEC, adjacent pairs: D / VE vectors;
-    // otherwise single pairs, then single elements
-    const int first = VEC ? (g.inter ? 2 * g.n / VE : g.n / VE) : g.n, items = first + (g.D - 2 * g.n) / (VEC ? VE : 1);
-    const int total = R * H * items;
-    for (int i = tid; i < total; i += 256) {
-        const int it = i % items, rh = i / items, hh = rh % H, r = rh / H;
-        const int w = hh >= g.H0, h = w ? hh - g.H0 : hh;
-        const long long row = row0 + r, t = row / g.B, b = row - t * g.B;
-        const E* x = (const E*)g.x[w] + t * g.xs[w][0] + b * g.xs[w][1] + h * g.xs[w][2];
-        E* o = (E*)g.o[w] + t * g.os[w][0] + b * g.os[w][1] + h * g.os[w][2];
-        const float *c = tc + r * g.n, *s = ts + r * g.n;
-        if constexpr (VEC) {
-            typedef u32x4_t vec;
-            if (it >= first) {
-                const int at = 2 * g.n + (it - first) * VE;
-                *reinterpret_cast<vec*>(o + at) = *reinterpret_cast<const vec*>(x + at);
-            } else if (g.inter) {
-                float u[VE];
-                const int at = it * VE, p = at / 2;
-                E e[VE];
-                *reinterpret_cast<vec*>(e) = *reinterpret_cast<const vec*>(x + at);
+    const int H = g.H0 + g.H1, items = g.ditems.d, total = R * H * items;
+    const int first = MODE == SINGLE ? g.n : MODE == HALVES ? g.n / VE : 2 * g.n / VE;
+    constexpr int U = MODE == SINGLE ? 1 : 4;
+    for (int i0 = tid; i0 < total; i0 += 256 * U) {
+        const E* x[U];
+        E* o[U];
+        int it[U], tab[U];
+        u32x4_t e[U], f[U];
 #pragma unroll
-                for (int j = 0; j < VE; ++j) u[j] = El<E>::ld(e + j);
+        for (int u = 0; u < U; ++u) {
+            const unsigned i = min(i0 + u * 256, total - 1), rh = g.ditems.of(i), r = g.dH.of(rh), hh = rh - r * H;      // (repeated items write the same)
+            it[u] = i - rh * items;
+            tab[u] = r * g.n;
+            const int w = (int)hh >= g.H0, h = w ? hh - g.H0 : hh;
+            const unsigned row = (unsigned)row0 + r, t = g.dB.of(row), b = row - t * g.B;
+            x[u] = (const E*)g.x[w] + (long long)t * g.xs[w][0] + (long long)b * g.xs[w][1] + h * g.xs[w][2];
+            o[u] = (E*)g.o[w] + (long long)t * g.os[w][0] + (long long)b * g.os[w][1] + h * g.os[w][2];
+            if constexpr (MODE != SINGLE) {
+                const int at = MODE == HALVES && it[u] >= first ? 2 * g.n + (it[u] - first) * VE : it[u] * VE;
+                e[u] = *reinterpret_cast<const u32x4_t*>(x[u] + at);
+                if (MODE == HALVES) f[u] = *reinterpret_cast<const u32x4_t*>(x[u] + (it[u] < first ? g.n : 0) + (it[u] < first ? at : 0));
+            }
+        }
 #pragma unroll
-                for (int j = 0; j < VE / 2; ++j) {
-                    El<E>::st(e + 2 * j, u[2 * j] * c[p + j] - u[2 * j + 1] * s[p + j]);
-                    El<E>::st(e + 2 * j + 1, u[2 * j] * s[p + j] + u[2 * j + 1] * c[p + j]);
+        for (int u = 0; u < U; ++u) {
+            if constexpr (MODE == SINGLE) {
+                if (it[u] >= first) {
+                    o[u][2 * g.n + it[u] - first] = x[u][2 * g.n + it[u] - first];
+                } else {
+                    const int a0 = g.inter ? 2 * it[u] : it[u], a1 = g.inter ? 2 * it[u] + 1 : g.n + it[u];
+                    const float v = El<E>::ld(x[u] + a0), z = El<E>::ld(x[u] + a1), c = tc[tab[u] + it[u]], s = ts[tab[u] + it[u]];
+                    El<E>::st(o[u] + a0, v * c - z * s);
+                    El<E>::st(o[u] + a1, v * s + z * c);
                 }
-                *reinterpret_cast<vec*>(o + at) = *reinterpret_cast<vec*>(e);
-            } else {
-                const int p = it * VE;
-                E e[VE], f[VE];
-                *reinterpret_cast<vec*>(e) = *reinterpret_cast<const vec*>(x + p);
-                *reinterpret_cast<vec*>(f) = *reinterpret_cast<const vec*>(x + g.n + p);
+            } else if (it[u] >= first) {
+                *reinterpret_cast<u32x4_t*>(o[u] + (MODE == HALVES ? 2 * g.n + (it[u] - first) * VE : it[u] * VE)) = e[u];
+            } else if constexpr (MODE == HALVES) {
+                const int p = it[u] * VE;
+                E a[VE], b[VE];
+                __builtin_memcpy(a, &e[u], 16);
+                __builtin_memcpy(b, &f[u], 16);
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
-                    const float u = El<E>::ld(e + j), v = El<E>::ld(f + j);
-                    El<E>::st(e + j, u * c[p + j] - v * s[p + j]);
-                    El<E>::st(f + j, u * s[p + j] + v * c[p + j]);
+                    const float v = El<E>::ld(a + j), z = El<E>::ld(b + j), c = tc[tab[u] + p + j], s = ts[tab[u] + p + j];
+                    El<E>::st(a + j, v * c - z * s);
+                    El<E>::st(b + j, v * s + z * c);
                 }
-                *reinterpret_cast<vec*>(o + p) = *reinterpret_cast<vec*>(e);
-                *reinterpret_cast<vec*>(o + g.n + p) = *reinterpret_cast<vec*>(f);
-            }
-        } else {
-            if (it >= first) {
-                o[2 * g.n + it - first] = x[2 * g.n + it - first];
+                __builtin_memcpy(&e[u], a, 16);
+                __builtin_memcpy(&f[u], b, 16);
+                *reinterpret_cast<u32x4_t*>(o[u] + p) = e[u];
+                *reinterpret_cast<u32x4_t*>(o[u] + g.n + p) = f[u];
             } else {
-                const int a0 = g.inter ? 2 * it : it, a1 = g.inter ? 2 * it + 1 : g.n + it;
-                const float u = El<E>::ld(x + a0), v = El<E>::ld(x + a1);
-                El<E>::st(o + a0, u * c[it] - v * s[it]);
-                El<E>::st(o + a1, u * s[it] + v * c[it]);
+                const int p = it[u] * VE / 2;
+                E a[VE];
+                __builtin_memcpy(a, &e[u], 16);
+#pragma unroll
+                for (int j = 0; j < VE / 2; ++j) {
+                    const float v = El<E>::ld(a + 2 * j), z = El<E>::ld(a + 2 * j + 1), c = tc[tab[u] + p + j], s = ts[tab[u] + p + j];
+                    El<E>::st(a + 2 * j, v * c - z * s);
+                    El<E>::st(a + 2 * j + 1, v * s + z * c);
+                }
+                __builtin_memcpy(&e[u], a, 16);
+                *reinterpret_cast<u32x4_t*>(o[u] + 2 * p) = e[u];
             }
         }
     }
@@ -102,7 +127,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
 // 8-bit output: row scale s = max|y| / 127, q = round-half-even(h w * (127 / max|h w|)), i.e. y / s: the row's root mean square cancels.  Products and the
 // quotient are formed in 64 bits, so q does not depend on the order of any sum.  A row of zeros has scale 0; a row with an infinity or NaN has scale NaN
 // and q = 0, i.e. stands for NaN.
-// TPR threads (a wave, or a workgroup of 256) hold one row in registers: V vectors of VE elements each.
+// TPR threads hold one row in registers: V vectors of VE elements each.
 struct NormArgs {
     const void *x, *res;
     const float* w;
@@ -115,147 +140,167 @@ struct NormArgs {
     float eps;
 };
 
-template <class E, int VE, int V, int TPR>
-__device__ __forceinline__ void row_load(const E* p, int N, int vec, int t, float* f) {
+// Value i of thread t of a row: column (i / VE * TPR + t) * VE + i % VE where rows are read 16 bytes at a time, i * TPR + t otherwise.
+template <int VE, int TPR> __device__ __forceinline__ int column(int i, int t, int vec) { return vec ? (i / VE * TPR + t) * VE + i % VE : i * TPR + t; }
+
+// a row as it lies in memory: the next row's loads are in flight while this one is reduced and written
+template <class E, int VE, int V, int TPR> struct Raw {
+    u32x4_t v[V];
+    __device__ __forceinline__ void load(const E* p, int N, int vec, int t) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int c = (v * TPR + t) * VE;
-        E e[VE];
-        if (vec) {
-            u32x4_t x = {0, 0, 0, 0};
-            if (c < N) x = *reinterpret_cast<const u32x4_t*>(p + c);
-            __builtin_memcpy(e, &x, 16);
-        } else {
+        for (int i = 0; i < V; ++i) {
+            v[i] = u32x4_t{0, 0, 0, 0};
+            if (vec) {
+                const int c = (i * TPR + t) * VE;
+                if (c < N) v[i] = *reinterpret_cast<const u32x4_t*>(p + c);
+            } else {
+                E e[VE];
 #pragma unroll
-            for (int j = 0; j < VE; ++j) e[j] = c + j < N ? p[c + j] : E(0);
+                for (int j = 0; j < VE; ++j) {
+                    const int c = (i * VE + j) * TPR + t;
+                    e[j] = c < N ? p[c] : E(0);
+                }
+                __builtin_memcpy(&v[i], e, 16);
+            }
         }
+    }
+    __device__ __forceinline__ float get(int i) const {      // (unrolled loops only: i is a constant)
+        E e[VE];
+        __builtin_memcpy(e, &v[i / VE], 16);
+        return El<E>::ld(e + i % VE);
+    }
+};
+template <int VE, int V, int TPR> __device__ __forceinline__ void load_weight(const float* w, int N, int vec, int t, float* f) {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) f[v * VE + j] = El<E>::ld(e + j);
+    for (int i = 0; i < V * VE; ++i) {
+        const int c = column<VE, TPR>(i, t, vec);
+        f[i] = c < N ? w[c] : 0.f;
     }
 }
 template <class E, int VE, int V, int TPR>
 __device__ __forceinline__ void row_store(E* p, int N, int vec, int t, const float* f) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int c = (v * TPR + t) * VE;
         E e[VE];
 #pragma unroll
         for (int j = 0; j < VE; ++j) El<E>::st(e + j, f[v * VE + j]);
         if (vec) {
+            const int c = (v * TPR + t) * VE;
             u32x4_t x;
             __builtin_memcpy(&x, e, 16);
             if (c < N) *reinterpret_cast<u32x4_t*>(p + c) = x;
         } else {
 #pragma unroll
-            for (int j = 0; j < VE; ++j)
-                if (c + j < N) p[c + j] = e[j];
+            for (int j = 0; j < VE; ++j) {
+                const int c = (v * VE + j) * TPR + t;
+                if (c < N) p[c] = e[j];
+            }
         }
     }
 }
-// sum over the threads of one row, the same value in all of them
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red, int tid) {
-    v = wave_sum(v);
-    if constexpr (TPR == 256) {
-        __syncthreads();
-        if ((tid & 63) == 0) red[tid >> 6] = v;
-        __syncthreads();
-        v = (red[0] + red[1]) + (red[2] + red[3]);
-    }
-    return v;
-}
-template <int TPR> __device__ __forceinline__ void row_sum2(float& u, float& v, float* red, int tid) {
+// two sums over the threads of one row, the same values in all of them; `red`: 2 TPR / 64 floats
+template <int TPR> __device__ __forceinline__ void row_sum(float& u, float& v, float* red, int tid) {
     u = wave_sum(u);
     v = wave_sum(v);
-    if constexpr (TPR == 256) {
+    if constexpr (TPR > 64) {
+        constexpr int NW = TPR / 64;
         __syncthreads();
-        if ((tid & 63) == 0) { red[tid >> 6] = u; red[4 + (tid >> 6)] = v; }
+        if ((tid & 63) == 0) { red[tid >> 6] = u; red[NW + (tid >> 6)] = v; }
         __syncthreads();
-        u = (red[0] + red[1]) + (red[2] + red[3]);
-        v = (red[4] + red[5]) + (red[6] + red[7]);
+        u = v = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) { u += red[i]; v += red[NW + i]; }
     }
+}
+template <int TPR> __device__ __forceinline__ float row_sum(float u, float* red, int tid) {
+    u = wave_sum(u);
+    if constexpr (TPR > 64) {
+        __syncthreads();
+        if ((tid & 63) == 0) red[tid >> 6] = u;
+        __syncthreads();
+        u = 0.f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) u += red[i];
+    }
+    return u;
 }
 template <int TPR> __device__ __forceinline__ double row_max(double v, double* red, int tid) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
-    if constexpr (TPR == 256) {
+    if constexpr (TPR > 64) {
         __syncthreads();
         if ((tid & 63) == 0) red[tid >> 6] = v;
         __syncthreads();
-        v = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < TPR / 64; ++i) v = fmax(v, red[i]);
     }
     return v;
 }
 
 template <class E, int V, int TPR, bool Q8, bool NORM>
-__global__ __launch_bounds__(256) void norm_fwd_kernel(const NormArgs g) {
-    constexpr int VE = 16 / sizeof(E);
-    __shared__ double redd[4];
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const NormArgs g) {
+    constexpr int VE = 16 / sizeof(E), NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
+    __shared__ double redd[NT / 64];
     float* red = reinterpret_cast<float*>(redd);
     const int tid = threadIdx.x, t = tid % TPR;
-    const long long row = (long long)blockIdx.x * (256 / TPR) + tid / TPR;
-    if (row >= g.M) return;                               // (whole waves; with TPR = 256 there is no such workgroup)
-    float h[V * VE], r[V * VE];
-    row_load<E, VE, V, TPR>((const E*)g.x + row * g.xs, g.N, g.vec, t, h);
-    if (g.res) row_load<E, VE, V, TPR>((const E*)g.res + row * g.rs, g.N, g.vec, t, r);
-    else {
+    float wv[V * VE];
+    if (NORM) load_weight<VE, V, TPR>(g.w, g.N, g.vec, t, wv);
+    Raw<E, VE, V, TPR> x, r;
+    const long long step = (long long)gridDim.x * RPW;
+    long long row = (long long)blockIdx.x * RPW + tid / TPR;
+    auto fetch = [&](long long at) {
+        x.load((const E*)g.x + at * g.xs, g.N, g.vec, t);
+        if (g.res) r.load((const E*)g.res + at * g.rs, g.N, g.vec, t);
+    };
+    if (row < g.M) fetch(row);
+    for (; row < g.M; row += step) {                       // (the same for all threads of a row, and of a workgroup whose waves meet)
+        float h[V * VE];
+        double hd[Q8 ? V * VE : 1];
 #pragma unroll
-        for (int i = 0; i < V * VE; ++i) r[i] = 0.f;
-    }
-    float ss = 0.f;
-    if constexpr (!Q8) {
+        for (int i = 0; i < V * VE; ++i) {
+            const float u = x.get(i), v = g.res ? r.get(i) : 0.f;
+            h[i] = u + v;
+            if (Q8) hd[i] = (double)u + (double)v;
+        }
+        if (row + step < g.M) fetch(row + step);
+        float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < V * VE; ++i) { h[i] += r[i]; ss += h[i] * h[i]; }
+        for (int i = 0; i < V * VE; ++i) ss += h[i] * h[i];
         if (g.sum) row_store<E, VE, V, TPR>((E*)g.sum + row * g.ss, g.N, g.vec, t, h);
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)g.N + g.eps);
+        if constexpr (!Q8) {
+            const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)g.N + g.eps);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * VE;
+            for (int i = 0; i < V * VE; ++i) h[i] *= rstd * wv[i];
+            row_store<E, VE, V, TPR>((E*)g.y + row * g.ys, g.N, g.vec, t, h);
+        } else {
+            double most = 0;
 #pragma unroll
-            for (int j = 0; j < VE; ++j) h[v * VE + j] *= rstd * (c + j < g.N ? g.w[c + j] : 0.f);
-        }
-        row_store<E, VE, V, TPR>((E*)g.y + row * g.ys, g.N, g.vec, t, h);
-    } else {
-        double most = 0;
-        float wv[V * VE];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * VE;
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                const int i = v * VE + j;
-                wv[i] = NORM ? (c + j < g.N ? g.w[c + j] : 0.f) : 1.f;
-                const double d = (double)h[i] + (double)r[i];
-                ss += (float)d * (float)d;
-                most = fmax(most, fabs(d * (double)wv[i]));
+            for (int i = 0; i < V * VE; ++i) {
+                if (NORM) hd[i] *= (double)wv[i];
+                most = fmax(most, fabs(hd[i]));
             }
-        }
-        if (g.sum) {
-            float s[V * VE];
+            ss = row_sum<TPR>(ss, red, tid);
+            most = row_max<TPR>(most, redd, tid);
+            const bool fine = ss < INFINITY && most < (double)INFINITY;      // (false for NaN)
+            const double to = fine && most > 0 ? 127.0 / most : 0.0;
+            if (t == 0) g.scale[row] = fine ? (float)(most * (NORM ? 1.0 / sqrt((double)ss / g.N + (double)g.eps) : 1.0) / 127.0) : NAN;
+            signed char* q = g.q + row * g.qs;
 #pragma unroll
-            for (int i = 0; i < V * VE; ++i) s[i] = h[i] + r[i];
-            row_store<E, VE, V, TPR>((E*)g.sum + row * g.ss, g.N, g.vec, t, s);
-        }
-        ss = row_sum<TPR>(ss, red, tid);
-        most = row_max<TPR>(most, redd, tid);
-        const bool fine = ss < INFINITY && most < (double)INFINITY;      // (false for NaN)
-        const double to = fine && most > 0 ? 127.0 / most : 0.0;
-        if (t == 0) g.scale[row] = fine ? (float)(most * (NORM ? 1.0 / sqrt((double)ss / g.N + (double)g.eps) : 1.0) / 127.0) : NAN;
-        signed char* q = g.q + row * g.qs;
+            for (int v = 0; v < V; ++v) {
+                signed char e[VE];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * VE;
-            signed char e[VE];
+                for (int j = 0; j < VE; ++j) e[j] = fine ? (signed char)(int)rint(hd[v * VE + j] * to) : 0;
+                if (g.vec) {
+                    const int c = (v * TPR + t) * VE;
+                    if (c < g.N) __builtin_memcpy(q + c, e, VE);
+                } else {
 #pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                const int i = v * VE + j;
-                e[j] = fine ? (signed char)(int)rint(((double)h[i] + (double)r[i]) * (double)wv[i] * to) : 0;
-            }
-            if (g.vec) {
-                if (c < g.N) __builtin_memcpy(q + c, e, VE);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VE; ++j)
-                    if (c + j < g.N) q[c + j] = e[j];
+                    for (int j = 0; j < VE; ++j) {
+                        const int c = (v * VE + j) * TPR + t;
+                        if (c < g.N) q[c] = e[j];
+                    }
+                }
             }
         }
     }
@@ -272,123 +317,127 @@ struct NormBwdArgs {
     float eps;
 };
 template <class E, int V, int TPR>
-__global__ __launch_bounds__(256) void norm_bwd_kernel(const NormBwdArgs g) {
-    constexpr int VE = 16 / sizeof(E), RPW = 256 / TPR;
-    __shared__ float red[8];
-    __shared__ float cols[RPW > 1 ? RPW * V * TPR * VE : 1];
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(const NormBwdArgs g) {
+    constexpr int VE = 16 / sizeof(E), NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
+    __shared__ float red[NT / 32];
+    __shared__ float cols[RPW > 1 ? NT * V * VE : 1];
     const int tid = threadIdx.x, t = tid % TPR;
     float wv[V * VE], dw[V * VE];
+    load_weight<VE, V, TPR>(g.w, g.N, g.vec, t, wv);
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int i = 0; i < V * VE; ++i) dw[i] = 0.f;
+    Raw<E, VE, V, TPR> x, r, dy, ds;
+    const long long step = (long long)gridDim.x * RPW;
+    long long row = (long long)blockIdx.x * RPW + tid / TPR;
+    auto fetch = [&](long long at) {
+        x.load((const E*)g.x + at * g.xs, g.N, g.vec, t);
+        if (g.res) r.load((const E*)g.res + at * g.rs, g.N, g.vec, t);
+        dy.load((const E*)g.dy + at * g.dys, g.N, g.vec, t);
+        if (g.dsum) ds.load((const E*)g.dsum + at * g.dss, g.N, g.vec, t);
+    };
+    if (row < g.M) fetch(row);
+    for (; row < g.M; row += step) {
+        float n[V * VE], d[V * VE], f[V * VE];
+        float ss = 0.f, dot = 0.f;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-            const int c = (v * TPR + t) * VE + j;
-            wv[v * VE + j] = c < g.N ? g.w[c] : 0.f;
-            dw[v * VE + j] = 0.f;
+        for (int i = 0; i < V * VE; ++i) {
+            n[i] = x.get(i) + (g.res ? r.get(i) : 0.f);
+            d[i] = dy.get(i);
+            f[i] = g.dsum ? ds.get(i) : 0.f;
+            ss += n[i] * n[i];
+            dot += d[i] * wv[i] * n[i];
         }
-    const long long per = (long long)gridDim.x * RPW;
-    for (long long row0 = (long long)blockIdx.x * RPW; row0 < g.M; row0 += per) {
-        const long long row = row0 + tid / TPR;
-        if (row < g.M) {                                  // (whole waves; TPR = 256: always)
-            float n[V * VE], d[V * VE], f[V * VE];
-            row_load<E, VE, V, TPR>((const E*)g.x + row * g.xs, g.N, g.vec, t, n);
-            if (g.res) row_load<E, VE, V, TPR>((const E*)g.res + row * g.rs, g.N, g.vec, t, f);
-            row_load<E, VE, V, TPR>((const E*)g.dy + row * g.dys, g.N, g.vec, t, d);
-            if (g.res) {
+        if (row + step < g.M) fetch(row + step);
+        row_sum<TPR>(ss, dot, red, tid);
+        const float rstd = 1.f / sqrtf(ss / (float)g.N + g.eps);
+        dot *= rstd / (float)g.N;
 #pragma unroll
-                for (int i = 0; i < V * VE; ++i) n[i] += f[i];
-            }
-            if (g.dsum) row_load<E, VE, V, TPR>((const E*)g.dsum + row * g.dss, g.N, g.vec, t, f);
-            float ss = 0.f, dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < V * VE; ++i) {
-                ss += n[i] * n[i];
-                dot += d[i] * wv[i] * n[i];
-            }
-            row_sum2<TPR>(ss, dot, red, tid);
-            const float rstd = 1.f / sqrtf(ss / (float)g.N + g.eps);
-            dot *= rstd / (float)g.N;
-#pragma unroll
-            for (int i = 0; i < V * VE; ++i) {
-                n[i] *= rstd;
-                dw[i] += d[i] * n[i];
-                d[i] *= wv[i];
-            }
-#pragma unroll
-            for (int i = 0; i < V * VE; ++i) d[i] = rstd * (d[i] - n[i] * dot) + (g.dsum ? f[i] : 0.f);
-            row_store<E, VE, V, TPR>((E*)g.dx + row * g.dxs, g.N, g.vec, t, d);
+        for (int i = 0; i < V * VE; ++i) {
+            n[i] *= rstd;
+            dw[i] += d[i] * n[i];
+            d[i] = rstd * (d[i] * wv[i] - n[i] * dot) + f[i];
         }
+        row_store<E, VE, V, TPR>((E*)g.dx + row * g.dxs, g.N, g.vec, t, d);
     }
+    float* part = g.part + (long long)blockIdx.x * g.N;
     if constexpr (RPW > 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int j = 0; j < VE; ++j) cols[(tid / TPR) * V * TPR * VE + (v * TPR + t) * VE + j] = dw[v * VE + j];
+        for (int i = 0; i < V * VE; ++i) cols[(tid / TPR) * V * TPR * VE + column<VE, TPR>(i, t, g.vec)] = dw[i];
         __syncthreads();
-        for (int c = tid; c < g.N; c += 256) {
+        for (int c = tid; c < g.N; c += NT) {
             float s = 0.f;
 #pragma unroll
-            for (int r = 0; r < RPW; ++r) s += cols[r * V * TPR * VE + c];
-            g.part[(long long)blockIdx.x * g.N + c] = s;
+            for (int k = 0; k < RPW; ++k) s += cols[k * V * TPR * VE + c];
+            part[c] = s;
         }
     } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                const int c = (v * TPR + t) * VE + j;
-                if (c < g.N) g.part[(long long)blockIdx.x * g.N + c] = dw[v * VE + j];
-            }
+        for (int i = 0; i < V * VE; ++i) {
+            const int c = column<VE, TPR>(i, t, g.vec);
+            if (c < g.N) part[c] = dw[i];
+        }
     }
 }
-// column sums of the workgroups' partial rows, in a fixed order
+// column sums of the workgroups' partial rows, in a fixed order: 16 columns (64 bytes) a workgroup, so that a narrow weight still fills some of the chip
 __global__ __launch_bounds__(1024) void norm_dw_kernel(const float* __restrict__ part, int n, int N, float* __restrict__ dw) {
-    __shared__ float red[16][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
+    __shared__ float red[64][17];
+    const int x = threadIdx.x & 15, c = blockIdx.x * 16 + x, y = threadIdx.x >> 4;
     float s = 0.f;
-    if (c < N)
-        for (int i = y; i < n; i += 16) s += part[(long long)i * N + c];
-    red[y][threadIdx.x & 63] = s;
+    if (c < N) {
+        float a[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int i = y; i < n; i += 512) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + k * 64 < n) a[k] += part[(long long)(i + k * 64) * N + c];
+        }
+        s = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+    }
+    red[y][x] = s;
     __syncthreads();
     if (y == 0 && c < N) {
         s = 0.f;
-        for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
+        for (int i = 0; i < 64; ++i) s += red[i][x];
         dw[c] = s;
     }
 }
 
 bool al(const void* p, long long stride, int bytes, int e) { return (uintptr_t)p % bytes == 0 && (stride * e) % bytes == 0; }
 
+// Threads of a row, so that its values stay in registers: a wave up to 128 vectors of 16 bytes (1024 bfloat16 / 512 float32 features), a workgroup of 256
+// up to 512, 512 up to 2048 (with four vectors a thread), 1024 for the widest.  Workgroups walk rows: the next row is in flight and the weight stays.  16384 x
+// 4096 bfloat16 with a residual: forward 88 us at 1024 workgroups, 93 at 2048, 156 with one a row; backward (512; 768: 149, 1024: 142 + 15 for dw) 144 us.
+#define NORM_ROWS(GO)                              \
+    do {                                           \
+        if (N <= 64 * VE) GO(1, 64);               \
+        else if (N <= 128 * VE) GO(2, 64);         \
+        else if (N <= 256 * VE) GO(1, 256);        \
+        else if (N <= 512 * VE) GO(2, 256);        \
+        else if (N <= 1024 * VE) GO(2, 512);       \
+        else if (N <= 2048 * VE) GO(4, 512);       \
+        else if constexpr (VE == 4) GO(4, 1024);   \
+    } while (0)
+
 template <class E, bool Q8, bool NORM>
 void fwd_launch(const NormArgs& g, hipStream_t st) {
     constexpr int VE = 16 / sizeof(E);
     const int N = g.N;
-#define ROWS64(V) hipLaunchKernelGGL((norm_fwd_kernel<E, V, 64, Q8, NORM>), dim3((unsigned)((g.M + 3) / 4)), dim3(256), 0, st, g)
-#define ROWS256(V) hipLaunchKernelGGL((norm_fwd_kernel<E, V, 256, Q8, NORM>), dim3((unsigned)g.M), dim3(256), 0, st, g)
-    if (N <= 64 * VE) ROWS64(1);
-    else if (N <= 128 * VE) ROWS64(2);
-    else if (N <= 512 * VE) ROWS256(2);
-    else if (N <= 1024 * VE) ROWS256(4);
-    else if (N <= 2048 * VE) ROWS256(8);
-    else ROWS256(16);
-#undef ROWS64
-#undef ROWS256
+    const long long rows = N <= 128 * VE ? (g.M + 3) / 4 : g.M;
+    const dim3 grid((unsigned)(rows < 1024 ? rows : 1024));
+#define GO(V, T) hipLaunchKernelGGL((norm_fwd_kernel<E, V, T, Q8, NORM>), grid, dim3(T > 256 ? T : 256), 0, st, g)
+    NORM_ROWS(GO);
+#undef GO
 }
 int bwd_groups(long long M, int N, int VE) {
     const long long rows = N <= 128 * VE ? (M + 3) / 4 : M;
-    return (int)(rows < 512 ? rows : 512);
+    const int most = N <= 128 * VE ? 256 : 512;
+    return (int)(rows < most ? rows : most);
 }
 template <class E>
 void bwd_launch(const NormBwdArgs& g, hipStream_t st) {
     constexpr int VE = 16 / sizeof(E);
     const int N = g.N, n = bwd_groups(g.M, N, VE);
-#define GO(V, T) hipLaunchKernelGGL((norm_bwd_kernel<E, V, T>), dim3(n), dim3(256), 0, st, g)
-    if (N <= 64 * VE) GO(1, 64);
-    else if (N <= 128 * VE) GO(2, 64);
-    else if (N <= 512 * VE) GO(2, 256);
-    else if (N <= 1024 * VE) GO(4, 256);
-    else if (N <= 2048 * VE) GO(8, 256);
-    else GO(16, 256);
+#define GO(V, T) hipLaunchKernelGGL((norm_bwd_kernel<E, V, T>), dim3(n), dim3(T > 256 ? T : 256), 0, st, g)
+    NORM_ROWS(GO);
 #undef GO
 }
 constexpr int NORM_MAX = 16384;
@@ -415,21 +464,22 @@ extern "C" int srvp_rotary(const srvp_rotary_desc* d, void* stream) {
     g.pos = (const long long*)d->positions; g.pt = d->pos_t; g.pb = d->pos_b; g.freq = d->freq;
     g.T = d->T; g.B = d->B; g.H0 = d->Hq; g.H1 = d->Hk; g.D = d->D; g.n = d->pairs; g.inter = d->interleaved;
     g.sign = d->back ? -1.f : 1.f; g.mult = d->magnitude;
-    const int n = d->pairs > 0 ? d->pairs : 1;
-    int R = 256 / n;                                      // one sine and cosine a thread, ..
-    if (R > 16) R = 16;
+    // rows a workgroup: at least one sine and cosine a thread, and about four 16-byte items a thread
+    const int n = d->pairs > 0 ? d->pairs : 1, H = d->Hq + d->Hk;
+    long long R = (256 + n - 1) / n, most = 16384LL / ((long long)H * d->D * e) + 1;
+    if (R > most) R = most;
+    if (R * n > ROT_TAB) R = ROT_TAB / n;
     if (R < 1) R = 1;
-    g.R = R;
+    g.R = (int)R;
+    const int first = !vec ? d->pairs : d->interleaved ? 2 * d->pairs / ve : d->pairs / ve, items = first + (d->D - 2 * d->pairs) / (vec ? ve : 1);
     const long long grid = (rows + R - 1) / R;
-    SRVP_REQUIRE(grid < (1LL << 31) && (long long)R * (d->Hq + d->Hk) * d->D < (1LL << 31), "srvp_rotary: too many rows or heads");
+    SRVP_REQUIRE(rows < (1LL << 31) && R * H * items < (1LL << 30), "srvp_rotary: too many rows or heads");
+    g.dB = divide(d->B); g.dn = divide(n); g.dH = divide(H); g.ditems = divide(items);
     hipStream_t st = (hipStream_t)stream;
-    if (d->elem_f32) {
-        if (vec) hipLaunchKernelGGL((rotary_kernel<float, 4, true>), dim3((unsigned)grid), dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((rotary_kernel<float, 4, false>), dim3((unsigned)grid), dim3(256), 0, st, g);
-    } else {
-        if (vec) hipLaunchKernelGGL((rotary_kernel<bf16_t, 8, true>), dim3((unsigned)grid), dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((rotary_kernel<bf16_t, 8, false>), dim3((unsigned)grid), dim3(256), 0, st, g);
-    }
+#define ROTARY(E, VE, MODE) hipLaunchKernelGGL((rotary_kernel<E, VE, MODE>), dim3((unsigned)grid), dim3(256), 0, st, g)
+    if (d->elem_f32) { if (!vec) ROTARY(float, 4, SINGLE); else if (d->interleaved) ROTARY(float, 4, PAIRS); else ROTARY(float, 4, HALVES); }
+    else { if (!vec) ROTARY(bf16_t, 8, SINGLE); else if (d->interleaved) ROTARY(bf16_t, 8, PAIRS); else ROTARY(bf16_t, 8, HALVES); }
+#undef ROTARY
     SRVP_CHECK_LAUNCH("srvp_rotary");
     return SRVP_OK;
 }
@@ -478,7 +528,7 @@ extern "C" int srvp_rms_norm_bwd(const srvp_rms_norm_bwd_desc* d, void* stream) 
     hipStream_t st = (hipStream_t)stream;
     if (d->elem_f32) bwd_launch<float>(g, st); else bwd_launch<bf16_t>(g, st);
     SRVP_CHECK_LAUNCH("srvp_rms_norm_bwd");
-    hipLaunchKernelGGL(norm_dw_kernel, dim3((d->N + 63) / 64), dim3(1024), 0, st, (const float*)d->ws, bwd_groups(d->M, d->N, ve), d->N, d->dw);
+    hipLaunchKernelGGL(norm_dw_kernel, dim3((d->N + 15) / 16), dim3(1024), 0, st, (const float*)d->ws, bwd_groups(d->M, d->N, ve), d->N, d->dw);
     SRVP_CHECK_LAUNCH("srvp_rms_norm_bwd(weight)");
     return SRVP_OK;
 }

@@ -394,7 +394,8 @@ def test_rms_norm_int8(M, N, dt):
     within(s[~bad], rs, rs, FP, 2.0 ** -24, 'plain scale')
 
 
-GEMM8 = [(1, 1, 1), (1, 16, 4), (3, 17, 5), (7, 4096, 4096), (16, 64, 128), (33, 65, 129), (128, 128, 128), (130, 1001, 77), (257, 192, 260), (512, 512, 512), (1000, 333, 300), (5, 20000, 40)]
+GEMM8 = [(1, 1, 1), (1, 16, 4), (3, 17, 5), (7, 4096, 4096), (16, 64, 128), (33, 65, 129), (128, 128, 128), (130, 1001, 77), (257, 192, 260), (512, 512, 512), (1000, 333, 300), (5, 20000, 40),
+         (40, 1000, 500), (64, 1040, 90), (17, 80, 33), (2000, 144, 2100), (1500, 48, 1500), (4000, 208, 4100), (3000, 65, 3100)]
 
 
 @pytest.mark.parametrize('M,K,N', GEMM8)
