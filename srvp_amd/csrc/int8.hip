@@ -11,7 +11,7 @@ struct Int8Args {
     const float *xs, *ws, *bias;
     void* y;
     long long ldx, ldw, ldy;
-    int M, N, K, vecy;
+    int M, N, K, vecy, vecy16;      // 4 outputs / 16 bytes of them may be stored together
 };
 
 // 16 bytes of row `p` from byte k on, zero behind K (rows may start at any byte)
@@ -32,13 +32,23 @@ __device__ __forceinline__ void put4(bf16_t* p, const f32x4_t& v) { *reinterpret
 __device__ __forceinline__ void put4(float* p, const f32x4_t& v) { *reinterpret_cast<f32x4_t*>(p) = v; }
 
 // W is the left operand of every product, so that a lane holds 4 neighbouring columns of one row of y.
-template <class E> __device__ __forceinline__ void finish(const Int8Args& g, int m, int n, const int* acc) {
+struct Cols { f32x4_t ws, bias; };
+__device__ __forceinline__ Cols cols_of(const Int8Args& g, int n) {
+    Cols c;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int at = min(n + r, g.N - 1);
+        c.ws[r] = g.ws[at];
+        c.bias[r] = g.bias ? g.bias[at] : 0.f;
+    }
+    return c;
+}
+template <class E> __device__ __forceinline__ void finish(const Int8Args& g, int m, int n, float xs, const Cols& c, const int* acc) {
     if (m >= g.M) return;
-    const float xs = g.xs[m];
     E* y = (E*)g.y + (long long)m * g.ldy + n;
     f32x4_t o;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = n + r < g.N ? (float)acc[r] * xs * g.ws[n + r] + (g.bias ? g.bias[n + r] : 0.f) : 0.f;
+    for (int r = 0; r < 4; ++r) o[r] = (float)acc[r] * xs * c.ws[r] + c.bias[r];
     if (g.vecy) {
         if (n < g.N) put4(y, o);
     } else {
@@ -60,11 +70,11 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned tm, unsigned tn, u
 __device__ __align__(16) signed char zero16[16];
 
 // BM x BN outputs a workgroup of WM x WN waves; rows 16-byte aligned, K a multiple of 16.  Four LDS stages of 64 bytes of k are filled by LDS-DMA three ahead
-// of the products; 16-byte chunks are exchanged (chunk ^= (row >> 1) & 3, on the global side: the LDS side of a DMA is linear) so that 8 rows of one chunk lie
-// on all 32 banks.  One barrier a stage: behind it every wave has both stage i (its own loads waited for) and left the buffer of stage i + 3.
-template <class E, int BM, int BN, int WM, int WN>
+// of the products; 16-byte chunks are exchanged (chunk ^= (row >> 2) & 3, on the global side: the LDS side of a DMA is linear) so that 16 rows of one chunk lie
+// on all 64 banks.  One barrier a stage: behind it every wave has both stage i (its own loads waited for) and left the buffer of stage i + 3.
+template <class E, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64, 2) void int8_dma_kernel(const Int8Args g) {
-    constexpr int NT = WM * WN * 64, BK = 64, STAGES = 4, MT = BM / WM / 32, NTL = BN / WN / 32, LA = BM * 4 / NT, LW = BN * 4 / NT;
+    constexpr int NT = WM * WN * 64, BK = 64, MT = BM / WM / 32, NTL = BN / WN / 32, LA = BM * 4 / NT, LW = BN * 4 / NT;
     typedef int i32x16_t __attribute__((ext_vector_type(16)));
     typedef __attribute__((address_space(1))) const void* gptr_t;
     typedef __attribute__((address_space(3))) void* lptr_t;
@@ -81,19 +91,19 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_dma_kernel(const Int8Arg
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
         const int row = (i * NT + tid) >> 2;
-        kx[i] = (chunk ^ ((row >> 1) & 3)) * 16;
+        kx[i] = (chunk ^ ((row >> 2) & 3)) * 16;
         px[i] = g.x + (long long)min(m0 + row, g.M - 1) * g.ldx + kx[i];
     }
 #pragma unroll
     for (int i = 0; i < LW; ++i) {
         const int row = (i * NT + tid) >> 2;
-        kw[i] = (chunk ^ ((row >> 1) & 3)) * 16;
+        kw[i] = (chunk ^ ((row >> 2) & 3)) * 16;
         pw[i] = g.w + (long long)min(n0 + row, g.N - 1) * g.ldw + kw[i];
     }
     const int steps = (g.K + BK - 1) / BK;
     auto issue = [&](int s) {
         const int k0 = s * BK;
-        signed char* lx = lds + (s & (STAGES - 1)) * (BM + BN) * BK;
+        signed char* lx = lds + (s % STAGES) * (BM + BN) * BK;
         signed char* lw = lx + BM * BK;
 #pragma unroll
         for (int i = 0; i < LA; ++i)
@@ -110,22 +120,20 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_dma_kernel(const Int8Arg
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
     // byte offset of the lane's chunk of k step ks in row l32 (+ 32 t: the same exchange)
-    const int sw = (l32 >> 1) & 3;
+    const int sw = (l32 >> 2) & 3;
     const int off[2] = {l32 * BK + ((half ^ sw) << 4), l32 * BK + (((2 + half) ^ sw) << 4)};
-    issue(0);
-    if (steps > 1) issue(1);
-    if (steps > 2) issue(2);
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+        if (s < steps) issue(s);
     for (int s = 0; s < steps; ++s) {
-        // stage s has landed: all but the loads of the stages behind it (at most two)
-        const int behind = min(steps - 1 - s, 2);
-        // (lgkmcnt: this wave's reads of the stage before it are back, so its buffer may be filled again)
-        if (behind == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * (LA + LW)) : "memory");
-        else if (behind == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LA + LW) : "memory");
+        // stage s has landed: all but the loads of the stages behind it; and this wave's reads of the stage before it are back, so its buffer may be filled again
+        if (steps - 1 - s >= STAGES - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * (LA + LW)) : "memory");
+        else if (STAGES == 4 && steps - 1 - s == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LA + LW) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 3 < steps) issue(s + 3);
-        const signed char* lx = lds + (s & (STAGES - 1)) * (BM + BN) * BK;
+        if (s + STAGES - 1 < steps) issue(s + STAGES - 1);
+        const signed char* lx = lds + (s % STAGES) * (BM + BN) * BK;
         const signed char* lw = lx + BM * BK;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -140,15 +148,55 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_dma_kernel(const Int8Arg
                 for (int j = 0; j < NTL; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
         }
     }
+    float xs[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) xs[i] = g.xs[min(m0 + wm + i * 32 + l32, g.M - 1)];
+    if (g.vecy16) {
+        // whole lines: a wave passes 32 rows at a time through its own part of LDS and stores 16 bytes a lane along the rows (4 columns a lane straight from
+        // the registers write a quarter of 32 lines at a time)
+        constexpr int CW = NTL * 32, LDE = CW + 16 / sizeof(E), VE = 16 / sizeof(E), PER = CW / VE;
+        static_assert(WM * WN * 32 * LDE * (int)sizeof(E) <= STAGES * (BM + BN) * BK, "the rows fit the stages' memory");
+        __syncthreads();
+        E* my = reinterpret_cast<E*>(lds) + wid * 32 * LDE;
+        Cols c[NTL][4];
 #pragma unroll
         for (int j = 0; j < NTL; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int a[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                finish<E>(g, m0 + wm + i * 32 + l32, n0 + wn + j * 32 + 8 * q + 4 * half, a);
+            for (int q = 0; q < 4; ++q) c[j][q] = cols_of(g, n0 + wn + j * 32 + 8 * q + 4 * half);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+            for (int j = 0; j < NTL; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    f32x4_t o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = (float)acc[i][j][4 * q + r] * xs[i] * c[j][q].ws[r] + c[j][q].bias[r];
+                    put4(my + l32 * LDE + j * 32 + 8 * q + 4 * half, o);
+                }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < 32 * PER / 64; ++k) {
+                const int at = k * 64 + lane, row = at / PER, n = n0 + wn + (at % PER) * VE, m = m0 + wm + i * 32 + row;
+                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(my + row * LDE + (at % PER) * VE);
+                if (m < g.M && n < g.N) *reinterpret_cast<u32x4_t*>((E*)g.y + (long long)m * g.ldy + n) = v;
             }
+            __builtin_amdgcn_wave_barrier();
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < NTL; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = n0 + wn + j * 32 + 8 * q + 4 * half;
+            const Cols c = cols_of(g, n);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int a[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                finish<E>(g, m0 + wm + i * 32 + l32, n, xs[i], c, a);
+            }
+        }
 }
 
 // BM x BN outputs a workgroup of 2 x 2 waves, rows at any byte: 64 bytes of k pass through registers, the next ones under the products.
@@ -204,13 +252,19 @@ __global__ __launch_bounds__(256, 2) void int8_tile_kernel(const Int8Args g) {
 #pragma unroll
             for (int j = 0; j < NTL; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
     }
+    float xs[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) xs[i] = g.xs[min(m0 + wm + i * 16 + ls, g.M - 1)];
 #pragma unroll
-        for (int j = 0; j < NTL; ++j) {
+    for (int j = 0; j < NTL; ++j) {
+        const int n = n0 + wn + j * 16 + lg * 4;
+        const Cols c = cols_of(g, n);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
             const int a[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-            finish<E>(g, m0 + wm + i * 16 + ls, n0 + wn + j * 16 + lg * 4, a);
+            finish<E>(g, m0 + wm + i * 16 + ls, n, xs[i], c, a);
         }
+    }
 }
 
 // Few rows (M <= 16 MT): the weight's bytes are the cost.  A workgroup owns 16 rows of w and all rows of x; its 8 waves deal the steps of 64 bytes of k among
@@ -221,6 +275,8 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(const Int8Args g) {
     __shared__ int red[8][MT * 4 * 64];
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
     const int n0 = blockIdx.x * 16;
+    const Cols c = cols_of(g, n0 + lg * 4);                  // (early: behind the sums they would be one more memory latency)
+    const float xs = wid < MT ? g.xs[min(wid * 16 + ls, g.M - 1)] : 0.f;
     const signed char* w = g.w + (long long)min(n0 + ls, g.N - 1) * g.ldw;
     const signed char* x[MT];
 #pragma unroll
@@ -258,7 +314,8 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(const Int8Args g) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) red[wid][(i * 4 + r) * 64 + lane] = acc[i][r];
     __syncthreads();
-    for (int i = wid; i < MT; i += 8) {
+    if (wid < MT) {
+        const int i = wid;
         int a[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -266,19 +323,25 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(const Int8Args g) {
 #pragma unroll
             for (int v = 0; v < 8; ++v) a[r] += red[v][(i * 4 + r) * 64 + lane];
         }
-        finish<E>(g, i * 16 + ls, n0 + lg * 4, a);
+        finish<E>(g, i * 16 + ls, n0 + lg * 4, xs, c, a);
     }
 }
 
-template <class E, int BM, int BN, int WM, int WN>
+template <class E, int BM, int BN, int WM, int WN, int STAGES>
 hipError_t dma_launch(const Int8Args& g, hipStream_t st) {
-    constexpr int bytes = 4 * (BM + BN) * 64;
-    const auto kern = int8_dma_kernel<E, BM, BN, WM, WN>;
+    constexpr int bytes = STAGES * (BM + BN) * 64;
+    const auto kern = int8_dma_kernel<E, BM, BN, WM, WN, STAGES>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3(((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN)), dim3(WM * WN * 64), bytes, st, g);
     return hipSuccess;
 }
+// Which kernel (K = N = 4096, bfloat16 out, us; x the chosen side):
+//   rows    7: x 6, 64 x 64 tiles 48    rows   64: x 7, 64 x 64 tiles 15     (up to 64 rows)
+//   rows  512: x 25 (64 x 64 tiles), 28 (128 x 128 by DMA)     rows 1024: x 30 (128 x 128 by DMA), 41 (64 x 64)     (by DMA from 192 tiles of 128 x 128 on)
+//   rows 3000: x 66 (256 x 256 by DMA), 84 (128 x 128)         rows 2048: x 49 (128 x 128), 61 (256 x 256)          (256 x 256 from 192 such tiles on)
+// 8192 x 4096 x 4096: 143 us = 1.92 P operations/s, 8192 x 8192 x 8192: 2.01 P/s; the dense peak is 5, and the large bfloat16 product of the vendor's library
+// reaches 56 % of its own here (the package's power limit).
 template <class E>
 hipError_t launch(const Int8Args& g, bool aligned, hipStream_t st) {
     const long long t256 = (long long)((g.M + 255) / 256) * ((g.N + 255) / 256), t128 = (long long)((g.M + 127) / 128) * ((g.N + 127) / 128);
@@ -295,8 +358,8 @@ hipError_t launch(const Int8Args& g, bool aligned, hipStream_t st) {
 #undef ROWS
         return hipSuccess;
     }
-    if (aligned && t256 >= 192) return dma_launch<E, 256, 256, 2, 4>(g, st);
-    if (aligned && t128 >= 128) return dma_launch<E, 128, 128, 2, 2>(g, st);
+    if (aligned && t256 >= 192) return dma_launch<E, 256, 256, 2, 4, 4>(g, st);
+    if (aligned && t128 >= 192) return dma_launch<E, 128, 128, 2, 2, 4>(g, st);
     if (!aligned && t128 >= 512) hipLaunchKernelGGL((int8_tile_kernel<E, 128, 128>), dim3((unsigned)t128), dim3(256), 0, st, g);
     else hipLaunchKernelGGL((int8_tile_kernel<E, 64, 64>), dim3((unsigned)(((g.M + 63) / 64) * ((g.N + 63) / 64))), dim3(256), 0, st, g);
     return hipSuccess;
@@ -316,6 +379,7 @@ extern "C" int srvp_linear_int8(const srvp_linear_int8_desc* d, void* stream) {
     g.x = (const signed char*)d->x; g.w = (const signed char*)d->w; g.xs = d->x_scale; g.ws = d->w_scale; g.bias = d->bias; g.y = d->y;
     g.ldx = d->ldx; g.ldw = d->ldw; g.ldy = d->ldy; g.M = d->M; g.N = d->N; g.K = d->K;
     g.vecy = (uintptr_t)d->y % (4 * e) == 0 && d->ldy % 4 == 0 && d->N % 4 == 0;
+    g.vecy16 = (uintptr_t)d->y % 16 == 0 && d->ldy * e % 16 == 0 && d->N * e % 16 == 0;
     SRVP_REQUIRE((long long)((d->M + 63) / 64) * ((d->N + 63) / 64) < (1LL << 30), "srvp_linear_int8: too many outputs (%d x %d)", d->M, d->N);
     const bool aligned = d->K % 16 == 0 && d->ldx % 16 == 0 && d->ldw % 16 == 0 && (uintptr_t)d->x % 16 == 0 && (uintptr_t)d->w % 16 == 0;
     const hipError_t err = d->out_f32 ? launch<float>(g, aligned, (hipStream_t)stream) : launch<bf16_t>(g, aligned, (hipStream_t)stream);
