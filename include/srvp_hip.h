@@ -594,6 +594,8 @@ typedef struct {
 int64_t srvp_linear_attention_ws_bytes(const srvp_linear_attention_desc* d, int32_t backward);
 int srvp_linear_attention_fwd(const srvp_linear_attention_desc* d, void* stream);
 int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* d, void* stream);
+/* *capturing = 1 while work on `stream` is being captured into a graph */
+int srvp_stream_is_capturing(void* stream, int* capturing);
 int srvp_linear_attention_step(const srvp_linear_attention_step_desc* d, void* stream);
 /* Rotary positions of q (T, B, Hq, D) and k (T, B, Hk, D; Hk = 0: none): pair p of every head -- features (2p, 2p + 1) if interleaved, (p, pairs + p)
  * otherwise -- is turned by positions[t][b] * freq[p] radians (back = 1: by the negative angle) and multiplied by `magnitude`; features from 2 * pairs on

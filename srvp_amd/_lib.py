@@ -83,6 +83,46 @@ class RolloutBwdDesc(C.Structure):
                 ('d_y0', c_vp), ('d_qz', c_vp), ('dhid_dyn', c_vp), ('dhid_pz', c_vp), ('work', c_vp), ('dinp_all', c_vp)]
 
 
+class LinearAttentionDesc(C.Structure):
+    _fields_ = [('q', c_vp), ('k', c_vp), ('v', c_vp), ('o', c_vp), ('qs', c_i64 * 3), ('ks', c_i64 * 3), ('vs', c_i64 * 3), ('os', c_i64 * 3),
+                ('log_decay', c_vp), ('state_in', c_vp), ('state_out', c_vp), ('lengths', c_vp), ('ws', c_vp), ('ws_bytes', c_i64),
+                ('T', c_i32), ('B', c_i32), ('H', c_i32), ('Dk', c_i32), ('Dv', c_i32), ('scale', c_f32), ('elem_f32', c_i32), ('reserved', c_i32)]
+
+
+class LinearAttentionBwdDesc(C.Structure):
+    _fields_ = [('f', LinearAttentionDesc), ('d_o', c_vp), ('dq', c_vp), ('dk', c_vp), ('dv', c_vp), ('d_os', c_i64 * 3), ('dqs', c_i64 * 3),
+                ('dks', c_i64 * 3), ('dvs', c_i64 * 3), ('d_state_out', c_vp), ('d_state_in', c_vp)]
+
+
+class LinearAttentionStepDesc(C.Structure):
+    _fields_ = [('q', c_vp), ('k', c_vp), ('v', c_vp), ('o', c_vp), ('qs', c_i64 * 2), ('ks', c_i64 * 2), ('vs', c_i64 * 2), ('os', c_i64 * 2),
+                ('log_decay', c_vp), ('state', c_vp), ('slots', c_vp),
+                ('B', c_i32), ('H', c_i32), ('Dk', c_i32), ('Dv', c_i32), ('nslots', c_i32), ('scale', c_f32), ('elem_f32', c_i32), ('reserved', c_i32)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [('q', c_vp), ('k', c_vp), ('oq', c_vp), ('ok', c_vp), ('qs', c_i64 * 3), ('ks', c_i64 * 3), ('oqs', c_i64 * 3), ('oks', c_i64 * 3),
+                ('positions', c_vp), ('pos_t', c_i64), ('pos_b', c_i64), ('freq', c_vp), ('T', c_i32), ('B', c_i32), ('Hq', c_i32), ('Hk', c_i32),
+                ('D', c_i32), ('pairs', c_i32), ('interleaved', c_i32), ('back', c_i32), ('magnitude', c_f32), ('elem_f32', c_i32)]
+
+
+class RmsNormDesc(C.Structure):
+    _fields_ = [('x', c_vp), ('residual', c_vp), ('w', c_vp), ('y', c_vp), ('sum', c_vp), ('q8', c_vp), ('scale', c_vp),
+                ('xs', c_i64), ('rs', c_i64), ('ys', c_i64), ('ss', c_i64), ('qs', c_i64), ('M', c_i64), ('N', c_i32), ('eps', c_f32),
+                ('elem_f32', c_i32), ('reserved', c_i32)]
+
+
+class RmsNormBwdDesc(C.Structure):
+    _fields_ = [('x', c_vp), ('residual', c_vp), ('d_y', c_vp), ('d_sum', c_vp), ('w', c_vp), ('dx', c_vp), ('dw', c_vp), ('ws', c_vp),
+                ('xs', c_i64), ('rs', c_i64), ('dys', c_i64), ('dss', c_i64), ('dxs', c_i64), ('M', c_i64), ('ws_bytes', c_i64), ('N', c_i32),
+                ('eps', c_f32), ('elem_f32', c_i32), ('reserved', c_i32)]
+
+
+class LinearInt8Desc(C.Structure):
+    _fields_ = [('x', c_vp), ('w', c_vp), ('x_scale', c_vp), ('w_scale', c_vp), ('bias', c_vp), ('y', c_vp), ('ldx', c_i64), ('ldw', c_i64),
+                ('ldy', c_i64), ('M', c_i32), ('N', c_i32), ('K', c_i32), ('out_f32', c_i32)]
+
+
 _SIGS = {
     'srvp_version': ([], c_i32),
     'srvp_stream_create_low_priority': ([C.POINTER(c_vp), C.POINTER(c_i32)], c_i32),
@@ -183,16 +223,16 @@ _SIGS = {
     'srvp_pad_f32': ([c_vp, c_vp, c_i64, c_i32, c_i32, c_vp], c_i32),
     'srvp_skip_grad_reduce_f32': ([c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp], c_i32),
     'srvp_frame_metrics': ([c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_f32, c_f32, c_f32, c_vp, c_vp, c_vp], c_i32),
-    # (descriptors of the temporal operators: packed bytes, srvp_amd/temporal.py)
-    'srvp_linear_attention_ws_bytes': ([C.c_char_p, c_i32], c_i64),
-    'srvp_linear_attention_fwd': ([C.c_char_p, c_vp], c_i32),
-    'srvp_linear_attention_bwd': ([C.c_char_p, c_vp], c_i32),
-    'srvp_linear_attention_step': ([C.c_char_p, c_vp], c_i32),
-    'srvp_rotary': ([C.c_char_p, c_vp], c_i32),
-    'srvp_rms_norm': ([C.c_char_p, c_vp], c_i32),
+    'srvp_stream_is_capturing': ([c_vp, C.POINTER(c_i32)], c_i32),
+    'srvp_linear_attention_ws_bytes': ([C.POINTER(LinearAttentionDesc), c_i32], c_i64),
+    'srvp_linear_attention_fwd': ([C.POINTER(LinearAttentionDesc), c_vp], c_i32),
+    'srvp_linear_attention_bwd': ([C.POINTER(LinearAttentionBwdDesc), c_vp], c_i32),
+    'srvp_linear_attention_step': ([C.POINTER(LinearAttentionStepDesc), c_vp], c_i32),
+    'srvp_rotary': ([C.POINTER(RotaryDesc), c_vp], c_i32),
+    'srvp_rms_norm': ([C.POINTER(RmsNormDesc), c_vp], c_i32),
     'srvp_rms_norm_bwd_ws_bytes': ([c_i64, c_i32, c_i32], c_i64),
-    'srvp_rms_norm_bwd': ([C.c_char_p, c_vp], c_i32),
-    'srvp_linear_int8': ([C.c_char_p, c_vp], c_i32),
+    'srvp_rms_norm_bwd': ([C.POINTER(RmsNormBwdDesc), c_vp], c_i32),
+    'srvp_linear_int8': ([C.POINTER(LinearInt8Desc), c_vp], c_i32),
     'srvp_skip_grad_reduce': ([c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp], c_i32),
 }
 

@@ -366,3 +366,12 @@ extern "C" int srvp_bn_stats_f32_det(const float* raw, int64_t rows, int C, doub
     SRVP_CHECK_LAUNCH("srvp_bn_stats_f32_det");
     return SRVP_OK;
 }
+
+extern "C" int srvp_stream_is_capturing(void* stream, int* capturing) {
+    SRVP_REQUIRE(capturing, "srvp_stream_is_capturing: null pointer");
+    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &s);
+    if (e != hipSuccess) { srvp_set_error("srvp_stream_is_capturing: %s", hipGetErrorString(e)); return SRVP_ERR_LAUNCH; }
+    *capturing = s != hipStreamCaptureStatusNone;
+    return SRVP_OK;
+}

@@ -2,7 +2,6 @@
 import ctypes as C
 import math
 import os
-import re
 import subprocess
 import tempfile
 
@@ -13,28 +12,35 @@ from srvp_amd import _lib as L
 from srvp_amd import temporal as t
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-STRUCTS = {'srvp_linear_attention_desc': t.ATTENTION, 'srvp_linear_attention_bwd_desc': t.ATTENTION_BWD, 'srvp_linear_attention_step_desc': t.STEP,
-           'srvp_rotary_desc': t.ROTARY, 'srvp_rms_norm_desc': t.NORM, 'srvp_rms_norm_bwd_desc': t.NORM_BWD, 'srvp_linear_int8_desc': t.INT8}
+STRUCTS = {'srvp_linear_attention_desc': L.LinearAttentionDesc, 'srvp_linear_attention_bwd_desc': L.LinearAttentionBwdDesc,
+           'srvp_linear_attention_step_desc': L.LinearAttentionStepDesc, 'srvp_rotary_desc': L.RotaryDesc, 'srvp_rms_norm_desc': L.RmsNormDesc,
+           'srvp_rms_norm_bwd_desc': L.RmsNormBwdDesc, 'srvp_linear_int8_desc': L.LinearInt8Desc}
 
 
-def test_packed_descriptors_match_the_header():
-    """Sizes, and that no padding lies between the fields (a packed string has none)."""
-    names = list(STRUCTS)
-    src = '#include <stdio.h>\n#include "srvp_hip.h"\nint main(void){' + ''.join(f'printf("%zu\\n", sizeof({n}));' for n in names) + 'return 0;}'
+def test_descriptors_match_the_header():
+    """Size and the offset of every field."""
+    src = '#include <stdio.h>\n#include <stddef.h>\n#include "srvp_hip.h"\nint main(void){'
+    mine = []
+    for name, s in STRUCTS.items():
+        src += f'printf("%zu ", sizeof({name}));' + ''.join(f'printf("%zu ", offsetof({name}, {f}));' for f, _ in s._fields_)
+        mine += [C.sizeof(s)] + [getattr(s, f).offset for f, _ in s._fields_]
     with tempfile.TemporaryDirectory() as d:
-        open(os.path.join(d, 'a.c'), 'w').write(src)
+        open(os.path.join(d, 'a.c'), 'w').write(src + 'return 0;}')
         subprocess.check_call(['gcc', '-I', os.path.join(ROOT, 'include'), os.path.join(d, 'a.c'), '-o', os.path.join(d, 'a')])
-        sizes = [int(x) for x in subprocess.check_output([os.path.join(d, 'a')]).split()]
-    assert sizes == [STRUCTS[n].size for n in names]
-    for s in STRUCTS.values():
-        assert s.size == sum(C.sizeof({'Q': C.c_uint64, 'q': C.c_int64, 'i': C.c_int32, 'f': C.c_float}[c]) * int(n or 1)
-                             for n, c in re.findall(r'(\d*)([Qqif])', s.format))
+        theirs = [int(x) for x in subprocess.check_output([os.path.join(d, 'a')]).split()]
+    assert theirs == mine
+
+
+def attention(T=8192, B=2, H=16, Dk=128, Dv=128, p=0, **kw):
+    d = L.LinearAttentionDesc(T=T, B=B, H=H, Dk=Dk, Dv=Dv, q=p, k=p, v=p, o=p, log_decay=p)
+    for k, v in dict(dict(scale=1.0), **kw).items():
+        setattr(d, k, v)
+    return d
 
 
 def test_workspace_sizes():
     """Long sequences of few heads are cut into segments (a state each); many heads and short sequences are not."""
-    def ws(T, B, H, backward, Dk=128, Dv=128, f32=0, scale=1.0):
-        return L.load().srvp_linear_attention_ws_bytes(t.ATTENTION.pack(*([0] * 20), 0, 0, T, B, H, Dk, Dv, scale, f32, 0), backward)
+    ws = lambda T, B, H, backward, **kw: L.load().srvp_linear_attention_ws_bytes(C.byref(attention(T, B, H, **kw)), backward)
     assert ws(12, 192, 4, 0) == 0 and ws(12, 192, 4, 1) == 0 and ws(64, 1, 1, 0) == 0 and ws(0, 1, 1, 0) == 0 and ws(4096, 0, 2, 0) == 0 and ws(4096, 2, 0, 1) == 0
     assert ws(8192, 2, 16, 0) % (2 * 16 * 128 * 128 * 4) == 0 and ws(8192, 2, 16, 0) > 0
     assert ws(8192, 2, 16, 1) % (2 * 2 * 16 * 128 * 128 * 4) == 0 and ws(8192, 2, 16, 1) > 0
@@ -44,18 +50,21 @@ def test_workspace_sizes():
 
 def test_c_entries_refuse_before_any_launch():
     """Null pointers, sizes and workspaces are turned into errors on the host."""
-    lib = L.load()
-    att = lambda ws=0, T=8192, D=128, p=0: t.ATTENTION.pack(*([p] * 4), *([0] * 12), p, 0, 0, 0, 0, ws, T, 1, 1, D, D, 1.0, 0, 0)
-    assert lib.srvp_linear_attention_fwd(att(), None) == 1
-    assert lib.srvp_linear_attention_fwd(att(p=16), None) == 1 and b'workspace' in lib.srvp_last_error()
-    assert lib.srvp_linear_attention_bwd(att(p=16) + bytes(t.ATTENTION_BWD.size - t.ATTENTION.size), None) == 1
-    assert lib.srvp_linear_attention_fwd(None, None) == 1 and lib.srvp_linear_attention_bwd(None, None) == 1 and lib.srvp_linear_attention_step(None, None) == 1
-    assert lib.srvp_linear_attention_step(t.STEP.pack(*([16] * 4), *([0] * 8), 16, 16, 0, 2, 1, 8, 8, 1, 1.0, 0, 0), None) == 1      # 2 rows, 1 state
-    assert lib.srvp_rotary(None, None) == 1 and lib.srvp_rms_norm(None, None) == 1 and lib.srvp_rms_norm_bwd(None, None) == 1 and lib.srvp_linear_int8(None, None) == 1
-    assert lib.srvp_rotary(t.ROTARY.pack(*([16] * 4), *([0] * 12), 16, 0, 0, 16, 1, 1, 1, 1, 8, 5, 0, 0, 1.0, 0), None) == 1           # 5 pairs of 8 features
-    assert lib.srvp_rms_norm(t.NORM.pack(*([16] * 7), *([0] * 5), 4, 20000, 0.0, 0, 0), None) == 1
-    assert lib.srvp_rms_norm_bwd(t.NORM_BWD.pack(*([16] * 8), *([0] * 5), 4, 0, 64, 0.0, 0, 0), None) == 1 and b'workspace' in lib.srvp_last_error()
-    assert lib.srvp_linear_int8(t.INT8.pack(*([16] * 6), 0, 0, 0, 1, 1, 200000, 1), None) == 1
+    lib, r = L.load(), C.byref
+    assert lib.srvp_linear_attention_fwd(r(attention()), None) == 1
+    assert lib.srvp_linear_attention_fwd(r(attention(p=16)), None) == 1 and b'workspace' in lib.srvp_last_error()
+    assert lib.srvp_linear_attention_bwd(r(L.LinearAttentionBwdDesc(f=attention(p=16))), None) == 1
+    for f in (lib.srvp_linear_attention_fwd, lib.srvp_linear_attention_bwd, lib.srvp_linear_attention_step, lib.srvp_rotary, lib.srvp_rms_norm,
+              lib.srvp_rms_norm_bwd, lib.srvp_linear_int8):
+        assert f(None, None) == 1
+    two_rows = dict(q=16, k=16, v=16, o=16, log_decay=16, state=16, B=2, H=1, Dk=8, Dv=8, nslots=1, scale=1.0)
+    assert lib.srvp_linear_attention_step(r(L.LinearAttentionStepDesc(**two_rows)), None) == 1 and b'2 rows for 1' in lib.srvp_last_error()
+    five_pairs = dict(q=16, oq=16, positions=16, freq=16, T=1, B=1, Hq=1, D=8, pairs=5, magnitude=1.0)
+    assert lib.srvp_rotary(r(L.RotaryDesc(**five_pairs)), None) == 1
+    assert lib.srvp_rms_norm(r(L.RmsNormDesc(x=16, w=16, y=16, M=4, N=20000)), None) == 1
+    assert lib.srvp_rms_norm_bwd(r(L.RmsNormBwdDesc(x=16, d_y=16, w=16, dx=16, dw=16, ws=16, M=4, N=64)), None) == 1 and b'workspace' in lib.srvp_last_error()
+    wide = dict(x=16, w=16, x_scale=16, w_scale=16, y=16, M=1, N=1)
+    assert lib.srvp_linear_int8(r(L.LinearInt8Desc(K=200000, **wide)), None) == 1 and lib.srvp_linear_int8(r(L.LinearInt8Desc(K=0, **wide)), None) == 1
 
 
 def test_no_cpu_path():
