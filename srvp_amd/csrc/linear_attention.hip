@@ -81,10 +81,10 @@ template <> struct Ty<bf16_t> {
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, const f32x4_t& c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
     }
-    // x * w as a sum of three bf16 values of 8 significant bits each: the fp32 product to its last bit, so the state (a result of its own) has fp32's
-    // accuracy.  Two terms (2^-17) would save 5 % of a long sequence's time, but outputs would then depend on whether the state was asked for.
-    static constexpr int SPLIT = 3;
-    static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) {
+    // x * w as a sum of SPLIT bf16 values of 8 significant bits each.  Three are the fp32 product to its last bit, so the state (a result of its own) has fp32's
+    // accuracy.  Two (2^-17) serve the gradients' sums, which only pass into bfloat16 values; the forward pass takes three always, or its output would
+    // depend on whether the state was asked for.
+    template <int SPLIT> static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) {
         float f[8];
         unpack8(__builtin_bit_cast(u32x4_t, x), f);
 #pragma unroll
@@ -151,8 +151,7 @@ template <> struct Ty<float> {
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
         return c;
     }
-    static constexpr int SPLIT = 1;
-    static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) { out[0] = frag{x[0] * w[0], x[1] * w[1], x[2] * w[2], x[3] * w[3]}; }
+    template <int SPLIT> static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) { out[0] = frag{x[0] * w[0], x[1] * w[1], x[2] * w[2], x[3] * w[3]}; }
 };
 template <int W> struct View<float, W> {
     typedef f32x4_t frag;
@@ -222,11 +221,11 @@ template <class E, int W, bool VEC> struct Tile {
 // fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel).
 // A chunk: the three tiles go to LDS (the next chunk's loads are in flight meanwhile); the lower-triangular 16 x 16 tiles of the scores are dealt to the
 // waves and exchanged through LDS; then every wave forms its columns of the output and of the state.
-template <class E, int DA, int NCT, bool OUT, bool VEC>
+template <class E, int DA, int NCT, bool OUT, bool VEC, int SPLIT>
 __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanArgs g) {
     using Y = Ty<E>;
     typedef typename Y::frag frag;
-    constexpr int C = Y::C, KS = Y::KS, TPK = Y::TPK, SPLIT = Y::SPLIT, CB = 64 * NCT, ND = DA / KS, NJ = C / KS, NTA = DA / 16, NTI = C / 16;
+    constexpr int C = Y::C, KS = Y::KS, TPK = Y::TPK, CB = 64 * NCT, ND = DA / KS, NJ = C / KS, NTA = DA / 16, NTI = C / 16;
     using VA = View<E, DA>;
     using VC = View<E, CB>;
     using VP = View<E, C>;
@@ -267,9 +266,17 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     if (tid <= C) pw[tid] = dpow(l2, tid);
     if (OUT) {
         // rows behind the sequence's last token: zero
-        const int cw = min(CB, dc - col0);
-        for (int t = max(t0, n); t < te; ++t)
-            for (int c = tid; c < cw; c += 256) put(po + t * r.ot + col0 + c, 0.f);
+        const int cw = min(CB, dc - col0), first = max(t0, n);
+        if (VEC) {
+            constexpr int PER = CB / 4;                    // (4 elements: what the output's alignment allows)
+            for (int i = tid; i < (te - first) * PER; i += 256) {
+                const int c = i % PER * 4;
+                if (c < cw) put4(po + (long long)(first + i / PER) * r.ot + col0 + c, f32x4_t{0, 0, 0, 0});
+            }
+        } else {
+            for (int t = first; t < te; ++t)
+                for (int c = tid; c < cw; c += 256) put(po + t * r.ot + col0 + c, 0.f);
+        }
         // scores above the diagonal tiles: zero, once
         for (int i = tid; i < VP::elems(C); i += 256) lp[i] = E(0);
     }
@@ -401,7 +408,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                 for (int x = 0; x < KS / 4; ++x) wt[x] = pw[max(0, mm - e - (j * KS + (x >> 2) * 16 + lg * 4 + (x & 3)))];     // (rows behind mm are zero)
                 frag wv[NCT][SPLIT];
 #pragma unroll
-                for (int ct = 0; ct < NCT; ++ct) Y::weigh(vf[j][ct], wt, wv[ct]);
+                for (int ct = 0; ct < NCT; ++ct) Y::template weigh<SPLIT>(vf[j][ct], wt, wv[ct]);
 #pragma unroll
                 for (int ta = 0; ta < NTA; ++ta) {
                     const frag kf = va.cols(lb, j * KS, ta);
@@ -604,23 +611,29 @@ void output(Role& r, void* p, const int64_t* s, int d, int f32) {
     r.ovec = aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, f32 ? 16 : 8);
 }
 
-template <class E, int DA, int NCT>
-void launch_one(const ScanArgs& g, bool out, bool vec, hipStream_t st) {
+template <class E, int DA, int NCT, int SPLIT>
+void launch_split(const ScanArgs& g, bool out, bool vec, hipStream_t st) {
     const dim3 grid((unsigned)g.nroles * g.B * g.nseg * g.H * g.ncb), wg(256);
     if (out) {
-        if (vec) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, true>), grid, wg, 0, st, g);
-        else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, false>), grid, wg, 0, st, g);
+        if (vec) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, true, SPLIT>), grid, wg, 0, st, g);
+        else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, false, SPLIT>), grid, wg, 0, st, g);
     } else {
-        if (vec) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false, true>), grid, wg, 0, st, g);
-        else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false, false>), grid, wg, 0, st, g);
+        if (vec) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false, true, SPLIT>), grid, wg, 0, st, g);
+        else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, false, false, SPLIT>), grid, wg, 0, st, g);
     }
+}
+template <class E, int DA, int NCT>
+void launch_one(const ScanArgs& g, bool out, bool vec, bool exact, hipStream_t st) {
+    if constexpr (sizeof(E) == 4) launch_split<E, DA, NCT, 1>(g, out, vec, st);
+    else if (exact) launch_split<E, DA, NCT, 3>(g, out, vec, st);
+    else launch_split<E, DA, NCT, 2>(g, out, vec, st);
 }
 int da_class(int da) { return da <= 64 ? 64 : da <= 128 ? 128 : 256; }
 int nct_of(int da, int dc) { return da <= 128 && dc > 64 ? 2 : 1; }       // (256 features of a: 64 columns a workgroup, or the state would not fit its registers)
 
 // Launches `n` roles; those that take the same kernel share a launch.
 template <class E>
-void launch(const ScanArgs& base, const Role* roles, int n, bool out, float* part, hipStream_t st) {
+void launch(const ScanArgs& base, const Role* roles, int n, bool out, bool exact, float* part, hipStream_t st) {
     bool done[3] = {false, false, false};
     for (int i = 0; i < n; ++i) {
         if (done[i]) continue;
@@ -637,9 +650,9 @@ void launch(const ScanArgs& base, const Role* roles, int n, bool out, float* par
         bool vec = true;                                  // 16-byte rows in and out
         for (int j = 0; j < g.nroles; ++j) vec = vec && g.r[j].b.vec && g.r[j].c.vec && (!out || (g.r[j].a.vec && g.r[j].ovec));
         g.part = part + (out ? 0 : (long long)i * g.B * g.H * g.nseg * roles[i].a.d * roles[i].c.d);
-        if (da == 64) { if (nct == 2) launch_one<E, 64, 2>(g, out, vec, st); else launch_one<E, 64, 1>(g, out, vec, st); }
-        else if (da == 128) { if (nct == 2) launch_one<E, 128, 2>(g, out, vec, st); else launch_one<E, 128, 1>(g, out, vec, st); }
-        else launch_one<E, 256, 1>(g, out, vec, st);
+        if (da == 64) { if (nct == 2) launch_one<E, 64, 2>(g, out, vec, exact, st); else launch_one<E, 64, 1>(g, out, vec, exact, st); }
+        else if (da == 128) { if (nct == 2) launch_one<E, 128, 2>(g, out, vec, exact, st); else launch_one<E, 128, 1>(g, out, vec, exact, st); }
+        else launch_one<E, 256, 1>(g, out, vec, exact, st);
     }
 }
 
@@ -648,7 +661,7 @@ void segments(const srvp_linear_attention_desc* d, int roles, int* nseg, int* se
     const int C = d->elem_f32 ? 32 : 64;
     const long long ncb = (d->Dv + 127) / 128, base = (long long)d->B * d->H * ncb * roles;
     const long long chunks = (d->T + C - 1) / C;
-    long long n = base >= 256 || base == 0 ? 1 : (512 + base - 1) / base;
+    long long n = base >= 256 || base == 0 ? 1 : 512 / base;
     if (n > (chunks + 3) / 4) n = (chunks + 3) / 4;
     if (n < 1) n = 1;
     const long long per = chunks > n ? (chunks + n - 1) / n : 1;
@@ -713,14 +726,14 @@ extern "C" int srvp_linear_attention_fwd(const srvp_linear_attention_desc* d, vo
     r.init_a = d->Dv; r.init_c = 1;
     if (g.nseg > 1) {
         float* part = (float*)d->ws;
-        if (d->elem_f32) launch<float>(g, &r, 1, false, part, st); else launch<bf16_t>(g, &r, 1, false, part, st);
+        if (d->elem_f32) launch<float>(g, &r, 1, false, true, part, st); else launch<bf16_t>(g, &r, 1, false, true, part, st);
         SRVP_CHECK_LAUNCH("srvp_linear_attention_fwd(segments)");
         const float* init[1] = {d->state_in};
         const float mul[1] = {1.f};
         if (int rc = run_join(g, d, 1, init, mul, part, st)) return rc;
         r.prefix = part;
     }
-    if (d->elem_f32) launch<float>(g, &r, 1, true, nullptr, st); else launch<bf16_t>(g, &r, 1, true, nullptr, st);
+    if (d->elem_f32) launch<float>(g, &r, 1, true, true, nullptr, st); else launch<bf16_t>(g, &r, 1, true, true, nullptr, st);
     SRVP_CHECK_LAUNCH("srvp_linear_attention_fwd");
     return SRVP_OK;
 }
@@ -737,6 +750,7 @@ extern "C" int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* b
     const int64_t need = srvp_linear_attention_ws_bytes(d, 1);
     SRVP_REQUIRE(need == 0 || (d->ws && d->ws_bytes >= need), "srvp_linear_attention_bwd: workspace of %lld bytes needed", (long long)need);
     const int f32 = d->elem_f32, Dk = d->Dk, Dv = d->Dv;
+    const bool exact = bd->d_state_in != nullptr;          // (the carry leaves as an fp32 gradient)
     const Operand q = operand(d->q, d->qs, Dk, f32), k = operand(d->k, d->ks, Dk, f32), v = operand(d->v, d->vs, Dv, f32), go = operand(bd->d_o, bd->d_os, Dv, f32);
     Role r[3];
     memset(r, 0, sizeof(r));
@@ -757,7 +771,7 @@ extern "C" int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* b
         memset(p, 0, sizeof(p));
         p[0].a = k; p[0].b = k; p[0].c = v; p[0].init_a = Dv; p[0].init_c = 1;
         p[1].a = q; p[1].b = q; p[1].c = go; p[1].init_a = Dv; p[1].init_c = 1; p[1].rev = 1;
-        if (f32) launch<float>(g, p, 2, false, part, st); else launch<bf16_t>(g, p, 2, false, part, st);
+        if (f32) launch<float>(g, p, 2, false, exact, part, st); else launch<bf16_t>(g, p, 2, false, exact, part, st);
         SRVP_CHECK_LAUNCH("srvp_linear_attention_bwd(segments)");
         const float* init[2] = {d->state_in, bd->d_state_out};
         const float mul[2] = {1.f, 1.f / d->scale};
@@ -765,7 +779,7 @@ extern "C" int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* b
         r[0].prefix = r[1].prefix = part + set;
         r[2].prefix = part;
     }
-    if (f32) launch<float>(g, r, 3, true, nullptr, st); else launch<bf16_t>(g, r, 3, true, nullptr, st);
+    if (f32) launch<float>(g, r, 3, true, exact, nullptr, st); else launch<bf16_t>(g, r, 3, true, exact, nullptr, st);
     SRVP_CHECK_LAUNCH("srvp_linear_attention_bwd");
     return SRVP_OK;
 }
