@@ -1,7 +1,7 @@
 """
 Command-line surface of the training program: the 47 flags of the reference's args.py:42-163 with the same names,
 types, defaults and required-ness (plain argparse; the AMP / Apex flags still parse but are no-ops because the HIP
-kernels are natively bf16-operand / fp32-accumulate).  Additions: `--local-rank` (torch >= 2 launcher spelling) and the
+kernels are natively bf16-operand / fp32-accumulate).  Additions: `--local-rank` (torch >= 2 launcher spelling), `--posterior` / `--posterior_heads` (the attention posterior) and the
 `synthetic` dataset used by bench.py / smoke tests (the reference's data loaders are out of scope).
 """
 import argparse
@@ -61,6 +61,12 @@ _FLAGS = [
     ('--seq_len_test', dict(type=int, default=None, help='validation sequence length (default: seq_len)')),
 ]
 
+# options of this framework's own: absent from the parsed options unless they are given
+_OWN = [
+    ('--posterior', dict(type=str, choices=['lstm', 'attention'], help='posterior network over the frames (lstm unless given)')),
+    ('--posterior_heads', dict(type=int, help='heads of the attention posterior (heads of 64 features unless given)')),
+]
+
 
 def create_args():
     p = argparse.ArgumentParser(prog='srvp_amd.train', description='SRVP training on MI355X (HIP kernels)',
@@ -70,4 +76,6 @@ def create_args():
             p.add_argument('--local_rank', '--local-rank', dest='local_rank', **kw)
         else:
             p.add_argument(flag, **kw)
+    for flag, kw in _OWN:
+        p.add_argument(flag, default=argparse.SUPPRESS, **kw)
     return p

@@ -60,6 +60,7 @@ class LatentNet:
         f32 = dict(dtype=torch.float32, device=device)
         nhx, nh, ny, nz, nhr = cfg['nhx'], cfg['nh_inf'], cfg['ny'], cfg['nz'], cfg['nh_res']
         self.nl_inf, self.nl_res, self.nt_inf = cfg['nlayers_inf'], cfg['nlayers_res'], cfg['nt_inf']
+        self.attention = cfg.get('posterior')          # posterior.AttentionPosterior in the LSTM's place, or None
         S = n_euler * (nt - 1)
         F = nt - 1
         self.S, self.F = S, F
@@ -76,7 +77,7 @@ class LatentNet:
         self.q_y0 = z(B, 2 * ny)
         self.y0 = z(B, ny)
         # LSTM / q_z
-        if T > 0:
+        if T > 0 and self.attention is None:
             self.lstm_bias = z(4 * nh)
             self.gates_x = z(T * B, 4 * nh)
             self.gates_act = z(T * B, 4 * nh)
@@ -109,8 +110,9 @@ class LatentNet:
             self.d_qy0_tot = z(B, 2 * ny)
             self.d_qz_tot = z(max(F, 1), B, 2 * nz)
             self.d_hz = z(max(T, 1) * B, nh)
-            self.dgates = z(max(T, 1) * B, 4 * nh)
-            self.lstm_scratch = z(2 * B * nh)
+            if self.attention is None:
+                self.dgates = z(max(T, 1) * B, 4 * nh)
+                self.lstm_scratch = z(2 * B * nh)
             self.d_hx = z(max(T, 1) * B, nhx)
             self.d_qy_hid = [z(B, nh) for _ in range(self.nl_inf - 1)]
             self.d_qy_in = z(B, ti * nhx)
@@ -194,12 +196,18 @@ class LatentNet:
 
     def lstm_bias_prep(self, params, st):
         """b_ih + b_hh of the posterior LSTM (it depends on the parameters only: the caller may form it ahead of the encoder's output)."""
+        if self.attention is not None:
+            return
         axpby(st, self.lstm_bias, 1.0, params['inf_z.bias_ih_l0'], 1.0, params['inf_z.bias_hh_l0'])
 
     def posterior(self, hx, params, st, bias_ready=False):
         """LSTM over the frame encodings + q_z (srvp.py:366,387,296): fills q_z[f] for frames f+1 < T."""
         T, B = hx.shape[0], self.B
         nh, nz = self.cfg['nh_inf'], self.cfg['nz']
+        if self.attention is not None:
+            self.hz, self._attention_saved = self.attention.run(hx, self.training)
+            self._q_z(params, T, st)
+            return
         if not bias_ready:
             self.lstm_bias_prep(params, st)
         linear_fwd(st, hx.view(T * B, -1), params['inf_z.weight_ih_l0'], self.lstm_bias, self.gates_x[:T * B])
@@ -213,6 +221,10 @@ class LatentNet:
         else:
             L.call('srvp_lstm_fwd', L.ptr(self.gates_x), L.ptr(params['inf_z.weight_hh_l0']), L.ptr(self.hz), L.ptr(self.cz),
                    L.ptr(self.gates_act), T, B, nh, st)
+        self._q_z(params, T, st)
+
+    def _q_z(self, params, T, st):
+        B, nz = self.B, self.cfg['nz']
         if T > 1:
             nq = min(T - 1, self.F)
             linear_fwd(st, self.hz[B:(nq + 1) * B], params['q_z.weight'], params['q_z.bias'], self.q_z.view(-1, 2 * nz)[:nq * B])
@@ -398,6 +410,10 @@ class LatentNet:
             self.d_hz[:B].zero_()
             linear_bwd(st, self.hz[B:T * B], params['q_z.weight'], dq, grads['q_z.weight'], grads['q_z.bias'],
                        dx=self.d_hz[B:T * B], defer=defer)
+        if nq > 0 and self.attention is not None:
+            # (kept until the next backward: the deferred launches read them on another stream, which the step waits for at its end)
+            self._attention_used = self.attention.backward(hx, self.d_hz[:T * B], self._attention_saved, grads, 'inf_z', self.d_hx, defer=defer)
+        elif nq > 0:
             ws = self.__dict__.get('_lstm_ws')
             if LSTM_BWD_FUSED and ws is not None and int(L.load().srvp_lstm_fused_ws_bytes(T, B, nh)) > 0:
                 # the recurrence as one persistent launch (csrc/rollout_fused.hip), like the forward that allocated the workspace

@@ -25,6 +25,7 @@ from . import _lib as L
 from . import arch
 from .convnet import EncoderNet, DecoderNet, cpad
 from .latent import LatentNet
+from .posterior import AttentionPosterior, PosteriorStream
 
 
 def _set_module(root, path, module):
@@ -141,8 +142,12 @@ class _SrvpForward(torch.autograd.Function):
 
 
 class StochasticLatentResidualVideoPredictor(nn.Module):
-    def __init__(self, nx, nc, nf, nhx, ny, nz, skipco, nt_inf, nh_inf, nlayers_inf, nh_res, nlayers_res, archi):
+    def __init__(self, nx, nc, nf, nhx, ny, nz, skipco, nt_inf, nh_inf, nlayers_inf, nh_res, nlayers_res, archi, *, posterior='lstm', posterior_heads=None):
+        """posterior: 'lstm' (the reference's) or 'attention' (srvp_amd.posterior; posterior_heads: default heads of 64 features)."""
         super().__init__()
+        if posterior not in ('lstm', 'attention'):
+            raise ValueError(f"posterior 'lstm' or 'attention', got {posterior!r}")
+        self.posterior = posterior
         assert nx == 64, 'the encoder / decoder families are 64x64 architectures (reference conv.py:45-48)'
         self.nx, self.nc, self.ny, self.nz, self.skipco = nx, nc, ny, nz, skipco
         self.nt_inf, self.nh_inf, self.nlayers_inf = nt_inf, nh_inf, nlayers_inf
@@ -161,7 +166,7 @@ class StochasticLatentResidualVideoPredictor(nn.Module):
         self.w_inf = _Holder()
         self.w_inf.add_module('0', nn.Linear(nh_inf, nh_inf))
         self.q_y = _mlp(nhx * nt_inf, nh_inf, ny * 2, nlayers_inf)
-        self.inf_z = nn.LSTM(nhx, nh_inf, 1)
+        self.inf_z = nn.LSTM(nhx, nh_inf, 1) if posterior == 'lstm' else AttentionPosterior(nhx, nh_inf, posterior_heads)
         self.q_z = nn.Linear(nh_inf, nz * 2)
         self.p_z = _mlp(ny, nh_res, nz * 2, nlayers_res)
         self.dynamics = _mlp(ny + nz, nh_res, ny, nlayers_res)
@@ -247,7 +252,7 @@ class StochasticLatentResidualVideoPredictor(nn.Module):
     def _cfg(self):
         return dict(nx=self.nx, nc=self.nc, nf=self.nf, nhx=self.nhx, ny=self.ny, nz=self.nz, skipco=self.skipco,
                     nt_inf=self.nt_inf, nh_inf=self.nh_inf, nlayers_inf=self.nlayers_inf, nh_res=self.nh_res,
-                    nlayers_res=self.nlayers_res, archi=self.archi)
+                    nlayers_res=self.nlayers_res, archi=self.archi, posterior=None if self.posterior == 'lstm' else self.inf_z)
 
     def _device(self):
         return self._enumerate()['plist'][0].device
@@ -883,6 +888,25 @@ class StochasticLatentResidualVideoPredictor(nn.Module):
             outs = self._forward_impl(x, nt, n_euler, tape, training=self.training)
             # fresh tensors, like the reference's outputs (the plan-owned buffers are overwritten by the next call)
             return tuple(o.clone() if o is not None else None for o in outs)
+
+    def quantize_posterior(self, on=True):
+        """posterior='attention': its two inner products on 8-bit integers in the inference calls from here on, until the next training pass
+        (on=False: back to fp32 now)."""
+        if self.posterior != 'attention':
+            raise ValueError("quantize_posterior: a model with posterior='attention'")
+        self._require_gpu()
+        if on:
+            self.inf_z.quantize()
+        else:
+            self.inf_z.drop_quantized()
+        return self
+
+    def posterior_stream(self, rows):
+        """posterior='attention': the posterior of `rows` live videos one frame at a time (srvp_amd.posterior.PosteriorStream); the LSTM's frames are
+        processed in sequences only."""
+        if self.posterior != 'attention':
+            raise ValueError("posterior_stream: a model with posterior='attention'")
+        return PosteriorStream(self.inf_z, self.q_z, int(rows), self._require_gpu())
 
     def drop_sample_plans(self):
         """Frees the S > 1 inference plans of sample() (activation buffers for S futures per video)."""

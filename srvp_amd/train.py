@@ -271,7 +271,9 @@ def main(opt):
 
     print('Building model...')
     model = StochasticLatentResidualVideoPredictor(opt.nx, opt.nc, opt.nf, opt.nhx, opt.ny, opt.nz, opt.skipco, opt.nt_inf,
-                                                   opt.nh_inf, opt.nlayers_inf, opt.nh_res, opt.nlayers_res, opt.archi)
+                                                   opt.nh_inf, opt.nlayers_inf, opt.nh_res, opt.nlayers_res, opt.archi,
+                                                   posterior=getattr(opt, 'posterior', None) or 'lstm',
+                                                   posterior_heads=getattr(opt, 'posterior_heads', None))
     model.init(res_gain=opt.res_gain)
     model.to(device)
     forward_fn = model

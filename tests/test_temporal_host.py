@@ -97,3 +97,24 @@ def test_decay_rates():
     assert t.decay_rates(1, 4, 16).exp().item() == pytest.approx(1 - 1 / 8, abs=1e-6)
     with pytest.raises(ValueError):
         t.decay_rates(2, 1.0, 5.0)
+
+
+def test_posterior_option():
+    """The attention posterior is asked for by name; without it the model, its state and its options are the reference's."""
+    import srvp_amd
+    from srvp_amd import args
+    ctor = (64, 1, 4, 8, 3, 3, False, 2, 24, 3, 16, 4, 'dcgan')
+    m = srvp_amd.StochasticLatentResidualVideoPredictor(*ctor, posterior='attention', posterior_heads=3)
+    assert [k for k in m.state_dict() if k.startswith('inf_z.')] == ['inf_z.inp.weight', 'inf_z.inp.bias', 'inf_z.norm.weight', 'inf_z.qkv.weight',
+                                                                     'inf_z.out_norm.weight', 'inf_z.out.weight', 'inf_z.last_norm.weight']
+    assert m.inf_z.heads == 3 and m.inf_z.width == 8 and 'inf_z.weight_hh_l0' in srvp_amd.StochasticLatentResidualVideoPredictor(*ctor).state_dict()
+    for bad in (dict(posterior='other'), dict(posterior='attention', posterior_heads=5), dict(posterior='attention', posterior_heads=0)):
+        with pytest.raises(ValueError):
+            srvp_amd.StochasticLatentResidualVideoPredictor(*ctor, **bad)
+    req = ['--save_path', 'x', '--ny', '2', '--nz', '2', '--nt_inf', '2', '--dataset', 'smmnist', '--data_dir', 'd', '--seq_len', '5', '--nc', '1', '--nt_cond', '2']
+    p = args.create_args()
+    assert 'posterior' not in vars(p.parse_args(req))
+    o = vars(p.parse_args(req + ['--posterior', 'attention', '--posterior_heads', '4']))
+    assert o['posterior'] == 'attention' and o['posterior_heads'] == 4
+    with pytest.raises(SystemExit):
+        p.parse_args(req + ['--posterior', 'other'])
