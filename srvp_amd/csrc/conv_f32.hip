@@ -109,7 +109,10 @@ __global__ __launch_bounds__(256) void conv_f32_kernel(const ConvF a) {
         const long long m = m0 + wid * 32 + (r & 3) + 8 * (r >> 2) + 4 * lhalf;
         if (m >= M) continue;
         const float v = acc[r];
-        s1 += v; s2 += v * v;
+        {
+#pragma clang fp contract(off)
+            s1 += v; s2 += v * v;         // (square and sum rounded apart, whatever instructions the compiler takes: the statistics stay those of every build)
+        }
         const int n = (int)(m / hw), q = (int)(m - (long long)n * hw);
         const int oy = q / a.OW, ox = q - oy * a.OW;
         const int Y = oy * a.so + a.ooy, X = ox * a.so + a.oox;
