@@ -380,7 +380,8 @@ extern "C" int srvp_linear_int8(const srvp_linear_int8_desc* d, void* stream) {
     g.ldx = d->ldx; g.ldw = d->ldw; g.ldy = d->ldy; g.M = d->M; g.N = d->N; g.K = d->K;
     g.vecy = (uintptr_t)d->y % (4 * e) == 0 && d->ldy % 4 == 0 && d->N % 4 == 0;
     g.vecy16 = (uintptr_t)d->y % 16 == 0 && d->ldy * e % 16 == 0 && d->N * e % 16 == 0;
-    SRVP_REQUIRE((long long)((d->M + 63) / 64) * ((d->N + 63) / 64) < (1LL << 30), "srvp_linear_int8: too many outputs (%d x %d)", d->M, d->N);
+    // (a grid is fewer than 2^32 threads: tiles of 128 x 128 for 256 of them, 16 columns for 512)
+    SRVP_REQUIRE(((long long)d->M + 63) / 64 * (((long long)d->N + 63) / 64) < (1LL << 25) && d->N <= (1 << 26) && d->M <= (1 << 30), "srvp_linear_int8: too many outputs (%d x %d)", d->M, d->N);
     const bool aligned = d->K % 16 == 0 && d->ldx % 16 == 0 && d->ldw % 16 == 0 && (uintptr_t)d->x % 16 == 0 && (uintptr_t)d->w % 16 == 0;
     const hipError_t err = d->out_f32 ? launch<float>(g, aligned, (hipStream_t)stream) : launch<bf16_t>(g, aligned, (hipStream_t)stream);
     if (err != hipSuccess) {

@@ -72,6 +72,9 @@ __device__ __forceinline__ int swz(int row) { return ((row & 3) << 2) | ((row >>
 template <> struct Ty<bf16_t> {
     static constexpr int KS = 32, TPK = 2, C = 64, VE = 8;
     typedef s16x8_t frag;
+    static __device__ __forceinline__ float value(bf16_t x) { return bf2f(x); }
+    // whether one of the two elements of a word is NaN or infinite: bits that reach the top one of their half
+    static __device__ __forceinline__ unsigned wild(unsigned x) { return ((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u; }
     static __device__ __forceinline__ frag pack(const f32x4_t* t) {
         u32x4_t v;
         v.x = pack2bf(t[0][0], t[0][1]); v.y = pack2bf(t[0][2], t[0][3]);
@@ -145,6 +148,8 @@ template <int W> struct View<bf16_t, W> {
 template <> struct Ty<float> {
     static constexpr int KS = 16, TPK = 1, C = 32, VE = 4;
     typedef f32x4_t frag;
+    static __device__ __forceinline__ float value(float x) { return x; }
+    static __device__ __forceinline__ unsigned wild(unsigned x) { return ((x & 0x7fffffffu) + 0x00800000u) & 0x80000000u; }
     static __device__ __forceinline__ frag pack(const f32x4_t* t) { return t[0]; }
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, f32x4_t c) {
 #pragma unroll
@@ -194,8 +199,14 @@ template <class E, int W, bool VEC> struct Tile {
             }
         }
     }
-    __device__ __forceinline__ void store(E* lds, const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) const {
+    // (returns whether this thread met a NaN or infinity, for WILD)
+    template <bool WILD> __device__ __forceinline__ bool store(E* lds, const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) const {
+        unsigned wild = 0;
         if constexpr (VEC) {
+            if constexpr (WILD) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) wild |= Ty<E>::wild(v[i].x) | Ty<E>::wild(v[i].y) | Ty<E>::wild(v[i].z) | Ty<E>::wild(v[i].w);
+            }
             const int row = tid / (W / VE), col = (tid % (W / VE)) * VE;
             if (mm == C && s.d - col0 >= W) {
 #pragma unroll
@@ -211,9 +222,12 @@ template <class E, int W, bool VEC> struct Tile {
 #pragma unroll 1
             for (int i = tid; i < C * W; i += 256) {
                 const int row = i / W, col = i % W;
-                lds[V::at(row, col)] = row < mm && col0 + col < s.d ? base[(long long)(c0 + (rev ? mm - 1 - row : row)) * s.st + col0 + col] : E(0);
+                const E x = row < mm && col0 + col < s.d ? base[(long long)(c0 + (rev ? mm - 1 - row : row)) * s.st + col0 + col] : E(0);
+                if (WILD) wild |= Ty<E>::value(x) - Ty<E>::value(x) != 0.f;
+                lds[V::at(row, col)] = x;
             }
         }
+        return wild != 0;
     }
 };
 
@@ -221,6 +235,8 @@ template <class E, int W, bool VEC> struct Tile {
 // fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel).
 // A chunk: the three tiles go to LDS (the next chunk's loads are in flight meanwhile); the lower-triangular 16 x 16 tiles of the scores are dealt to the
 // waves and exchanged through LDS; then every wave forms its columns of the output and of the state.
+// The products run over whole tiles, tokens behind the row's own weighted with zero: a chunk whose c holds a NaN or infinity (`wild`, seen on the way into
+// LDS, 1 % of the time) forms its output's sums term by term up to the row's own token, so that nothing reaches the rows in front of it.
 template <class E, int DA, int NCT, bool OUT, bool VEC, int SPLIT>
 __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanArgs g) {
     using Y = Ty<E>;
@@ -231,6 +247,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     using VP = View<E, C>;
     __shared__ __align__(16) E lb[VA::elems(C)], lc[VC::elems(C)], la[OUT ? VA::elems(C) : 1], lp[OUT ? VP::elems(C) : 1];      // lp: scores [i][j]
     __shared__ float pw[C + 1];                              // a^n
+    __shared__ int wild[2];                                  // (of this chunk and the next)
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
     int id = blockIdx.x;
@@ -264,6 +281,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     if (nch > 0) fetch(0);
 
     if (tid <= C) pw[tid] = dpow(l2, tid);
+    if (tid < 2) wild[tid] = 0;
     if (OUT) {
         // rows behind the sequence's last token: zero
         const int cw = min(CB, dc - col0), first = max(t0, n);
@@ -316,7 +334,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     for (int ct = 0; ct < NCT; ++ct) vcol[ct] = VC::column(lane, w * NCT + ct);
     const VP vp(lane);
 
-    auto chunk = [&](int c0, int mm) {
+    auto chunk = [&](int c0, int mm, bool careful) {
         if (OUT) {
             // tiles (ti, tj <= ti), dealt in turn
             int ti = 0, tj = w;
@@ -367,9 +385,19 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     const float past = pw[ti * 16 + ls + e];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) acc[ct] *= past;
+                    if (careful) {
+#pragma unroll 1
+                        for (int j = 0; j <= ti * 16 + ls; ++j) {
+                            const float p = Y::value(lp[VP::at(ti * 16 + ls, j)]);
+#pragma unroll
+                            for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) acc[ct][x] += p * Y::value(lc[VC::at(j, (w * NCT + ct) * 16 + lg * 4 + x)]);
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
-                        if (j * KS <= ti * 16 + 15) {
+                        if (j * KS <= ti * 16 + 15 && !careful) {
                             const frag pf = vp.rows(lp, ti * 16, j);
 #pragma unroll
                             for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf, acc[ct]);
@@ -424,12 +452,13 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     for (int cc = 0; cc < nch; ++cc) {
         const int c0 = t0 + (rev ? nch - 1 - cc : cc) * C, mm = min(C, t1 - c0);
         __syncthreads();                                  // (the previous chunk's tiles have been read)
-        if (OUT) ra.store(la, r.a, pa, c0, mm, rev, 0, tid);
-        rb.store(lb, r.b, pb, c0, mm, rev, 0, tid);
-        rc.store(lc, r.c, pc, c0, mm, rev, col0, tid);
+        if (OUT) ra.template store<false>(la, r.a, pa, c0, mm, rev, 0, tid);
+        rb.template store<false>(lb, r.b, pb, c0, mm, rev, 0, tid);
+        if (rc.template store<OUT>(lc, r.c, pc, c0, mm, rev, col0, tid)) wild[cc & 1] = 1;
+        if (OUT && tid == 0) wild[(cc + 1) & 1] = 0;
         __syncthreads();
         if (cc + 1 < nch) fetch(cc + 1);                  // in flight under this chunk's products
-        chunk(c0, mm);
+        chunk(c0, mm, OUT && __builtin_amdgcn_readfirstlane(wild[cc & 1]));
     }
 
     float* dst = nullptr;
@@ -675,7 +704,8 @@ int check(const srvp_linear_attention_desc* d, const char* who) {
     SRVP_REQUIRE(d->T >= 0 && d->B >= 0 && d->H >= 0, "%s: negative size", who);
     SRVP_REQUIRE(d->Dk >= 1 && d->Dk <= 256 && d->Dv >= 1 && d->Dv <= 256, "%s: heads of 1 to 256 features (got %d, %d)", who, d->Dk, d->Dv);
     SRVP_REQUIRE(d->T < (1 << 30) && (long long)d->B * d->H < (1 << 20), "%s: more than 2^30 tokens or 2^20 (sequence, head) pairs", who);
-    SRVP_REQUIRE(d->scale != 0.f && d->scale - d->scale == 0.f, "%s: scale must be finite and not zero", who);
+    const float size = fabsf(d->scale);                     // (the gradients of the state pass through 1 / scale)
+    SRVP_REQUIRE(size >= 1e-30f && size <= 1e30f, "%s: scale of 1e-30 to 1e30", who);
     return SRVP_OK;
 }
 
@@ -786,7 +816,7 @@ extern "C" int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* b
 
 extern "C" int srvp_linear_attention_step(const srvp_linear_attention_step_desc* d, void* stream) {
     SRVP_REQUIRE(d, "srvp_linear_attention_step: null descriptor");
-    SRVP_REQUIRE(d->B >= 0 && d->H >= 0 && d->nslots >= 0 && (long long)d->B * d->H < (1 << 30), "srvp_linear_attention_step: bad sizes");
+    SRVP_REQUIRE(d->B >= 0 && d->H >= 0 && d->nslots >= 0 && (long long)d->B * d->H < (1 << 24), "srvp_linear_attention_step: fewer than 2^24 (row, head) pairs");
     SRVP_REQUIRE(d->Dk >= 1 && d->Dk <= 256 && d->Dv >= 1 && d->Dv <= 256, "srvp_linear_attention_step: heads of 1 to 256 features (got %d, %d)", d->Dk, d->Dv);
     if (d->B == 0 || d->H == 0) return SRVP_OK;
     SRVP_REQUIRE(d->q && d->k && d->v && d->o && d->log_decay && (d->state || d->nslots == 0), "srvp_linear_attention_step: null pointer");

@@ -212,13 +212,14 @@ template <int TPR> __device__ __forceinline__ void row_sum(float& u, float& v, f
         for (int i = 0; i < NW; ++i) { u += red[i]; v += red[NW + i]; }
     }
 }
-template <int TPR> __device__ __forceinline__ float row_sum(float u, float* red, int tid) {
-    u = wave_sum(u);
+template <int TPR, class F> __device__ __forceinline__ F row_sum(F u, F* red, int tid) {
+    if constexpr (sizeof(F) == 8) u = wave_sum_d(u);
+    else u = wave_sum(u);
     if constexpr (TPR > 64) {
         __syncthreads();
         if ((tid & 63) == 0) red[tid >> 6] = u;
         __syncthreads();
-        u = 0.f;
+        u = 0;
 #pragma unroll
         for (int i = 0; i < TPR / 64; ++i) u += red[i];
     }
@@ -264,27 +265,28 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
             if (Q8) hd[i] = (double)u + (double)v;
         }
         if (row + step < g.M) fetch(row + step);
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < V * VE; ++i) ss += h[i] * h[i];
         if (g.sum) row_store<E, VE, V, TPR>((E*)g.sum + row * g.ss, g.N, g.vec, t, h);
         if constexpr (!Q8) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < V * VE; ++i) ss += h[i] * h[i];
             const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)g.N + g.eps);
 #pragma unroll
             for (int i = 0; i < V * VE; ++i) h[i] *= rstd * wv[i];
             row_store<E, VE, V, TPR>((E*)g.y + row * g.ys, g.N, g.vec, t, h);
         } else {
-            double most = 0;
+            double most = 0, ss = 0;                       // (the squares in 64 bits too: a row of 1e20s is not an infinite one)
 #pragma unroll
             for (int i = 0; i < V * VE; ++i) {
+                ss += hd[i] * hd[i];
                 if (NORM) hd[i] *= (double)wv[i];
                 most = fmax(most, fabs(hd[i]));
             }
-            ss = row_sum<TPR>(ss, red, tid);
+            ss = row_sum<TPR>(ss, redd, tid);
             most = row_max<TPR>(most, redd, tid);
-            const bool fine = ss < INFINITY && most < (double)INFINITY;      // (false for NaN)
+            const bool fine = ss < (double)INFINITY && most < (double)INFINITY;      // (false for NaN)
             const double to = fine && most > 0 ? 127.0 / most : 0.0;
-            if (t == 0) g.scale[row] = fine ? (float)(most * (NORM ? 1.0 / sqrt((double)ss / g.N + (double)g.eps) : 1.0) / 127.0) : NAN;
+            if (t == 0) g.scale[row] = fine ? (float)(most * (NORM ? 1.0 / sqrt(ss / g.N + (double)g.eps) : 1.0) / 127.0) : NAN;
             signed char* q = g.q + row * g.qs;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
@@ -446,8 +448,8 @@ constexpr int NORM_MAX = 16384;
 
 extern "C" int srvp_rotary(const srvp_rotary_desc* d, void* stream) {
     SRVP_REQUIRE(d, "srvp_rotary: null descriptor");
-    SRVP_REQUIRE(d->T >= 0 && d->B >= 0 && d->Hq >= 0 && d->Hk >= 0 && d->D >= 1 && d->pairs >= 0 && 2 * d->pairs <= d->D && d->D <= 4096,
-                 "srvp_rotary: bad sizes (heads of 1 to 4096 features, at most half as many pairs)");
+    SRVP_REQUIRE(d->T >= 0 && d->B >= 0 && d->Hq >= 0 && d->Hk >= 0 && d->Hq < (1 << 20) && d->Hk < (1 << 20) && d->D >= 1 && d->pairs >= 0 && 2 * d->pairs <= d->D && d->D <= 4096,
+                 "srvp_rotary: bad sizes (fewer than 2^20 heads of 1 to 4096 features, at most half as many pairs)");
     const long long rows = (long long)d->T * d->B;
     if (rows == 0 || d->Hq + d->Hk == 0) return SRVP_OK;
     SRVP_REQUIRE((d->Hq == 0 || (d->q && d->oq)) && (d->Hk == 0 || (d->k && d->ok)) && d->positions && (d->freq || d->pairs == 0), "srvp_rotary: null pointer");
@@ -468,12 +470,13 @@ extern "C" int srvp_rotary(const srvp_rotary_desc* d, void* stream) {
     const int n = d->pairs > 0 ? d->pairs : 1, H = d->Hq + d->Hk;
     long long R = (256 + n - 1) / n, most = 16384LL / ((long long)H * d->D * e) + 1;
     if (R > most) R = most;
+    if (R < (rows >> 23) + 1) R = (rows >> 23) + 1;       // (a grid is fewer than 2^24 workgroups)
     if (R * n > ROT_TAB) R = ROT_TAB / n;
     if (R < 1) R = 1;
     g.R = (int)R;
     const int first = !vec ? d->pairs : d->interleaved ? 2 * d->pairs / ve : d->pairs / ve, items = first + (d->D - 2 * d->pairs) / (vec ? ve : 1);
     const long long grid = (rows + R - 1) / R;
-    SRVP_REQUIRE(rows < (1LL << 31) && R * H * items < (1LL << 30), "srvp_rotary: too many rows or heads");
+    SRVP_REQUIRE(rows < (1LL << 31) && grid < (1 << 24) && R * H * items < (1LL << 30), "srvp_rotary: too many rows or heads");
     g.dB = divide(d->B); g.dn = divide(n); g.dH = divide(H); g.ditems = divide(items);
     hipStream_t st = (hipStream_t)stream;
 #define ROTARY(E, VE, MODE) hipLaunchKernelGGL((rotary_kernel<E, VE, MODE>), dim3((unsigned)grid), dim3(256), 0, st, g)

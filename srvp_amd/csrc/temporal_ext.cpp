@@ -31,14 +31,16 @@ struct Entries {
     ENTRIES(X)
 #undef X
 } lib;
-PyObject* hip_error = nullptr;      // srvp_amd._lib.SrvpHipError
+PyObject *hip_error = nullptr, *memory_error = nullptr;      // srvp_amd._lib.SrvpHipError, torch.OutOfMemoryError
 
-void bind(const py::dict& addresses, const py::object& error) {
+void bind(const py::dict& addresses, const py::object& error, const py::object& no_memory) {
 #define X(name) lib.name = reinterpret_cast<decltype(&::name)>(addresses[#name].cast<uintptr_t>());
     ENTRIES(X)
 #undef X
     Py_INCREF(error.ptr());
+    Py_INCREF(no_memory.ptr());
     hip_error = error.ptr();
+    memory_error = no_memory.ptr();
 }
 
 // ---- errors
@@ -128,7 +130,7 @@ Attention attention_args(const char* what, const Tensor& q, const Tensor& k, con
     floats(what, {&q, &k, &v});
     const int64_t B = q.size(1), H = q.size(2), Dk = q.size(3), Dv = v.size(3);
     if (Dk < 1 || Dk > 256 || Dv < 1 || Dv > 256) value_error(std::string(what) + ": heads of 1 to 256 features, got " + std::to_string(Dk) + " and " + std::to_string(Dv));
-    if (q.size(0) >= (1 << 30) || B * H >= (1 << 20)) value_error(std::string(what) + ": fewer than 2^30 tokens and 2^20 (sequence, head) pairs");
+    if (q.size(0) >= (1 << 30) || B >= (1 << 20) || H >= (1 << 20) || B * H >= (1 << 20)) value_error(std::string(what) + ": fewer than 2^30 tokens and 2^20 (sequence, head) pairs");
     Attention a;
     a.log_decay = decays(what, log_decay, H);
     if (state) {
@@ -143,7 +145,7 @@ Attention attention_args(const char* what, const Tensor& q, const Tensor& k, con
     }
     same_device(what, q, {&k, &v, &a.log_decay, &a.state, &a.lengths});
     a.scale = scale ? *scale : 1.0 / std::sqrt((double)Dk);
-    if ((float)a.scale == 0.f || !std::isfinite((float)a.scale)) value_error(std::string(what) + ": scale must be finite and not zero");
+    if (!(std::abs(a.scale) >= 1e-30 && std::abs(a.scale) <= 1e30)) value_error(std::string(what) + ": scale of 1e-30 to 1e30, got " + std::to_string(a.scale));
     a.q = inner(q);
     a.k = inner(k);
     a.v = inner(v);
@@ -253,6 +255,7 @@ Tensor linear_attention_step(const Tensor& q0, const Tensor& k0, const Tensor& v
     no_gradient(what, {&q0, &k0, &v0, &state});
     const int64_t B = q0.size(0), H = q0.size(1), Dk = q0.size(2), Dv = v0.size(2);
     if (Dk < 1 || Dk > 256 || Dv < 1 || Dv > 256) value_error(std::string(what) + ": heads of 1 to 256 features, got " + std::to_string(Dk) + " and " + std::to_string(Dv));
+    if (B >= (1 << 24) || H >= (1 << 24) || B * H >= (1 << 24) || (state.dim() == 4 && state.size(0) >= (1LL << 31))) value_error(std::string(what) + ": fewer than 2^24 (row, head) pairs and 2^31 states");
     const Tensor ld = decays(what, log_decay, H);
     if (state.scalar_type() != at::kFloat || state.dim() != 4 || state.size(1) != H || state.size(2) != Dk || state.size(3) != Dv || !state.is_contiguous() ||
         (state.numel() && (uintptr_t)state.data_ptr() % 16))
@@ -335,6 +338,8 @@ py::object rotary(const Tensor& q, const Maybe& k, const Tensor& positions0, con
         value_error(std::string(what) + ": q (T, B, Hq, D) and k (T, B, Hk, D), got " + shape(q) + (k ? ", " + shape(kk) : ""));
     floats(what, {&q, &kk});
     const int64_t T = q.size(0), B = q.size(1), D = q.size(3);
+    if (T >= (1LL << 31) || B >= (1LL << 31) || T * B >= (1LL << 31) || q.size(2) >= (1 << 20) || (k && kk.size(2) >= (1 << 20)))
+        value_error(std::string(what) + ": fewer than 2^31 rows and 2^20 heads, got " + shape(q) + (k ? ", " + shape(kk) : ""));
     if (D < 1 || D > 4096) value_error(std::string(what) + ": heads of 1 to 4096 features, got " + std::to_string(D));
     if (!(positions0.dim() == 1 && positions0.size(0) == T) && !(positions0.dim() == 2 && positions0.size(0) == T && positions0.size(1) == B))
         value_error(std::string(what) + ": positions (" + std::to_string(T) + ",) or (" + std::to_string(T) + ", " + std::to_string(B) + "), got " + shape(positions0));
@@ -487,6 +492,8 @@ PYBIND11_MODULE(_temporal, m) {
             if (p) std::rethrow_exception(p);
         } catch (const HipError& e) {
             PyErr_SetString(hip_error ? hip_error : PyExc_RuntimeError, e.what());
+        } catch (const c10::OutOfMemoryError& e) {
+            PyErr_SetString(memory_error ? memory_error : PyExc_RuntimeError, e.what_without_backtrace());
         }
     });
     m.def("bind", &bind);

@@ -35,7 +35,7 @@ def load():
         except ImportError as e:
             raise L.SrvpHipError(f'srvp_amd/_temporal.so: {e}.  Build it with `make -C srvp_amd/csrc` (or `python -c "import __graft_entry__ as g; '
                                  'g.build()"`).') from e
-        ext.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in _ENTRIES}, L.SrvpHipError)
+        ext.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in _ENTRIES}, L.SrvpHipError, torch.OutOfMemoryError)
         _ext = ext
     return _ext
 
@@ -54,7 +54,7 @@ def linear_attention(q, k, v, log_decay, *, state=None, lengths=None, scale=None
     q, k (T, B, H, Dk), v (T, B, H, Dv), heads of 1 to 256 features; log_decay (H,) float32, normally <= 0 (-inf: no memory); state (B, H, Dk, Dv)
     float32: S in front of the first token (None: zero; it is not changed); lengths (B,): tokens of each sequence (outputs behind them are zero, values
     there are not read); scale: default Dk ** -0.5.  Returns o (T, B, H, Dv), or (o, new state) with return_state.  Gradients: q, k, v, state.
-    A NaN or infinity in v or k reaches the outputs of the chunk (64 tokens, float32: 32) that its token lies in, and those behind it."""
+    A NaN or infinity reaches the outputs of its own token and of those behind it."""
     return (_ext or load()).linear_attention(q, k, v, log_decay, state, lengths, scale, return_state)
 
 

@@ -1,0 +1,239 @@
+"""
+Temporal operators at their edges: values that are not finite, offsets past 32 bits, rows of the largest values, calls from two threads, refusals.
+"""
+import threading
+
+import pytest
+import torch
+
+from test_gpu_temporal import BF, DEV, FP, decays, inner_of, rnd, rows8, scan, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+@pytest.mark.parametrize('T,Dk,Dv,dt', [(50, 64, 64, FP), (50, 33, 17, FP), (150, 128, 128, BF), (150, 40, 72, BF), (150, 21, 35, BF), (90, 256, 200, BF)])
+def test_linear_attention_is_causal_for_what_is_not_finite(T, Dk, Dv, dt, bad):
+    """A NaN or infinity of token p changes nothing in front of p (gradients that run backwards in time: behind it), nor other columns of v."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(T + Dk)
+    H, p, c = 2, T // 2 + 3, Dv - 2
+    ld, sc = decays(H), Dk ** -0.5
+    q, k, v, do = rnd(g, T, 1, H, Dk, dtype=dt), rnd(g, T, 1, H, Dk, dtype=dt), rnd(g, T, 1, H, Dv, dtype=dt), rnd(g, T, 1, H, Dv, dtype=dt)
+    inn = inner_of(dt, T, max(Dk, Dv))
+
+    def spoil(x, col):
+        y = x.clone()
+        y[p, :, 0, col] = bad
+        return y
+    others = [i for i in range(Dv) if i != c]
+    fwd = lambda x: t.linear_attention(*x, ld)
+    full, size = scan(q, k, v, ld, sc, False)
+    o = fwd((q, k, spoil(v, c)))
+    within(o[:p], full[:p], size[:p], dt, inn, 'o in front of a spoilt v')
+    within(o[..., others], full[..., others], size[..., others], dt, inn, 'o beside a spoilt v')
+    assert torch.equal(o[:, :, 1], fwd((q, k, v))[:, :, 1]) and not torch.isfinite(o[p, 0, 0, c])
+    o = fwd((q, spoil(k, 0), v))
+    within(o[:p], full[:p], size[:p], dt, inn, 'o in front of a spoilt k')
+    o = fwd((spoil(q, 0), k, v))
+    keep = [i for i in range(T) if i != p]
+    within(o[keep], full[keep], size[keep], dt, inn, 'o beside a spoilt q')
+
+    def back(*x):
+        return t.linear_attention_backward(*x, ld)[:3]
+    (rq, zq), (rk, zk), (rv, zv) = scan(do, v, k, ld, sc, False), scan(v, do, q, ld, sc, True), scan(k, q, do, ld, sc, True)
+    after = slice(p + 1, T)
+    dq, dk, dv = back(spoil(do, c), q, k, v)
+    within(dq[keep], rq[keep], zq[keep], dt, inn, 'dq beside a spoilt do')
+    within(dk[after], rk[after], zk[after], dt, inn, 'dk behind a spoilt do')
+    within(dv[after], rv[after], zv[after], dt, inn, 'dv behind a spoilt do')
+    within(dv[..., others], rv[..., others], zv[..., others], dt, inn, 'dv beside a spoilt do')
+    dq, dk, dv = back(do, spoil(q, 0), k, v)
+    within(dq, rq, zq, dt, inn, 'dq of a spoilt q')
+    within(dk[after], rk[after], zk[after], dt, inn, 'dk behind a spoilt q')
+    within(dv[after], rv[after], zv[after], dt, inn, 'dv behind a spoilt q')
+    dq, dk, dv = back(do, q, spoil(k, 0), v)
+    within(dq[:p], rq[:p], zq[:p], dt, inn, 'dq in front of a spoilt k')
+    within(dk, rk, zk, dt, inn, 'dk of a spoilt k')
+    within(dv[keep], rv[keep], zv[keep], dt, inn, 'dv beside a spoilt k')
+    dq, dk, dv = back(do, q, k, spoil(v, c))
+    within(dq[:p], rq[:p], zq[:p], dt, inn, 'dq in front of a spoilt v')
+    within(dk[keep], rk[keep], zk[keep], dt, inn, 'dk beside a spoilt v')
+    within(dv, rv, zv, dt, inn, 'dv of a spoilt v')
+
+
+def test_linear_attention_padding_without_lengths():
+    """Right-padded rows full of NaN leave the tokens in front of them alone, also where a sequence is cut into segments."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(7)
+    T, H, D = 900, 2, 64
+    q, k, v = (rnd(g, T, 2, H, D, dtype=BF) for _ in range(3))
+    ref, size = scan(q, k, v, decays(H), D ** -0.5, False)
+    for x in (q, k, v):
+        x[517:, 0] = float('nan')
+    o = t.linear_attention(q, k, v, decays(H))
+    within(o[:517], ref[:517], size[:517], BF, inner_of(BF, T, D), 'in front of the padding')
+    within(o[:, 1], ref[:, 1], size[:, 1], BF, inner_of(BF, T, D), 'the other sequence')
+
+
+@pytest.mark.parametrize('dt', [FP, BF])
+def test_int8_rows_of_the_largest_values(dt):
+    """Rows whose squares pass 32 bits, and rows of the smallest values: as exact as any other."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(3)
+    x = rnd(g, 6, 300)
+    for i, e in enumerate((1e20, 3e37, 1e-30, 1e-38, 1.0, 0.0)):
+        x[i] *= e
+    x, w = x.to(dt), rnd(g, 300)
+    q, s = t.quantize_int8(x)
+    rq, rs = rows8(x.double(), None, 0)
+    assert torch.equal(q.double(), rq)
+    # half a step, and 2^-150 where the scale is subnormal
+    assert ((s.double() - rs).abs() <= 2.0 ** -24 * rs + 2.0 ** -150).all()
+    q, s = t.rms_norm_int8(x, w)
+    rq, rs = rows8(x.double(), w.double(), 1e-6)
+    assert torch.equal(q.double(), rq)
+    assert ((s.double() - rs).abs() <= (2.0 ** -24 + 1e-12) * rs + 2.0 ** -150).all()
+
+
+def test_offsets_past_32_bits():
+    """Strides and slots whose products pass 2^31 elements: the results of the packed copies."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(5)
+    big = torch.empty(5 * 2 ** 30, dtype=torch.uint8, device=DEV)
+
+    def apart(x, stride):
+        """x with its rows `stride` elements apart."""
+        inner = x[0].numel()
+        y = big.view(x.dtype).as_strided(x.shape, (stride,) + x[0].contiguous().stride())
+        assert (x.shape[0] - 1) * stride + inner <= big.numel() // x.element_size() and (x.shape[0] - 1) * stride >= 2 ** 31 // (1 if x.element_size() < 4 else 2)
+        return y.copy_(x)
+    H, D = 2, 64
+    ld = decays(H)
+    # by 16-byte loads (a step under 2^23 elements) and one by one
+    for T, stride in ((300, 2 ** 23 - 8), (36, 2 ** 26 + 8)):
+        q, k, v = (rnd(g, T, 1, H, D, dtype=BF) for _ in range(3))
+        ref = t.linear_attention(q, k, v, ld)
+        assert torch.equal(t.linear_attention(apart(q, stride), k, v, ld), ref)
+        assert torch.equal(t.linear_attention(q, apart(k, stride), v, ld), ref)
+        assert torch.equal(t.linear_attention(q, k, apart(v, stride), ld), ref)
+        ref = t.linear_attention_backward(v, q, k, v, ld)
+        for a, b in zip(t.linear_attention_backward(apart(v, stride), q, k, v, ld)[:3], ref):
+            assert torch.equal(a, b)
+    pos, w = torch.arange(36, device=DEV), t.rotary_frequencies(D, device=DEV)
+    assert torch.equal(t.rotary(apart(q, stride), None, pos, w), t.rotary(q, None, pos, w))
+    x, wt = q.reshape(36, -1), rnd(g, H * D)
+    wide = apart(x, stride)
+    for a, b in zip(t.rms_norm(wide, wt, residual=x) + t.rms_norm_int8(x, wt, residual=wide) + t.rms_norm_backward(wide, x, wt),
+                    t.rms_norm(x, wt, residual=x) + t.rms_norm_int8(x, wt, residual=x) + t.rms_norm_backward(x, x, wt)):
+        assert torch.equal(a, b)
+    for M, K in ((40, 128), (70, 128), (70, 51)):
+        a, b = (torch.randint(-128, 128, s, generator=g, dtype=torch.int8).to(DEV) for s in ((M, K), (70, K)))
+        sa, sb = rnd(g, M), rnd(g, 70)
+        ref = t.linear_int8(a, sa, b, sb)
+        assert torch.equal(t.linear_int8(apart(a, 2 ** 26), sa, b, sb), ref)
+        assert torch.equal(t.linear_int8(a, sa, apart(b, 2 ** 26), sb), ref)
+    # a pool of states of more than 2^31 bytes and elements: 140000 slots of 8192 values
+    pool = big.view(FP)[:140000 * 8192].view(140000, H, D, D)
+    slots = torch.tensor([139999, 7, 70001], device=DEV)
+    few = rnd(g, 3, H, D, D)
+    pool[slots] = few
+    q, k, v = (rnd(g, 3, H, D) for _ in range(3))
+    assert torch.equal(t.linear_attention_step(q, k, v, ld, pool, slots=slots), t.linear_attention_step(q, k, v, ld, few))
+    assert torch.equal(pool[slots], few)
+
+
+def test_two_threads():
+    """Calls from two threads on their own streams: each thread's own results."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(6)
+    ld = decays(2)
+    ins = [tuple(rnd(g, 700, 1, 2, 64, dtype=BF) for _ in range(3)) for _ in range(2)]
+    ref = [t.linear_attention(*x, ld) for x in ins]
+    torch.cuda.synchronize()
+    out = [None, None]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            out[i] = [t.linear_attention(*ins[i], ld) for _ in range(20)]
+        s.synchronize()
+    both = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for x in both:
+        x.start()
+    for x in both:
+        x.join()
+    for i in range(2):
+        assert all(torch.equal(o, ref[i]) for o in out[i])
+
+
+def test_inference_mode_and_versions():
+    """States that are advanced in place are seen as changed; inference mode takes the same calls."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(9)
+    q, k, v, ld = rnd(g, 2, 2, 16), rnd(g, 2, 2, 16), rnd(g, 2, 2, 16), decays(2)
+    s = torch.zeros(2, 2, 16, 16, device=DEV)
+    n = s._version
+    o = t.linear_attention_step(q, k, v, ld, s)
+    assert s._version == n + 1
+    x = rnd(g, 5, 2, 2, 16).requires_grad_()
+    y = t.linear_attention(x, x, x, ld, state=s)
+    t.linear_attention_step(q, k, v, ld, s)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+    with torch.inference_mode():
+        z = torch.zeros(2, 2, 16, 16, device=DEV)
+        assert torch.equal(t.linear_attention_step(q, k, v, ld, z), o)
+        assert torch.equal(t.linear_attention(x, x, x, ld, state=s), t.linear_attention(x.detach(), x.detach(), x.detach(), ld, state=s))
+
+
+def test_refusals():
+    from srvp_amd import temporal as t
+    from srvp_amd._lib import SrvpHipError
+    z = lambda *s, dt=FP: torch.zeros(*s, dtype=dt, device=DEV)
+    x, ld, w = z(4, 2, 3, 8), decays(3), t.rotary_frequencies(8, device=DEV)
+    st, pos, i8 = z(2, 3, 8, 8), torch.arange(4, device=DEV), lambda *s: z(*s, dt=torch.int8)
+    la, step, rot, norm, lin = t.linear_attention, t.linear_attention_step, t.rotary, t.rms_norm, t.linear_int8
+    grad = lambda *s: z(*s).requires_grad_()
+    cases = [
+        (ValueError, lambda: la(x[0], x[0], x[0], ld)), (ValueError, lambda: la(x, z(4, 2, 3, 9), x, ld)), (ValueError, lambda: la(x, x, z(4, 2, 2, 8), ld)),
+        (TypeError, lambda: la(x.half(), x.half(), x.half(), ld)), (TypeError, lambda: la(x, x.to(BF), x, ld)), (ValueError, lambda: la(x, x, x, ld.double())),
+        (ValueError, lambda: la(x, x, x, ld[:2])), (ValueError, lambda: la(x, x, x, ld.clone().requires_grad_())), (ValueError, lambda: la(x, x, x, ld.cpu())),
+        (ValueError, lambda: la(x, x, x, ld, state=st[:1])), (ValueError, lambda: la(x, x, x, ld, state=st.to(BF))), (ValueError, lambda: la(x, x, x, ld, lengths=pos)),
+        (TypeError, lambda: la(x, x, x, ld, lengths=z(2))), (ValueError, lambda: la(x, x, x, ld, scale=0.0)), (ValueError, lambda: la(x, x, x, ld, scale=1e-35)),
+        (ValueError, lambda: la(x, x, x, ld, scale=float('nan'))), (ValueError, lambda: la(z(1, 1, 1, 257), z(1, 1, 1, 257), z(1, 1, 1, 4), ld[:1])),
+        (ValueError, lambda: la(z(1, 1, 1, 8).expand(2, 2 ** 20, 1, 8), z(1, 1, 1, 8).expand(2, 2 ** 20, 1, 8), z(1, 1, 1, 8).expand(2, 2 ** 20, 1, 8), ld[:1])),
+        (ValueError, lambda: t.linear_attention_backward(x[:3], x, x, x, ld)), (ValueError, lambda: t.linear_attention_backward(x, x, x, x, ld, d_state=st[:1])),
+        (ValueError, lambda: t.linear_attention_backward(x, grad(4, 2, 3, 8), x, x, ld)), (SrvpHipError, lambda: la(x.cpu(), x.cpu(), x.cpu(), ld.cpu())),
+        (ValueError, lambda: step(x, x, x, ld, st)), (ValueError, lambda: step(x[:, 0], x[:, 0], x[:, 0], ld, st)), (ValueError, lambda: step(x[0], x[0], x[0], ld, st.transpose(2, 3))),
+        (ValueError, lambda: step(x[0], x[0], x[0], ld, st.to(BF))), (TypeError, lambda: step(x[0], x[0], x[0], ld, st, slots=z(2))), (ValueError, lambda: step(x[0], x[0], x[0], ld, st, slots=pos)),
+        (ValueError, lambda: step(grad(2, 3, 8), x[0], x[0], ld, st)), (ValueError, lambda: step(x[0], x[0], x[0], ld, z(2 * 3 * 64 + 1)[1:].view(2, 3, 8, 8))),
+        (ValueError, lambda: rot(x, z(4, 2, 3, 6), pos, w)), (ValueError, lambda: rot(x, None, pos[:3], w)), (TypeError, lambda: rot(x, None, z(4), w)),
+        (ValueError, lambda: rot(x, None, pos, w.float())), (ValueError, lambda: rot(x, None, pos, t.rotary_frequencies(10, device=DEV))), (ValueError, lambda: rot(x, None, pos.cpu(), w)),
+        (ValueError, lambda: rot(x, None, pos, w, magnitude=float('inf'))), (ValueError, lambda: rot(z(1, 1, 1, 8).expand(2 ** 20, 2 ** 11, 1, 8), None, pos, w)),
+        (ValueError, lambda: rot(z(1, 1, 1, 2).expand(1, 1, 2 ** 20, 2), None, pos[:1], w[:1])),
+        (ValueError, lambda: norm(x, z(7))), (ValueError, lambda: norm(x, z(8, dt=BF))), (ValueError, lambda: norm(x, z(8), residual=x[:2])), (TypeError, lambda: norm(x, z(8), residual=x.to(BF))),
+        (TypeError, lambda: norm(x.double(), z(8))), (ValueError, lambda: norm(z(2, 16385), z(16385))), (ValueError, lambda: norm(x, torch.zeros(8))), (ValueError, lambda: norm(z(2, 0), z(0))),
+        (ValueError, lambda: t.rms_norm_backward(x[:2], x, z(8))), (ValueError, lambda: t.rms_norm_int8(grad(2, 8), z(8))), (ValueError, lambda: t.quantize_int8(grad(2, 8))),
+        (TypeError, lambda: lin(x, z(4, 2, 3), i8(5, 8), z(5))), (ValueError, lambda: lin(i8(4, 9), z(4), i8(5, 8), z(5))), (ValueError, lambda: lin(i8(4, 8), z(4, 1), i8(5, 8), z(5))),
+        (ValueError, lambda: lin(i8(4, 8), z(4), i8(5, 8), z(4))), (ValueError, lambda: lin(i8(4, 8), z(4), i8(5, 8), z(5), bias=z(4))), (TypeError, lambda: lin(i8(4, 8), z(4), i8(5, 8), z(5), out_dtype=torch.float16)),
+        (ValueError, lambda: lin(i8(1, 131072), z(1), i8(1, 131072), z(1))), (ValueError, lambda: lin(i8(4, 8), z(4), i8(5, 8).cpu(), z(5))), (ValueError, lambda: lin(i8(4, 8), z(4), i8(5, 8), grad(5))),
+    ]
+    for i, (kind, f) in enumerate(cases):
+        try:
+            f()
+        except kind:
+            continue
+        except Exception as e:
+            raise AssertionError(f'case {i}: {type(e).__name__}: {e}')
+        raise AssertionError(f'case {i}: not refused')
+    # differentiable once
+    q = rnd(torch.Generator().manual_seed(1), 4, 2, 3, 8).requires_grad_()
+    for y in (la(q, q, q, ld), rot(q, None, pos, w), norm(q, torch.ones(8, device=DEV))):
+        with pytest.raises(RuntimeError, match='create_graph'):
+            torch.autograd.grad(y.sum(), q, create_graph=True)
+    # an output that cannot be allocated is torch's own error, and the next call works
+    far = z(1, 1, 1, 256).expand(2 ** 29, 4, 1, 256)
+    with pytest.raises(torch.OutOfMemoryError):
+        la(far, far, far, ld[:1])
+    assert la(x, x, x, ld).shape == x.shape

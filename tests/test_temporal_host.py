@@ -65,6 +65,14 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.srvp_rms_norm_bwd(r(L.RmsNormBwdDesc(x=16, d_y=16, w=16, dx=16, dw=16, ws=16, M=4, N=64)), None) == 1 and b'workspace' in lib.srvp_last_error()
     wide = dict(x=16, w=16, x_scale=16, w_scale=16, y=16, M=1, N=1)
     assert lib.srvp_linear_int8(r(L.LinearInt8Desc(K=200000, **wide)), None) == 1 and lib.srvp_linear_int8(r(L.LinearInt8Desc(K=0, **wide)), None) == 1
+    # more workgroups than a launch takes
+    assert lib.srvp_linear_int8(r(L.LinearInt8Desc(K=16, **dict(wide, M=1, N=2 ** 30))), None) == 1 and b'too many' in lib.srvp_last_error()
+    assert lib.srvp_linear_int8(r(L.LinearInt8Desc(K=16, **dict(wide, M=2 ** 20, N=2 ** 20))), None) == 1 and b'too many' in lib.srvp_last_error()
+    assert lib.srvp_linear_int8(r(L.LinearInt8Desc(K=16, **dict(wide, M=2 ** 31 - 1, N=1))), None) == 1 and b'too many' in lib.srvp_last_error()
+    assert lib.srvp_linear_attention_step(r(L.LinearAttentionStepDesc(**dict(two_rows, B=2 ** 20, H=16, nslots=2 ** 20))), None) == 1
+    many = dict(q=16, oq=16, positions=16, freq=16, T=2 ** 26, B=1, Hq=1, D=4096, pairs=2048, magnitude=1.0)
+    assert lib.srvp_rotary(r(L.RotaryDesc(**many)), None) == 1 and b'too many' in lib.srvp_last_error()
+    assert lib.srvp_linear_attention_fwd(r(attention(scale=1e-35, p=16)), None) == 1 and b'scale' in lib.srvp_last_error()
 
 
 def test_no_cpu_path():
