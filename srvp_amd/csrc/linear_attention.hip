@@ -73,8 +73,16 @@ template <> struct Ty<bf16_t> {
     static constexpr int KS = 32, TPK = 2, C = 64, VE = 8;
     typedef s16x8_t frag;
     static __device__ __forceinline__ float value(bf16_t x) { return bf2f(x); }
-    // whether one of the two elements of a word is NaN or infinite: bits that reach the top one of their half
-    static __device__ __forceinline__ unsigned wild(unsigned x) { return ((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u; }
+    // whether an element is NaN or infinite (the exponent's bits and one more carry into the sign's)
+    static __device__ __forceinline__ unsigned wild(const frag& x) {
+        const u32x4_t v = __builtin_bit_cast(u32x4_t, x), y = (v & 0x7fff7fffu) + 0x00800080u;
+        return (y.x | y.y | y.z | y.w) & 0x80008000u;
+    }
+    static __device__ __forceinline__ frag tame(frag x) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (x[i] & 0x7f80) == 0x7f80 ? 0 : x[i];
+        return x;
+    }
     static __device__ __forceinline__ frag pack(const f32x4_t* t) {
         u32x4_t v;
         v.x = pack2bf(t[0][0], t[0][1]); v.y = pack2bf(t[0][2], t[0][3]);
@@ -149,7 +157,15 @@ template <> struct Ty<float> {
     static constexpr int KS = 16, TPK = 1, C = 32, VE = 4;
     typedef f32x4_t frag;
     static __device__ __forceinline__ float value(float x) { return x; }
-    static __device__ __forceinline__ unsigned wild(unsigned x) { return ((x & 0x7fffffffu) + 0x00800000u) & 0x80000000u; }
+    static __device__ __forceinline__ unsigned wild(const frag& x) {
+        const u32x4_t v = __builtin_bit_cast(u32x4_t, x), y = (v & 0x7fffffffu) + 0x00800000u;
+        return (y.x | y.y | y.z | y.w) & 0x80000000u;
+    }
+    static __device__ __forceinline__ frag tame(frag x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = x[i] - x[i] == 0.f ? x[i] : 0.f;
+        return x;
+    }
     static __device__ __forceinline__ frag pack(const f32x4_t* t) { return t[0]; }
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, f32x4_t c) {
 #pragma unroll
@@ -199,14 +215,8 @@ template <class E, int W, bool VEC> struct Tile {
             }
         }
     }
-    // (returns whether this thread met a NaN or infinity, for WILD)
-    template <bool WILD> __device__ __forceinline__ bool store(E* lds, const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) const {
-        unsigned wild = 0;
+    __device__ __forceinline__ void store(E* lds, const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) const {
         if constexpr (VEC) {
-            if constexpr (WILD) {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) wild |= Ty<E>::wild(v[i].x) | Ty<E>::wild(v[i].y) | Ty<E>::wild(v[i].z) | Ty<E>::wild(v[i].w);
-            }
             const int row = tid / (W / VE), col = (tid % (W / VE)) * VE;
             if (mm == C && s.d - col0 >= W) {
 #pragma unroll
@@ -222,12 +232,9 @@ template <class E, int W, bool VEC> struct Tile {
 #pragma unroll 1
             for (int i = tid; i < C * W; i += 256) {
                 const int row = i / W, col = i % W;
-                const E x = row < mm && col0 + col < s.d ? base[(long long)(c0 + (rev ? mm - 1 - row : row)) * s.st + col0 + col] : E(0);
-                if (WILD) wild |= Ty<E>::value(x) - Ty<E>::value(x) != 0.f;
-                lds[V::at(row, col)] = x;
+                lds[V::at(row, col)] = row < mm && col0 + col < s.d ? base[(long long)(c0 + (rev ? mm - 1 - row : row)) * s.st + col0 + col] : E(0);
             }
         }
-        return wild != 0;
     }
 };
 
@@ -235,8 +242,8 @@ template <class E, int W, bool VEC> struct Tile {
 // fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel).
 // A chunk: the three tiles go to LDS (the next chunk's loads are in flight meanwhile); the lower-triangular 16 x 16 tiles of the scores are dealt to the
 // waves and exchanged through LDS; then every wave forms its columns of the output and of the state.
-// The products run over whole tiles, tokens behind the row's own weighted with zero: a chunk whose c holds a NaN or infinity (`wild`, seen on the way into
-// LDS, 1 % of the time) forms its output's sums term by term up to the row's own token, so that nothing reaches the rows in front of it.
+// The products run over whole tiles, tokens behind the row's own weighted with zero, which a NaN or infinity in c would pass through: it enters them as zero,
+// and its column of the output (from its row on) and of the state are made NaN behind them.
 template <class E, int DA, int NCT, bool OUT, bool VEC, int SPLIT>
 __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanArgs g) {
     using Y = Ty<E>;
@@ -247,7 +254,6 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     using VP = View<E, C>;
     __shared__ __align__(16) E lb[VA::elems(C)], lc[VC::elems(C)], la[OUT ? VA::elems(C) : 1], lp[OUT ? VP::elems(C) : 1];      // lp: scores [i][j]
     __shared__ float pw[C + 1];                              // a^n
-    __shared__ int wild[2];                                  // (of this chunk and the next)
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
     int id = blockIdx.x;
@@ -281,7 +287,6 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     if (nch > 0) fetch(0);
 
     if (tid <= C) pw[tid] = dpow(l2, tid);
-    if (tid < 2) wild[tid] = 0;
     if (OUT) {
         // rows behind the sequence's last token: zero
         const int cw = min(CB, dc - col0), first = max(t0, n);
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     for (int ct = 0; ct < NCT; ++ct) vcol[ct] = VC::column(lane, w * NCT + ct);
     const VP vp(lane);
 
-    auto chunk = [&](int c0, int mm, bool careful) {
+    auto chunk = [&](int c0, int mm) {
         if (OUT) {
             // tiles (ti, tj <= ti), dealt in turn
             int ti = 0, tj = w;
@@ -356,6 +361,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                 while (tj > ti) { tj -= ti + 1; ++ti; }
             }
         }
+        bool spoilt = false;
         frag vf[NJ][NCT];
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
@@ -369,6 +375,18 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
 #pragma unroll
                 for (int ct = 0; ct < NCT; ++ct) sf[d][ct] = Y::pack(S[ct] + d * TPK);
             __syncthreads();                              // the scores are complete
+            unsigned x = 0;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int ct = 0; ct < NCT; ++ct) x |= Y::wild(vf[j][ct]);
+            spoilt = __any(x != 0);
+            if (spoilt) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = Y::tame(vf[j][ct]);
+            }
 #pragma unroll
             for (int ti = 0; ti < NTI; ++ti) {
                 if (ti * 16 < mm) {
@@ -385,19 +403,9 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     const float past = pw[ti * 16 + ls + e];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) acc[ct] *= past;
-                    if (careful) {
-#pragma unroll 1
-                        for (int j = 0; j <= ti * 16 + ls; ++j) {
-                            const float p = Y::value(lp[VP::at(ti * 16 + ls, j)]);
-#pragma unroll
-                            for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-                                for (int x = 0; x < 4; ++x) acc[ct][x] += p * Y::value(lc[VC::at(j, (w * NCT + ct) * 16 + lg * 4 + x)]);
-                        }
-                    }
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
-                        if (j * KS <= ti * 16 + 15 && !careful) {
+                        if (j * KS <= ti * 16 + 15) {
                             const frag pf = vp.rows(lp, ti * 16, j);
 #pragma unroll
                             for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf, acc[ct]);
@@ -447,18 +455,37 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                 }
             }
         }
+        if (spoilt) {
+            auto first = [&](int c) {                     // the first row whose value of column c is not finite
+                int j = 0;
+                while (j < mm && Y::value(lc[VC::at(j, c)]) - Y::value(lc[VC::at(j, c)]) == 0.f) ++j;
+                return j;
+            };
+#pragma unroll 1
+            for (int x = 0; x < NCT * 4; ++x) {           // (this lane's own outputs, overwritten)
+                const int c = (w * NCT + x / 4) * 16 + lg * 4 + x % 4, from = first(c);
+#pragma unroll 1
+                for (int i = ls; i < mm; i += 16)
+                    if (i >= from && col0 + c < dc) put(po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot + col0 + c, NAN);
+            }
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) {
+                const float add = first((w * NCT + ct) * 16 + ls) < mm ? NAN : 0.f;
+#pragma unroll
+                for (int ta = 0; ta < NTA; ++ta) S[ct][ta] += add;
+            }
+        }
     };
 
     for (int cc = 0; cc < nch; ++cc) {
         const int c0 = t0 + (rev ? nch - 1 - cc : cc) * C, mm = min(C, t1 - c0);
         __syncthreads();                                  // (the previous chunk's tiles have been read)
-        if (OUT) ra.template store<false>(la, r.a, pa, c0, mm, rev, 0, tid);
-        rb.template store<false>(lb, r.b, pb, c0, mm, rev, 0, tid);
-        if (rc.template store<OUT>(lc, r.c, pc, c0, mm, rev, col0, tid)) wild[cc & 1] = 1;
-        if (OUT && tid == 0) wild[(cc + 1) & 1] = 0;
+        if (OUT) ra.store(la, r.a, pa, c0, mm, rev, 0, tid);
+        rb.store(lb, r.b, pb, c0, mm, rev, 0, tid);
+        rc.store(lc, r.c, pc, c0, mm, rev, col0, tid);
         __syncthreads();
         if (cc + 1 < nch) fetch(cc + 1);                  // in flight under this chunk's products
-        chunk(c0, mm, OUT && __builtin_amdgcn_readfirstlane(wild[cc & 1]));
+        chunk(c0, mm);
     }
 
     float* dst = nullptr;
