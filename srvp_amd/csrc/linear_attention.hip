@@ -23,6 +23,12 @@ namespace {
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
+// what is written in front stays in front (arithmetic may pass): keeps reads of LDS ahead of the products that hide them
+#define PIN __builtin_amdgcn_sched_barrier(0x6)
+#ifndef READ_AHEAD
+#define READ_AHEAD 0
+#endif
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 
 struct Operand {
     const void* p;
@@ -198,35 +204,32 @@ __device__ __forceinline__ void put4(float* p, const f32x4_t& v) { *reinterpret_
 
 // ---- global -> registers -> LDS: C rows x W columns of one operand, zero outside the chunk's tokens and the operand's features.  Row i of the tile is
 // token c0 + i, or c0 + mm - 1 - i in reversed time: everything behind the loader sees time running forwards.
-// VEC: 16 bytes at a time.  The loads carry no condition (rows and columns are clamped to valid ones and zeroed on the way into LDS): a load under a branch
-// makes the compiler wait for every load in flight where the paths meet, three memory latencies a chunk.  Otherwise the elements go straight to LDS in `store`.
+// VEC: 16 bytes at a time, by buffer loads whose bound is the chunk's last row: what lies behind it and behind the operand's features comes as zero, with no
+// condition (a load under a branch makes the compiler wait for every load in flight where the paths meet, three memory latencies a chunk) and one address
+// register.  Otherwise the elements go straight to LDS in `store`.
+constexpr unsigned OUTSIDE = 0x80000000u;      // an offset behind every bound: a chunk is at most 2^30 bytes (see operand())
 template <class E, int W, bool VEC> struct Tile {
     using V = View<E, W>;
     static constexpr int C = Ty<E>::C, VE = Ty<E>::VE, NV = C * W / VE / 256, ROWS = 256 / (W / VE);
     u32x4_t v[NV];
     __device__ __forceinline__ void load(const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) {
         if constexpr (VEC) {
-            const char* p = (const char*)(base + (long long)c0 * s.st);
-            const unsigned step = (unsigned)s.st * sizeof(E), row = tid / (W / VE), col = min(col0 + (int)(tid % (W / VE)) * VE, s.d - VE) * sizeof(E);
+            const unsigned step = (unsigned)s.st * sizeof(E);
+            const int row = tid / (W / VE), col = col0 + (tid % (W / VE)) * VE;
+            const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long long)c0 * s.st), 0, mm * step, 0x00027000);
+            unsigned at = col < s.d ? (unsigned)(rev ? mm - 1 - row : row) * step + col * (unsigned)sizeof(E) : OUTSIDE;      // (rows behind the last, reversed: below zero)
+            const unsigned next = rev ? 0u - ROWS * step : ROWS * step;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const unsigned at = min((int)row + i * ROWS, mm - 1);
-                v[i] = *reinterpret_cast<const u32x4_t*>(p + (size_t)((rev ? mm - 1 - at : at) * step + col));      // (64 tokens are less than 2^31 bytes apart)
-            }
+            for (int i = 0; i < NV; ++i, at += next) v[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
         }
     }
     __device__ __forceinline__ void store(E* lds, const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) const {
         if constexpr (VEC) {
             const int row = tid / (W / VE), col = (tid % (W / VE)) * VE;
-            if (mm == C && s.d - col0 >= W) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) V::put16(lds, row + i * ROWS, col, v[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const bool in = row + i * ROWS < mm && col0 + col < s.d;
-                    V::put16(lds, row + i * ROWS, col, in ? v[i] : u32x4_t{0, 0, 0, 0});
-                }
+            for (int i = 0; i < NV; ++i) {
+                if constexpr (ROWS % 16 == 0) V::put16(lds + i * V::elems(ROWS), row, col, v[i]);      // (the exchange of chunks repeats every 16 rows)
+                else V::put16(lds, row + i * ROWS, col, v[i]);
             }
         } else {
 #pragma unroll 1
@@ -253,14 +256,19 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     using VC = View<E, CB>;
     using VP = View<E, C>;
     __shared__ __align__(16) E lb[VA::elems(C)], lc[VC::elems(C)], la[OUT ? VA::elems(C) : 1], lp[OUT ? VP::elems(C) : 1];      // lp: scores [i][j]
-    __shared__ float pw[C + 1];                              // a^n
+    __shared__ float power[2][2 * C + 4];                    // a^n and scale a^n, n = -C .. C: zero in front of n = 0
+    const float *pw = power[0] + C, *spw = power[1] + C;
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
-    int id = blockIdx.x;
+    // what reads the same tokens (roles, column blocks) follows one another on one XCD, whose L2 (or the memory-side cache, for the role that walks the other
+    // way) then holds them: workgroups go round the 8 XCDs
+    int id = blockIdx.x / 8;
     const int cb = id % g.ncb; id /= g.ncb;
+    const int ro = id % g.nroles;
+    id = id / g.nroles * 8 + blockIdx.x % 8;
     const int h = id % g.H; id /= g.H;
-    const int seg = id % g.nseg; id /= g.nseg;
-    const int b = id % g.B, ro = id / g.B;
+    const int seg = id % g.nseg, b = id / g.nseg;
+    if (b >= g.B) return;
     const Role& r = g.r[ro];
     const long long bh = (long long)b * g.H + h;
     const int da = r.a.d, dc = r.c.d, col0 = cb * CB, rev = r.rev, e = rev ? 0 : 1;
@@ -286,7 +294,10 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
     };
     if (nch > 0) fetch(0);
 
-    if (tid <= C) pw[tid] = dpow(l2, tid);
+    if (tid <= 2 * C) {
+        power[0][tid] = tid < C ? 0.f : dpow(l2, tid - C);
+        power[1][tid] = power[0][tid] * g.scale;
+    }
     if (OUT) {
         // rows behind the sequence's last token: zero
         const int cw = min(CB, dc - col0), first = max(t0, n);
@@ -324,15 +335,6 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     S[ct][ta][i] = (src && a < da && c < dc) ? mul * src[(long long)a * r.init_a + (long long)c * r.init_c] : 0.f;
                 }
     }
-    float near[4], next[4];                               // a^(i-j) inside a diagonal tile (0 above it); a^(16 + i - j) for the tile left of it
-    if (OUT) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int gap = ls - lg * 4 - x;
-            near[x] = gap >= 0 ? dpow(l2, gap) : 0.f;
-            next[x] = dpow(l2, 16 + gap);
-        }
-    }
     const VA va(lane);
     int vcol[NCT];
 #pragma unroll
@@ -341,24 +343,24 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
 
     auto chunk = [&](int c0, int mm) {
         if (OUT) {
-            // tiles (ti, tj <= ti), dealt in turn
-            int ti = 0, tj = w;
-            while (tj > ti) { tj -= ti + 1; ++ti; }
-            while (ti < NTI && (ti * 16 < mm)) {
+            // Tiles (ti, tj <= ti).  bf16: wave w has (w, w) and one more, waves 0 and 1 a third: (2, 0), (3, 0); (2, 1), (3, 1); (3, 2); (1, 0).
+            // fp32: (0, 0), (1, 1), (1, 0).  Those on the diagonal come first: they alone have scores to be left out.
+            auto score = [&](int ti, int tj, bool diagonal) {
                 f32x4_t P = {0, 0, 0, 0};
 #pragma unroll
                 for (int d = 0; d < ND; ++d) P = Y::mfma(va.rows(lb, tj * 16, d), va.rows(la, ti * 16, d), P);
-                if (tj == ti) {
+                const float* f = spw + (ti - tj) * 16 + ls - lg * 4;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) P[x] = ls >= lg * 4 + x ? P[x] * near[x] : 0.f;
-                } else {
-                    const float back = pw[16 * (ti - tj - 1)];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) P[x] *= next[x] * back;
-                }
+                for (int x = 0; x < 4; ++x) P[x] = diagonal && ls < lg * 4 + x ? 0.f : P[x] * f[-x];
                 put4(lp + VP::at(ti * 16 + ls, tj * 16 + lg * 4), P);      // bf16: the scores are rounded once
-                tj += 4;
-                while (tj > ti) { tj -= ti + 1; ++ti; }
+            };
+            if constexpr (NTI == 4) {
+                score(w, w, true);
+                score(w < 2 ? 2 : w == 2 ? 3 : 1, w < 3 ? w : 0, false);
+                if (w < 2) score(3, w, false);
+            } else {
+                if (w < 2) score(w, w, true);
+                else if (w == 2) score(1, 0, false);
             }
         }
         bool spoilt = false;
@@ -387,44 +389,56 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = Y::tame(vf[j][ct]);
             }
+            // output^T tiles: rows = columns of c (4 lg + ..), column = token ti * 16 + ls
+            frag af[2][ND], pf[2][NJ];
+            auto read = [&](int ti) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) af[ti & 1][d] = va.rows(la, ti * 16, d);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    if (j * KS <= ti * 16 + 15) pf[ti & 1][j] = vp.rows(lp, ti * 16, j);
+            };
+            // stores by offsets whose bound is the chunk's last row, as the loads
+            const unsigned step = (unsigned)r.ot * sizeof(E), next = rev ? 0u - 16 * step : 16 * step;
+            const auto out = __builtin_amdgcn_make_buffer_rsrc(po + (long long)c0 * r.ot, 0, mm * step, 0x00027000);
+            unsigned at[NCT];
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) {
+                const int c = col0 + (w * NCT + ct) * 16 + lg * 4;
+                at[ct] = c < dc ? (unsigned)(rev ? mm - 1 - ls : ls) * step + c * (unsigned)sizeof(E) : OUTSIDE;
+            }
+            if (READ_AHEAD) read(0);
 #pragma unroll
             for (int ti = 0; ti < NTI; ++ti) {
-                if (ti * 16 < mm) {
-                    // output^T tiles: rows = columns of c (4 lg + ..), column = token ti * 16 + ls
-                    f32x4_t acc[NCT];
+                // bf16: all four tiles of 16 tokens in one run of code (with a branch a tile the waits of one tile do not overlap the next's products)
+                if (VEC && sizeof(E) == 2 || ti * 16 < mm) {
+                    if (!READ_AHEAD) read(ti);
+                    else if (ti + 1 < NTI) { read(ti + 1); PIN; }
+                    f32x4_t acc[NCT], old[NCT];
 #pragma unroll
-                    for (int ct = 0; ct < NCT; ++ct) acc[ct] = f32x4_t{0, 0, 0, 0};
+                    for (int ct = 0; ct < NCT; ++ct) acc[ct] = old[ct] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const frag af = va.rows(la, ti * 16, d);
+                    for (int d = 0; d < ND; ++d)
 #pragma unroll
-                        for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(sf[d][ct], af, acc[ct]);
-                    }
-                    const float past = pw[ti * 16 + ls + e];
+                        for (int ct = 0; ct < NCT; ++ct) old[ct] = Y::mfma(sf[d][ct], af[ti & 1][d], old[ct]);
 #pragma unroll
-                    for (int ct = 0; ct < NCT; ++ct) acc[ct] *= past;
+                    for (int j = 0; j < NJ; ++j)
+                        if (j * KS <= ti * 16 + 15)
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        if (j * KS <= ti * 16 + 15) {
-                            const frag pf = vp.rows(lp, ti * 16, j);
+                            for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf[ti & 1][j], acc[ct]);
+                    const float past = spw[ti * 16 + ls + e];
 #pragma unroll
-                            for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf, acc[ct]);
-                        }
-                    }
-                    const int i = ti * 16 + ls;
-                    if (i < mm) {
-                        E* q = po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot;
+                    for (int ct = 0; ct < NCT; ++ct) {
+                        acc[ct] += old[ct] * past;
+                        if constexpr (VEC) {
+                            if constexpr (sizeof(E) == 2) __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{pack2bf(acc[ct][0], acc[ct][1]), pack2bf(acc[ct][2], acc[ct][3])}, out, at[ct], 0, 0);
+                            else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[ct]), out, at[ct], 0, 0);
+                            at[ct] += next;
+                        } else {
+                            const int i = ti * 16 + ls, c = col0 + (w * NCT + ct) * 16 + lg * 4;
 #pragma unroll
-                        for (int ct = 0; ct < NCT; ++ct) {
-                            const int c = col0 + (w * NCT + ct) * 16 + lg * 4;
-                            acc[ct] *= g.scale;
-                            if (VEC) {
-                                if (c < dc) put4(q + c, acc[ct]);
-                            } else {
-#pragma unroll
-                                for (int x = 0; x < 4; ++x)
-                                    if (c + x < dc) put(q + c + x, acc[ct][x]);
-                            }
+                            for (int x = 0; x < 4; ++x)
+                                if (i < mm && c + x < dc) put(po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot + c + x, acc[ct][x]);
                         }
                     }
                 }
@@ -436,22 +450,27 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
         for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
             for (int ta = 0; ta < NTA; ++ta) S[ct][ta] *= all;
+        constexpr int AHEAD = 2;                          // tiles of b in flight under the products
+        frag kf[AHEAD + 1];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            if (j * KS < mm) {
+            if (sizeof(E) == 2 || j * KS < mm) {
+#pragma unroll
+                for (int n = 0; n < AHEAD; ++n) kf[n] = va.cols(lb, j * KS, n);
+                const float* f = pw + mm - e - j * KS - lg * 4;      // (rows behind mm: zero by zero)
                 float wt[KS / 4];
 #pragma unroll
-                for (int x = 0; x < KS / 4; ++x) wt[x] = pw[max(0, mm - e - (j * KS + (x >> 2) * 16 + lg * 4 + (x & 3)))];     // (rows behind mm are zero)
+                for (int x = 0; x < KS / 4; ++x) wt[x] = f[-((x >> 2) * 16 + (x & 3))];
                 frag wv[NCT][SPLIT];
 #pragma unroll
                 for (int ct = 0; ct < NCT; ++ct) Y::template weigh<SPLIT>(vf[j][ct], wt, wv[ct]);
 #pragma unroll
                 for (int ta = 0; ta < NTA; ++ta) {
-                    const frag kf = va.cols(lb, j * KS, ta);
+                    if (ta + AHEAD < NTA) { kf[(ta + AHEAD) % (AHEAD + 1)] = va.cols(lb, j * KS, ta + AHEAD); PIN; }
 #pragma unroll
-                    for (int ct = 0; ct < NCT; ++ct)
+                    for (int x = 0; x < SPLIT; ++x)
 #pragma unroll
-                        for (int x = 0; x < SPLIT; ++x) S[ct][ta] = Y::mfma(kf, wv[ct][x], S[ct][ta]);
+                        for (int ct = 0; ct < NCT; ++ct) S[ct][ta] = Y::mfma(kf[ta % (AHEAD + 1)], wv[ct][x], S[ct][ta]);
                 }
             }
         }
@@ -497,13 +516,15 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
         if (seg == last) { dst = r.fin + bh * (long long)da * dc; mul = r.fin_mul; }
     }
     if (dst) {
+        int row = lg * 4;
+        asm volatile("" : "+v"(row));                     // (or the addresses of the state's first read would be kept, in memory, for its last write)
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
             for (int ta = 0; ta < NTA; ++ta)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int a = ta * 16 + lg * 4 + i, c = ccol + ct * 16;
+                    const int a = ta * 16 + row + i, c = ccol + ct * 16;
                     if (a < da && c < dc) dst[(long long)a * r.init_a + (long long)c * r.init_c] = mul * S[ct][ta][i];
                 }
     }
@@ -660,16 +681,16 @@ bool aligned(const void* p, long long s0, long long s1, long long s2, int d, int
     return ((uintptr_t)p % bytes) == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0 && d % n == 0;
 }
 Operand operand(const void* p, const int64_t* s, int d, int f32) {
-    return Operand{p, s[0], s[1], s[2], d, aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, 16) && s[0] >= 0 && s[0] < (1 << 23) ? 1 : 0};
+    return Operand{p, s[0], s[1], s[2], d, aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, 16) && s[0] >= d && s[0] < (1 << 22) ? 1 : 0};      // (rows apart; 64 of them under 2^30 bytes)
 }
 void output(Role& r, void* p, const int64_t* s, int d, int f32) {
     r.o = p; r.ot = s[0]; r.ob = s[1]; r.oh = s[2];
-    r.ovec = aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, f32 ? 16 : 8);
+    r.ovec = aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, f32 ? 16 : 8) && s[0] >= d && s[0] < (1 << 22);
 }
 
 template <class E, int DA, int NCT, int SPLIT>
 void launch_split(const ScanArgs& g, bool out, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)g.nroles * g.B * g.nseg * g.H * g.ncb), wg(256);
+    const dim3 grid((unsigned)g.nroles * g.ncb * ((g.B * g.nseg * g.H + 7) / 8) * 8), wg(256);
     if (out) {
         if (vec) hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, true, SPLIT>), grid, wg, 0, st, g);
         else hipLaunchKernelGGL((scan_kernel<E, DA, NCT, true, false, SPLIT>), grid, wg, 0, st, g);
