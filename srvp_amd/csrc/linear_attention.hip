@@ -25,9 +25,6 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 // what is written in front stays in front (arithmetic may pass): keeps reads of LDS ahead of the products that hide them
 #define PIN __builtin_amdgcn_sched_barrier(0x6)
-#ifndef READ_AHEAD
-#define READ_AHEAD 0
-#endif
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 
 struct Operand {
@@ -62,22 +59,25 @@ struct ScanArgs {
 
 __device__ __forceinline__ float dpow(float l2, int n) { return n <= 0 ? 1.f : exp2f(l2 * (float)n); }      // decay^n, n >= 0 (0^0 = 1)
 
-// ---- the two element types.  KS = contraction elements of one step; a fragment holds, for lane (g = lane >> 4, s = lane & 15), the KS/4 elements
-// whose index in the step is 4g .. 4g+3 (and 16 + 4g .. for bf16) of row / column s.  That order is the one in which a 16x16 accumulator tile holds its
-// rows, so a product's result is the next product's operand without leaving the registers.
+// ---- the two element types.  KS = contraction elements of one step; lane (g = lane >> 4, s = lane & 15) holds KS/4 of them, of row / column s.
+//
+// Over features (scores, a S): bf16 8g .. 8g+7 of every 32, 16 bytes of a row.  The state's tiles lie so that they are the next product's operand without
+// leaving the registers: a 16x16 accumulator has rows 4g .. 4g+3 in lane group g, so tiles 2d and 2d+1 are given the features 32d + 8g + {0..3} and {4..7}
+// (`feature`).  Columns likewise where a wave owns 32 of them (`col_of`): a lane's two tiles are 8 neighbouring columns of the output, 16 bytes.
+// Over tokens: 4g .. 4g+3 and 16 + 4g .. of every 32, what a transposing read gives; the scores are laid down in that order.
+// fp32: 4g .. 4g+3 of every 16, everything in its natural place.
 //
 // View<E, W>: a tile of W features a row in LDS, read as fragments along its rows (contraction over features) and across them (over tokens).
-// bf16: 8-byte chunks, exchanged within every 128 bytes of a row by chunk ^= swz(row).  A wave reads 16 rows of one chunk, or (ds_read_b64_tr_b16) 4 rows of 4
-// chunks, 16 lanes at a time: both touch each pair of the 32 banks once.  (Rows padded by 16 bytes instead: two-way conflicts in both, 43 % of the LDS time.)
-// fp32: rows padded by 16 bytes.
+// bf16: 16-byte units, exchanged within every 256 bytes (128 for W = 64) by unit ^= swz(row).  16 lanes read one unit of 16 rows, write whole rows, or
+// (ds_read_b64_tr_b16) read half of 4 units of 4 rows: all of them touch every bank at most once.  fp32: rows padded by 16 bytes.
 template <class E> struct Ty;
 template <class E, int W> struct View;
-
-__device__ __forceinline__ int swz(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
 
 template <> struct Ty<bf16_t> {
     static constexpr int KS = 32, TPK = 2, C = 64, VE = 8;
     typedef s16x8_t frag;
+    static __device__ __forceinline__ int feature(int tile, int g) { return (tile >> 1) * 32 + g * 8 + (tile & 1) * 4; }      // of row 4g of a tile
+    template <int NCT> static __device__ __forceinline__ int col_of(int w, int ct, int i) { return NCT == 2 ? w * 32 + (i >> 2) * 8 + ct * 4 + (i & 3) : w * 16 + i; }
     static __device__ __forceinline__ float value(bf16_t x) { return bf2f(x); }
     // whether an element is NaN or infinite (the exponent's bits and one more carry into the sign's)
     static __device__ __forceinline__ unsigned wild(const frag& x) {
@@ -122,46 +122,45 @@ template <int W> struct View<bf16_t, W> {
     typedef s16x8_t frag;
     static constexpr int RB = W * 2;                       // bytes of a row
     static constexpr int elems(int rows) { return rows * W; }
-    static __device__ __forceinline__ int at(int row, int col) { return row * W + ((((col >> 2) ^ swz(row)) << 2) | (col & 3)); }      // (the low 4 bits of the chunk)
-    int r[4], t[4];                                        // byte offsets of the lane's chunks 4x: row s; row 4g + (s >> 2), chunk s & 3
+    static __device__ __forceinline__ int swz(int row) { return W == 64 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3); }
+    static __device__ __forceinline__ int at(int row, int col) { return row * W + ((((col >> 3) ^ swz(row)) << 3) | (col & 7)); }
+    int r[4], t[4];                                        // byte offsets of the lane's units 4x + ..: row s, unit g; row 4g + (s >> 2), unit s & 3
     __device__ __forceinline__ explicit View(int lane) {
         const int g = lane >> 4, s = lane & 15, q = 4 * g + (s >> 2);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            r[x] = s * RB + (((4 * x + g) ^ swz(s)) << 3);
-            t[x] = q * RB + (((4 * x + (s & 3)) ^ swz(q)) << 3);
+            r[x] = s * RB + (((4 * x + g) ^ swz(s)) << 4);
+            t[x] = q * RB + (((4 * x + (s & 3)) ^ swz(q)) << 4);
         }
     }
     // rows row0 + s, step d of the features
     __device__ __forceinline__ frag rows(const bf16_t* base, int row0, int d) const {
-        const char* p = (const char*)base + row0 * RB;
-        const s16x4_t lo = *reinterpret_cast<const s16x4_t*>(p + ((2 * d) >> 2) * 128 + r[(2 * d) & 3]);
-        const s16x4_t hi = *reinterpret_cast<const s16x4_t*>(p + ((2 * d + 1) >> 2) * 128 + r[(2 * d + 1) & 3]);
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return *reinterpret_cast<const s16x8_t*>((const char*)base + row0 * RB + (d >> 2) * 256 + r[d & 3]);
     }
-    // byte offset of the lane's chunk of columns 16 c ..
-    static __device__ __forceinline__ int column(int lane, int c) {
-        const int s = lane & 15, q = 4 * (lane >> 4) + (s >> 2);
-        return q * RB + (((4 * c + (s & 3)) ^ swz(q)) << 3);
+    // tile c of the features, tokens row0 .. row0 + 31.  ds_read_b64_tr_b16: lane s of a 16-lane group receives column s of the 4 x 16 block whose row j the
+    // lanes 4j .. 4j+3 address
+    __device__ __forceinline__ frag cols(const bf16_t* base, int row0, int c) const { return at_column(base, row0, (c >> 3) * 256 + t[(c >> 1) & 3] + (c & 1) * 8); }
+    // the same for tile ct of wave w's columns: the byte offset, and the read
+    template <int NCT> static __device__ __forceinline__ int column(int lane, int w, int ct) {
+        const int s = lane & 15, q = 4 * (lane >> 4) + (s >> 2), col = Ty<bf16_t>::col_of<NCT>(w, ct, 4 * (s & 3));
+        return at(q, col) * 2;
     }
-    // columns 16 c + s, tokens row0 .. row0 + 31.  ds_read_b64_tr_b16: lane s of a 16-lane group receives column s of the 4 x 16 block whose row j the lanes
-    // 4j .. 4j+3 address
-    __device__ __forceinline__ frag cols(const bf16_t* base, int row0, int c) const { return at_column(base, row0, (c >> 2) * 128 + t[c & 3]); }
     static __device__ __forceinline__ frag at_column(const bf16_t* base, int row0, int off) {
         const char* p = (const char*)base + row0 * RB + off;
         const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)p);
         const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(p + 16 * RB));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
-    static __device__ __forceinline__ void put16(bf16_t* base, int row, int col, const u32x4_t& v) {
-        *reinterpret_cast<uint2*>(base + at(row, col)) = make_uint2(v.x, v.y);
-        *reinterpret_cast<uint2*>(base + at(row, col + 4)) = make_uint2(v.z, v.w);
-    }
+    static __device__ __forceinline__ void put16(bf16_t* base, int row, int col, const u32x4_t& v) { *reinterpret_cast<u32x4_t*>(base + at(row, col)) = v; }
+    // where the scores of row `row` with tokens 16 tile + 4g .. lie
+    static __device__ __forceinline__ int score(int row, int tile, int g) { return at(row, (tile >> 1) * 32 + g * 8 + (tile & 1) * 4); }
 };
 
 template <> struct Ty<float> {
     static constexpr int KS = 16, TPK = 1, C = 32, VE = 4;
     typedef f32x4_t frag;
+    static __device__ __forceinline__ int feature(int tile, int g) { return tile * 16 + g * 4; }
+    template <int NCT> static __device__ __forceinline__ int col_of(int w, int ct, int i) { return (w * NCT + ct) * 16 + i; }
     static __device__ __forceinline__ float value(float x) { return x; }
     static __device__ __forceinline__ unsigned wild(const frag& x) {
         const u32x4_t v = __builtin_bit_cast(u32x4_t, x), y = (v & 0x7fffffffu) + 0x00800000u;
@@ -188,13 +187,14 @@ template <int W> struct View<float, W> {
     int r, t;
     __device__ __forceinline__ explicit View(int lane) : r((lane & 15) * LD + (lane >> 4) * 4), t((lane >> 4) * 4 * LD + (lane & 15)) {}
     __device__ __forceinline__ frag rows(const float* base, int row0, int d) const { return *reinterpret_cast<const f32x4_t*>(base + row0 * LD + d * 16 + r); }
-    static __device__ __forceinline__ int column(int lane, int c) { return (lane >> 4) * 4 * LD + (lane & 15) + c * 16; }
+    template <int NCT> static __device__ __forceinline__ int column(int lane, int w, int ct) { return (lane >> 4) * 4 * LD + (lane & 15) + (w * NCT + ct) * 16; }
     __device__ __forceinline__ frag cols(const float* base, int row0, int c) const { return at_column(base, row0, t + c * 16); }
     static __device__ __forceinline__ frag at_column(const float* base, int row0, int off) {
         const float* p = base + row0 * LD + off;
         return frag{p[0], p[LD], p[2 * LD], p[3 * LD]};
     }
     static __device__ __forceinline__ void put16(float* base, int row, int col, const u32x4_t& v) { *reinterpret_cast<u32x4_t*>(base + at(row, col)) = v; }
+    static __device__ __forceinline__ int score(int row, int tile, int g) { return at(row, tile * 16 + g * 4); }
 };
 
 __device__ __forceinline__ void put(bf16_t* p, float v) { *p = f2bf(v); }
@@ -212,13 +212,17 @@ template <class E, int W, bool VEC> struct Tile {
     using V = View<E, W>;
     static constexpr int C = Ty<E>::C, VE = Ty<E>::VE, NV = C * W / VE / 256, ROWS = 256 / (W / VE);
     u32x4_t v[NV];
-    __device__ __forceinline__ void load(const Operand& s, const E* base, int c0, int mm, int rev, int col0, int tid) {
+    // chunk: its first token; step: bytes of a token; col: this thread's columns, in bytes (column())
+    static __device__ __forceinline__ unsigned column(int d, int col0, int tid) {
+        const int c = col0 + tid % (W / VE) * VE;
+        return c < d ? c * (unsigned)sizeof(E) : OUTSIDE;
+    }
+    __device__ __forceinline__ void load(const char* chunk, unsigned step, unsigned col, int mm, int rev, int tid) {
         if constexpr (VEC) {
-            const unsigned step = (unsigned)s.st * sizeof(E);
-            const int row = tid / (W / VE), col = col0 + (tid % (W / VE)) * VE;
-            const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long long)c0 * s.st), 0, mm * step, 0x00027000);
-            unsigned at = col < s.d ? (unsigned)(rev ? mm - 1 - row : row) * step + col * (unsigned)sizeof(E) : OUTSIDE;      // (rows behind the last, reversed: below zero)
+            const int row = tid / (W / VE);
+            const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)chunk, 0, mm * step, 0x00027000);
             const unsigned next = rev ? 0u - ROWS * step : ROWS * step;
+            unsigned at = (unsigned)(rev ? mm - 1 - row : row) * step + col;      // (rows behind the last, reversed: below zero)
 #pragma unroll
             for (int i = 0; i < NV; ++i, at += next) v[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
         }
@@ -286,11 +290,13 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
 
     Tile<E, DA, VEC> ra, rb;
     Tile<E, CB, VEC> rc;
+    const unsigned stepa = (unsigned)r.a.st * sizeof(E), stepb = (unsigned)r.b.st * sizeof(E), stepc = (unsigned)r.c.st * sizeof(E);
+    const unsigned colb = Tile<E, DA, VEC>::column(da, 0, tid), colc = Tile<E, CB, VEC>::column(dc, col0, tid);
     auto fetch = [&](int cc) {
         const int c0 = t0 + (rev ? nch - 1 - cc : cc) * C, mm = min(C, t1 - c0);
-        if (OUT) ra.load(r.a, pa, c0, mm, rev, 0, tid);
-        rb.load(r.b, pb, c0, mm, rev, 0, tid);
-        rc.load(r.c, pc, c0, mm, rev, col0, tid);
+        if (OUT) ra.load((const char*)pa + (unsigned long long)c0 * stepa, stepa, colb, mm, rev, tid);
+        rb.load((const char*)pb + (unsigned long long)c0 * stepb, stepb, colb, mm, rev, tid);
+        rc.load((const char*)pc + (unsigned long long)c0 * stepc, stepc, colc, mm, rev, tid);
     };
     if (nch > 0) fetch(0);
 
@@ -315,8 +321,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
         for (int i = tid; i < VP::elems(C); i += 256) lp[i] = E(0);
     }
 
-    // state: tile (ta, ct) holds rows 16 ta + 4 lg + {0..3}, column ccol + 16 ct
-    const int ccol = col0 + w * 16 * NCT + ls;
+    // state: tile (ta, ct) holds rows feature(ta, lg) + {0..3}, column col_of(w, ct, ls)
     f32x4_t S[NCT][NTA];
     {
         const float* src = nullptr;
@@ -331,14 +336,14 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
             for (int ta = 0; ta < NTA; ++ta)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int a = ta * 16 + lg * 4 + i, c = ccol + ct * 16;
+                    const int a = Y::feature(ta, lg) + i, c = col0 + Y::template col_of<NCT>(w, ct, ls);
                     S[ct][ta][i] = (src && a < da && c < dc) ? mul * src[(long long)a * r.init_a + (long long)c * r.init_c] : 0.f;
                 }
     }
     const VA va(lane);
     int vcol[NCT];
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) vcol[ct] = VC::column(lane, w * NCT + ct);
+    for (int ct = 0; ct < NCT; ++ct) vcol[ct] = VC::template column<NCT>(lane, w, ct);
     const VP vp(lane);
 
     auto chunk = [&](int c0, int mm) {
@@ -351,8 +356,11 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                 for (int d = 0; d < ND; ++d) P = Y::mfma(va.rows(lb, tj * 16, d), va.rows(la, ti * 16, d), P);
                 const float* f = spw + (ti - tj) * 16 + ls - lg * 4;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) P[x] = diagonal && ls < lg * 4 + x ? 0.f : P[x] * f[-x];
-                put4(lp + VP::at(ti * 16 + ls, tj * 16 + lg * 4), P);      // bf16: the scores are rounded once
+                for (int x = 0; x < 4; ++x) {
+                    P[x] *= f[-x];
+                    if (diagonal) P[x] = ls < lg * 4 + x ? 0.f : P[x];
+                }
+                put4(lp + VP::score(ti * 16 + ls, tj, lg), P);      // bf16: the scores are rounded once
             };
             if constexpr (NTI == 4) {
                 score(w, w, true);
@@ -404,16 +412,16 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
             unsigned at[NCT];
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct) {
-                const int c = col0 + (w * NCT + ct) * 16 + lg * 4;
+                const int c = col0 + Y::template col_of<NCT>(w, ct, lg * 4);
                 at[ct] = c < dc ? (unsigned)(rev ? mm - 1 - ls : ls) * step + c * (unsigned)sizeof(E) : OUTSIDE;
             }
-            if (READ_AHEAD) read(0);
+            read(0);
 #pragma unroll
             for (int ti = 0; ti < NTI; ++ti) {
                 // bf16: all four tiles of 16 tokens in one run of code (with a branch a tile the waits of one tile do not overlap the next's products)
                 if (VEC && sizeof(E) == 2 || ti * 16 < mm) {
-                    if (!READ_AHEAD) read(ti);
-                    else if (ti + 1 < NTI) { read(ti + 1); PIN; }
+                    if (ti + 1 < NTI) read(ti + 1);
+                    PIN;
                     f32x4_t acc[NCT], old[NCT];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) acc[ct] = old[ct] = f32x4_t{0, 0, 0, 0};
@@ -428,14 +436,23 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                             for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf[ti & 1][j], acc[ct]);
                     const float past = spw[ti * 16 + ls + e];
 #pragma unroll
-                    for (int ct = 0; ct < NCT; ++ct) {
-                        acc[ct] += old[ct] * past;
-                        if constexpr (VEC) {
+                    for (int ct = 0; ct < NCT; ++ct) acc[ct] += old[ct] * past;
+                    if constexpr (VEC && sizeof(E) == 2 && NCT == 2) {
+                        const u32x4_t v = {pack2bf(acc[0][0], acc[0][1]), pack2bf(acc[0][2], acc[0][3]), pack2bf(acc[1][0], acc[1][1]), pack2bf(acc[1][2], acc[1][3])};
+                        __builtin_amdgcn_raw_buffer_store_b128(v, out, at[0], 0, 0);
+                        at[0] += next;
+                    } else if constexpr (VEC) {
+#pragma unroll
+                        for (int ct = 0; ct < NCT; ++ct) {
                             if constexpr (sizeof(E) == 2) __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{pack2bf(acc[ct][0], acc[ct][1]), pack2bf(acc[ct][2], acc[ct][3])}, out, at[ct], 0, 0);
                             else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[ct]), out, at[ct], 0, 0);
                             at[ct] += next;
-                        } else {
-                            const int i = ti * 16 + ls, c = col0 + (w * NCT + ct) * 16 + lg * 4;
+                        }
+                    } else {
+                        const int i = ti * 16 + ls;
+#pragma unroll
+                        for (int ct = 0; ct < NCT; ++ct) {
+                            const int c = col0 + Y::template col_of<NCT>(w, ct, lg * 4);
 #pragma unroll
                             for (int x = 0; x < 4; ++x)
                                 if (i < mm && c + x < dc) put(po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot + c + x, acc[ct][x]);
@@ -482,14 +499,14 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
             };
 #pragma unroll 1
             for (int x = 0; x < NCT * 4; ++x) {           // (this lane's own outputs, overwritten)
-                const int c = (w * NCT + x / 4) * 16 + lg * 4 + x % 4, from = first(c);
+                const int c = Y::template col_of<NCT>(w, x / 4, lg * 4 + x % 4), from = first(c);
 #pragma unroll 1
                 for (int i = ls; i < mm; i += 16)
                     if (i >= from && col0 + c < dc) put(po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot + col0 + c, NAN);
             }
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct) {
-                const float add = first((w * NCT + ct) * 16 + ls) < mm ? NAN : 0.f;
+                const float add = first(Y::template col_of<NCT>(w, ct, ls)) < mm ? NAN : 0.f;
 #pragma unroll
                 for (int ta = 0; ta < NTA; ++ta) S[ct][ta] += add;
             }
@@ -516,15 +533,15 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
         if (seg == last) { dst = r.fin + bh * (long long)da * dc; mul = r.fin_mul; }
     }
     if (dst) {
-        int row = lg * 4;
-        asm volatile("" : "+v"(row));                     // (or the addresses of the state's first read would be kept, in memory, for its last write)
+        int g4 = lg;
+        asm volatile("" : "+v"(g4));                      // (or the addresses of the state's first read would be kept, in memory, for its last write)
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
             for (int ta = 0; ta < NTA; ++ta)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int a = ta * 16 + row + i, c = ccol + ct * 16;
+                    const int a = Y::feature(ta, g4) + i, c = col0 + Y::template col_of<NCT>(w, ct, ls);
                     if (a < da && c < dc) dst[(long long)a * r.init_a + (long long)c * r.init_c] = mul * S[ct][ta][i];
                 }
     }
@@ -685,7 +702,7 @@ Operand operand(const void* p, const int64_t* s, int d, int f32) {
 }
 void output(Role& r, void* p, const int64_t* s, int d, int f32) {
     r.o = p; r.ot = s[0]; r.ob = s[1]; r.oh = s[2];
-    r.ovec = aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, f32 ? 16 : 8) && s[0] >= d && s[0] < (1 << 22);
+    r.ovec = aligned(p, s[0], s[1], s[2], d, f32 ? 4 : 2, 16) && s[0] >= d && s[0] < (1 << 22);
 }
 
 template <class E, int DA, int NCT, int SPLIT>
