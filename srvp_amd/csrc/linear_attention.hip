@@ -298,7 +298,6 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
         rb.load((const char*)pb + (unsigned long long)c0 * stepb, stepb, colb, mm, rev, tid);
         rc.load((const char*)pc + (unsigned long long)c0 * stepc, stepc, colc, mm, rev, tid);
     };
-    if (nch > 0) fetch(0);
 
     if (tid <= 2 * C) {
         power[0][tid] = tid < C ? 0.f : dpow(l2, tid - C);
@@ -321,7 +320,14 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
         for (int i = tid; i < VP::elems(C); i += 256) lp[i] = E(0);
     }
 
-    // state: tile (ta, ct) holds rows feature(ta, lg) + {0..3}, column col_of(w, ct, ls)
+    // state: tile (ta, ct) holds rows feature(ta, lg) + {0..3}, column col_of(w, ct, ls).  Read and written through a bound too, the four rows of a lane together
+    // where they are neighbours (with a branch an element: 24 us more for 512 states of 128 x 128 read, 14 written).
+    const unsigned state_bytes = (unsigned)(da * dc) * 4u, bya = (unsigned)r.init_a * 4u, byc = (unsigned)r.init_c * 4u;
+    auto place = [&](int ta, int ct, int g4, int i) {
+        const int a = Y::feature(ta, g4) + i, c = col0 + Y::template col_of<NCT>(w, ct, ls);
+        return a < da && c < dc ? (unsigned)a * bya + (unsigned)c * byc : OUTSIDE;
+    };
+    auto in_fours = [&](const float* p) { return r.init_a == 1 && da % 4 == 0 && (uintptr_t)p % 16 == 0; };
     f32x4_t S[NCT][NTA];
     {
         const float* src = nullptr;
@@ -330,16 +336,27 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
             if (r.prefix) src = r.prefix + (bh * g.nseg + seg) * (long long)da * dc;
             else if (r.init) { src = r.init + bh * (long long)da * dc; mul = r.init_mul; }
         }
+        const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, state_bytes, 0x00027000);
+        if (!src) {
 #pragma unroll
-        for (int ct = 0; ct < NCT; ++ct)
+            for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int ta = 0; ta < NTA; ++ta)
+                for (int ta = 0; ta < NTA; ++ta) S[ct][ta] = f32x4_t{0, 0, 0, 0};
+        } else if (in_fours(src)) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int a = Y::feature(ta, lg) + i, c = col0 + Y::template col_of<NCT>(w, ct, ls);
-                    S[ct][ta][i] = (src && a < da && c < dc) ? mul * src[(long long)a * r.init_a + (long long)c * r.init_c] : 0.f;
-                }
+            for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                for (int ta = 0; ta < NTA; ++ta) S[ct][ta] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(from, place(ta, ct, lg, 0), 0, 0)) * mul;
+        } else {
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                for (int ta = 0; ta < NTA; ++ta)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[ct][ta][i] = mul * __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(from, place(ta, ct, lg, i), 0, 0));
+        }
     }
+    if (nch > 0) fetch(0);
     const VA va(lane);
     int vcol[NCT];
 #pragma unroll
@@ -398,14 +415,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = Y::tame(vf[j][ct]);
             }
             // output^T tiles: rows = columns of c (4 lg + ..), column = token ti * 16 + ls
-            frag af[2][ND], pf[2][NJ];
-            auto read = [&](int ti) {
-#pragma unroll
-                for (int d = 0; d < ND; ++d) af[ti & 1][d] = va.rows(la, ti * 16, d);
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-                    if (j * KS <= ti * 16 + 15) pf[ti & 1][j] = vp.rows(lp, ti * 16, j);
-            };
+            frag af[ND], pf[NJ];
             // stores by offsets whose bound is the chunk's last row, as the loads
             const unsigned step = (unsigned)r.ot * sizeof(E), next = rev ? 0u - 16 * step : 16 * step;
             const auto out = __builtin_amdgcn_make_buffer_rsrc(po + (long long)c0 * r.ot, 0, mm * step, 0x00027000);
@@ -415,25 +425,27 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                 const int c = col0 + Y::template col_of<NCT>(w, ct, lg * 4);
                 at[ct] = c < dc ? (unsigned)(rev ? mm - 1 - ls : ls) * step + c * (unsigned)sizeof(E) : OUTSIDE;
             }
-            read(0);
 #pragma unroll
             for (int ti = 0; ti < NTI; ++ti) {
                 // bf16: all four tiles of 16 tokens in one run of code (with a branch a tile the waits of one tile do not overlap the next's products)
                 if (VEC && sizeof(E) == 2 || ti * 16 < mm) {
-                    if (ti + 1 < NTI) read(ti + 1);
-                    PIN;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) af[d] = va.rows(la, ti * 16, d);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        if (j * KS <= ti * 16 + 15) pf[j] = vp.rows(lp, ti * 16, j);
                     f32x4_t acc[NCT], old[NCT];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) acc[ct] = old[ct] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
 #pragma unroll
-                        for (int ct = 0; ct < NCT; ++ct) old[ct] = Y::mfma(sf[d][ct], af[ti & 1][d], old[ct]);
+                        for (int ct = 0; ct < NCT; ++ct) old[ct] = Y::mfma(sf[d][ct], af[d], old[ct]);
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
                         if (j * KS <= ti * 16 + 15)
 #pragma unroll
-                            for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf[ti & 1][j], acc[ct]);
+                            for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf[j], acc[ct]);
                     const float past = spw[ti * 16 + ls + e];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) acc[ct] += old[ct] * past;
@@ -533,17 +545,22 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
         if (seg == last) { dst = r.fin + bh * (long long)da * dc; mul = r.fin_mul; }
     }
     if (dst) {
+        const auto to = __builtin_amdgcn_make_buffer_rsrc(dst, 0, state_bytes, 0x00027000);
         int g4 = lg;
-        asm volatile("" : "+v"(g4));                      // (or the addresses of the state's first read would be kept, in memory, for its last write)
+        asm volatile("" : "+v"(g4));                      // (or the offsets of the state's read would be kept, in memory, for its write)
+        if (in_fours(dst)) {
 #pragma unroll
-        for (int ct = 0; ct < NCT; ++ct)
+            for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int ta = 0; ta < NTA; ++ta)
+                for (int ta = 0; ta < NTA; ++ta) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, S[ct][ta] * mul), to, place(ta, ct, g4, 0), 0, 0);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int a = Y::feature(ta, g4) + i, c = col0 + Y::template col_of<NCT>(w, ct, ls);
-                    if (a < da && c < dc) dst[(long long)a * r.init_a + (long long)c * r.init_c] = mul * S[ct][ta][i];
-                }
+            for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                for (int ta = 0; ta < NTA; ++ta)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, mul * S[ct][ta][i]), to, place(ta, ct, g4, i), 0, 0);
+        }
     }
 }
 
