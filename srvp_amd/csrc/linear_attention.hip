@@ -99,8 +99,8 @@ template <> struct Ty<bf16_t> {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
     }
     // x * w as a sum of SPLIT bf16 values of 8 significant bits each.  Three are the fp32 product to its last bit, so the state (a result of its own) has fp32's
-    // accuracy.  Two (2^-17) serve the gradients' sums, which only pass into bfloat16 values; the forward pass takes three always, or its output would
-    // depend on whether the state was asked for.
+    // accuracy.  Two (2^-17) serve the gradients' sums, which only pass into bfloat16 values (16 % of the backward pass); the forward pass takes three always,
+    // or its output would depend on whether the state was asked for.
     template <int SPLIT> static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) {
         float f[8];
         unpack8(__builtin_bit_cast(u32x4_t, x), f);
@@ -249,23 +249,32 @@ template <class E, int W, bool VEC> struct Tile {
 // fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel).
 // A chunk: the three tiles go to LDS (the next chunk's loads are in flight meanwhile); the lower-triangular 16 x 16 tiles of the scores are dealt to the
 // waves and exchanged through LDS; then every wave forms its columns of the output and of the state.
+//
+// Bound: HBM, where two workgroups share a CU.  A chunk of bfloat16, 128 features, moves 64 KB: 7400 cycles at the CU's part of 5.3 TB/s; it costs 164 matrix
+// instructions (2600 cycles), 650 others (2600) and 2700 cycles of LDS, in turn within a wave, under each other between the waves.  Measured (16 heads of 128,
+// bfloat16): 512 x 32 forward 61 us = 4.4 TB/s, backward (three roles, each reads three operands) 155; 2048 x 16 (one workgroup a CU: the latency of a chunk's
+// steps, 10 700 cycles) 147 and 330.  fp32 (12 x 192, 4 heads of 64, one chunk a workgroup) 8 and 17 us; 1024 x 16 206 and 526: fp32 products at a sixteenth of the rate.
+// Four waves of 32 columns: eight of 16 read every tile of a and b twice as often; one chunk of 64 tokens: 32 halve the products between barriers.  The limit
+// is the registers: 255 of 256 (the state 64, the loads in flight 48), whatever is added is spilt.
+//
 // The products run over whole tiles, tokens behind the row's own weighted with zero, which a NaN or infinity in c would pass through: it enters them as zero,
 // and its column of the output (from its row on) and of the state are made NaN behind them.
 template <class E, int DA, int NCT, bool OUT, bool VEC, int SPLIT>
-__global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanArgs g) {
+__global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kernel(const ScanArgs g) {
     using Y = Ty<E>;
     typedef typename Y::frag frag;
     constexpr int C = Y::C, KS = Y::KS, TPK = Y::TPK, CB = 64 * NCT, ND = DA / KS, NJ = C / KS, NTA = DA / 16, NTI = C / 16;
     using VA = View<E, DA>;
     using VC = View<E, CB>;
     using VP = View<E, C>;
-    __shared__ __align__(16) E lb[VA::elems(C)], lc[VC::elems(C)], la[OUT ? VA::elems(C) : 1], lp[OUT ? VP::elems(C) : 1];      // lp: scores [i][j]
+    constexpr int PT = sizeof(E) == 2 ? 2 : 1;              // bf16: a score is the sum of two terms, as the products that formed it are fp32
+    __shared__ __align__(16) E lb[VA::elems(C)], lc[VC::elems(C)], la[OUT ? VA::elems(C) : 1], lp[OUT ? PT * VP::elems(C) : 1];      // lp: scores [term][i][j]
     __shared__ float power[2][2 * C + 4];                    // a^n and scale a^n, n = -C .. C: zero in front of n = 0
     const float *pw = power[0] + C, *spw = power[1] + C;
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
     // what reads the same tokens (roles, column blocks) follows one another on one XCD, whose L2 (or the memory-side cache, for the role that walks the other
-    // way) then holds them: workgroups go round the 8 XCDs
+    // way) then holds them: workgroups go round the 8 XCDs (backward, 512 x 32 x 16 x 128: 179 us; one role behind the other: 184)
     int id = blockIdx.x / 8;
     const int cb = id % g.ncb; id /= g.ncb;
     const int ro = id % g.nroles;
@@ -317,7 +326,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                 for (int c = tid; c < cw; c += 256) put(po + t * r.ot + col0 + c, 0.f);
         }
         // scores above the diagonal tiles: zero, once
-        for (int i = tid; i < VP::elems(C); i += 256) lp[i] = E(0);
+        for (int i = tid; i < PT * VP::elems(C); i += 256) lp[i] = E(0);
     }
 
     // state: tile (ta, ct) holds rows feature(ta, lg) + {0..3}, column col_of(w, ct, ls).  Read and written through a bound too, the four rows of a lane together
@@ -377,7 +386,14 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     P[x] *= f[-x];
                     if (diagonal) P[x] = ls < lg * 4 + x ? 0.f : P[x];
                 }
-                put4(lp + VP::score(ti * 16 + ls, tj, lg), P);      // bf16: the scores are rounded once
+                E* at = lp + VP::score(ti * 16 + ls, tj, lg);
+                put4(at, P);
+                if constexpr (PT == 2) {
+                    // (one term alone: a short sequence's few scores carry their rounding into whole rows of the output, 1.7 times its own rounding)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) P[x] -= Y::value(f2bf(P[x]));
+                    put4(at + VP::elems(C), P);
+                }
             };
             if constexpr (NTI == 4) {
                 score(w, w, true);
@@ -415,7 +431,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = Y::tame(vf[j][ct]);
             }
             // output^T tiles: rows = columns of c (4 lg + ..), column = token ti * 16 + ls
-            frag af[ND], pf[NJ];
+            frag af[ND], pf[PT][NJ];
             // stores by offsets whose bound is the chunk's last row, as the loads
             const unsigned step = (unsigned)r.ot * sizeof(E), next = rev ? 0u - 16 * step : 16 * step;
             const auto out = __builtin_amdgcn_make_buffer_rsrc(po + (long long)c0 * r.ot, 0, mm * step, 0x00027000);
@@ -433,7 +449,9 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     for (int d = 0; d < ND; ++d) af[d] = va.rows(la, ti * 16, d);
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
-                        if (j * KS <= ti * 16 + 15) pf[j] = vp.rows(lp, ti * 16, j);
+                        if (j * KS <= ti * 16 + 15)
+#pragma unroll
+                            for (int x = 0; x < PT; ++x) pf[x][j] = vp.rows(lp + x * VP::elems(C), ti * 16, j);
                     f32x4_t acc[NCT], old[NCT];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) acc[ct] = old[ct] = f32x4_t{0, 0, 0, 0};
@@ -445,7 +463,9 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
                     for (int j = 0; j < NJ; ++j)
                         if (j * KS <= ti * 16 + 15)
 #pragma unroll
-                            for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf[j], acc[ct]);
+                            for (int x = 0; x < PT; ++x)
+#pragma unroll
+                                for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf[x][j], acc[ct]);
                     const float past = spw[ti * 16 + ls + e];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct) acc[ct] += old[ct] * past;
@@ -565,6 +585,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : 2) void scan_kernel(const ScanA
 }
 
 // Segment sums -> the carry in front of every segment, in place.  One thread owns one element of the state and walks the segments in scan order.
+// 512 states of 128 x 128 (67 MB in and out): 12.5 us = 5.4 TB/s.
 struct JoinArgs {
     float* part;
     const float* init[2];
@@ -605,6 +626,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs g) {
 // ---- recurrent form: one token a row, states updated in place.  A workgroup owns one (row, head): the state passes through the registers once
 // (read + written: 8 Dk Dv bytes are the whole cost), columns across the lanes, rows of the state across the rest of the workgroup.
 // Rows that name the same slot are successive tokens of that sequence, in row order: the first of them does the others' work as well.
+// 512 rows x 16 heads of 128 x 128: 224 us = 4.9 TB/s; one row x 4 heads of 64 x 64: 4.6 us, the launch's.
 struct StepArgs {
     const void *q, *k, *v;
     void* o;
@@ -767,14 +789,19 @@ void launch(const ScanArgs& base, const Role* roles, int n, bool out, bool exact
     }
 }
 
-// Segments: with fewer (sequence, head) pairs than the chip has room for, a sequence is cut and its segments walked side by side.
+// Segments: with fewer (sequence, head) pairs than the chip has room for (two workgroups on each of 256 CUs), a sequence is cut into as many segments as fill
+// it, of four chunks or more, walked side by side.  That costs the segments' own sums first and a pass over them, so three segments are the least.  bfloat16, us,
+// whole and cut (pairs x roles; forward unless said):
+//   192, 1024 tokens: 65 and 110 (2 segments)      210, 4096 tokens, backward: 224 and 283 (2)      256, 2048 tokens: 160 and 271 (2)
+//   128, 2048 tokens: 122 and 129 (4); 8192 tokens: 481 and 416; float32, 64 features: 145 and 96      144, 4096 tokens, backward: 220 and 202 (3)
+// Twice as many segments: 8192 x 2 x 16 x 128 115 -> 144, 4096 x 3 x 12 x 128 77 -> 94; half as many: 141 -> 147 (an earlier kernel).
 void segments(const srvp_linear_attention_desc* d, int roles, int* nseg, int* seg_len) {
     const int C = d->elem_f32 ? 32 : 64;
     const long long ncb = (d->Dv + 127) / 128, base = (long long)d->B * d->H * ncb * roles;
     const long long chunks = (d->T + C - 1) / C;
-    long long n = base >= 256 || base == 0 ? 1 : 512 / base;
+    long long n = base == 0 ? 1 : 512 / base;
     if (n > (chunks + 3) / 4) n = (chunks + 3) / 4;
-    if (n < 1) n = 1;
+    if (n < 3) n = 1;
     const long long per = chunks > n ? (chunks + n - 1) / n : 1;
     *seg_len = (int)(per * C);
     *nseg = (int)((chunks + per - 1) / per);
