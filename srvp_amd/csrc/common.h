@@ -98,6 +98,13 @@ __device__ __forceinline__ float act_bwd(float v, int act) {
     }
 }
 
+// A value into a sum and its square into another, every operation rounded by itself: left to the compiler, the square would be fused into its sum or not as the
+// instructions at hand suit it, and the statistics' last bits (with them, units at their kink) would change from build to build.
+__device__ __forceinline__ void add_square(float& s1, float& s2, float v) {
+#pragma clang fp contract(off)
+    s1 += v;
+    s2 += v * v;
+}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);

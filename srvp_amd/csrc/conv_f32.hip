@@ -109,10 +109,7 @@ __global__ __launch_bounds__(256) void conv_f32_kernel(const ConvF a) {
         const long long m = m0 + wid * 32 + (r & 3) + 8 * (r >> 2) + 4 * lhalf;
         if (m >= M) continue;
         const float v = acc[r];
-        {
-#pragma clang fp contract(off)
-            s1 += v; s2 += v * v;         // (square and sum rounded apart, whatever instructions the compiler takes: the statistics stay those of every build)
-        }
+        add_square(s1, s2, v);
         const int n = (int)(m / hw), q = (int)(m - (long long)n * hw);
         const int oy = q / a.OW, ox = q - oy * a.OW;
         const int Y = oy * a.so + a.ooy, X = ox * a.so + a.oox;

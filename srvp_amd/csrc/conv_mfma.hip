@@ -145,7 +145,7 @@ __device__ __forceinline__ void conv_epilogue(f32x16_t (&acc)[TM][TN], const Con
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) { const float v = acc[i][j][r]; s1 += v; s2 += v * v; }
+                for (int r = 0; r < 16; ++r) { add_square(s1, s2, acc[i][j][r]); }
             s1 += __shfl_xor(s1, 32);
             s2 += __shfl_xor(s2, 32);
             if (lhalf == 0) {
@@ -171,7 +171,7 @@ __device__ __forceinline__ void conv_epilogue(f32x16_t (&acc)[TM][TN], const Con
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     float v = ok[i][r] ? acc[i][j][r] : 0.f;
-                    s1 += v; s2 += v * v;
+                    add_square(s1, s2, v);
                 }
             s1 += __shfl_xor(s1, 32);
             s2 += __shfl_xor(s2, 32);

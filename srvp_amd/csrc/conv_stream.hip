@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
                 for (int r = 0; r < SGROUP_ROWS; ++r)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) { const float v = acc[r][i]; s1 += v; s2 += v * v; }
+                    for (int i = 0; i < 16; ++i) { add_square(s1, s2, acc[r][i]); }
                 d1 += (double)s1; d2 += (double)s2;
             }
 #pragma unroll

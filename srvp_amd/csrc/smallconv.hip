@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BNR ? 2 : 4
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float v = acc[j][r];
-                s1[j] += v; s2[j] += v * v;
+                add_square(s1[j], s2[j], v);
                 Cs[(wid * 32 + (r & 3) + 8 * (r >> 2) + 4 * lhalf) * LDC + j * 32 + lcol] = f2bf(v);
             }
         }
