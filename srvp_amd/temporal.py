@@ -103,7 +103,8 @@ def rotary(q, k, positions, frequencies, *, interleaved=False, back=False, magni
 
 def rms_norm(x, weight, *, residual=None, eps=1e-6):
     """y = h * weight / sqrt(mean(h^2) + eps) over the last axis, h = x + residual.  x, residual (..., N), N <= 16384; weight (N,) float32.  Returns y, or
-    (y, h) with a residual (h rounded to x's type; y and the gradients are those of the unrounded sum).  Gradients: x, residual, weight."""
+    (y, h) with a residual (h rounded to x's type; y and the gradients are those of the unrounded sum).  Squares are summed in float32: rows above 1.8e19
+    come out as zero.  Gradients: x, residual, weight."""
     return (_ext or load()).rms_norm(x, weight, residual, eps)
 
 
