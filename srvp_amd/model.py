@@ -147,6 +147,8 @@ class StochasticLatentResidualVideoPredictor(nn.Module):
         super().__init__()
         if posterior not in ('lstm', 'attention'):
             raise ValueError(f"posterior 'lstm' or 'attention', got {posterior!r}")
+        if posterior == 'lstm' and posterior_heads is not None:
+            raise ValueError("posterior_heads: heads of the attention posterior (posterior='attention')")
         self.posterior = posterior
         assert nx == 64, 'the encoder / decoder families are 64x64 architectures (reference conv.py:45-48)'
         self.nx, self.nc, self.ny, self.nz, self.skipco = nx, nc, ny, nz, skipco

@@ -116,7 +116,7 @@ def test_posterior_option():
     assert [k for k in m.state_dict() if k.startswith('inf_z.')] == ['inf_z.inp.weight', 'inf_z.inp.bias', 'inf_z.norm.weight', 'inf_z.qkv.weight',
                                                                      'inf_z.out_norm.weight', 'inf_z.out.weight', 'inf_z.last_norm.weight']
     assert m.inf_z.heads == 3 and m.inf_z.width == 8 and 'inf_z.weight_hh_l0' in srvp_amd.StochasticLatentResidualVideoPredictor(*ctor).state_dict()
-    for bad in (dict(posterior='other'), dict(posterior='attention', posterior_heads=5), dict(posterior='attention', posterior_heads=0)):
+    for bad in (dict(posterior='other'), dict(posterior='attention', posterior_heads=5), dict(posterior='attention', posterior_heads=0), dict(posterior_heads=3)):
         with pytest.raises(ValueError):
             srvp_amd.StochasticLatentResidualVideoPredictor(*ctor, **bad)
     req = ['--save_path', 'x', '--ny', '2', '--nz', '2', '--nt_inf', '2', '--dataset', 'smmnist', '--data_dir', 'd', '--seq_len', '5', '--nc', '1', '--nt_cond', '2']
