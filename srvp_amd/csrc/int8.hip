@@ -199,13 +199,17 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void int8_dma_kernel(const Int8Arg
         }
 }
 
-// BM x BN outputs a workgroup of 2 x 2 waves, rows at any byte: 64 bytes of k pass through registers, the next ones under the products.  2305 x 1001 x 771:
-// 13 us, 16 steps of a latency each (two to four of them in flight: 14; the barriers' and the odd rows' latency, not the loads').
-template <class E, int BM, int BN>
-__global__ __launch_bounds__(256, 2) void int8_tile_kernel(const Int8Args g) {
+// BM x BN outputs a workgroup, rows at any byte: 64 bytes of k pass through registers, the next ones under the products (2305 x 1001 x 771: 13 us, 16 steps
+// of a latency each; two to four steps in flight: 14).  KG groups of 2 x 2 waves take the
+// steps of k in turn, each with its own stages, and their sums (whole numbers: any order) meet in LDS: where there are fewer tiles than the chip takes, the
+// steps one behind the other are the time, a latency each.
+template <class E, int BM, int BN, int KG>
+__global__ __launch_bounds__(256 * KG, KG > 2 ? 1 : 2) void int8_tile_kernel(const Int8Args g) {
     constexpr int BK = 64, LD = BK + 16, MT = BM / 32, NTL = BN / 32, LA = BM * 4 / 256, LW = BN * 4 / 256;
-    __shared__ __align__(16) signed char lx[BM * LD], lw[BN * LD];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, lg = lane >> 4, ls = lane & 15;
+    __shared__ __align__(16) signed char lds[KG][(BM + BN) * LD];
+    static_assert(KG / 2 * BM * BN * 4 <= KG * (BM + BN) * LD, "half the groups' sums fit the stages' memory");
+    const int tid = threadIdx.x & 255, lane = tid & 63, wv = tid >> 6, lg = lane >> 4, ls = lane & 15, kg = threadIdx.x >> 8;
+    signed char *lx = lds[kg], *lw = lx + BM * LD;
     unsigned im, in;
     tile_of(blockIdx.x, (g.M + BM - 1) / BM, (g.N + BN - 1) / BN, im, in);
     const int m0 = im * BM, n0 = in * BN, wm = (wv & 1) * (BM / 2), wn = (wv >> 1) * (BN / 2);
@@ -227,22 +231,22 @@ __global__ __launch_bounds__(256, 2) void int8_tile_kernel(const Int8Args g) {
             for (int i = 0; i < LA; ++i) __builtin_memcpy(&vx[i], px[i] + k0 + kc, 16);
 #pragma unroll
             for (int i = 0; i < LW; ++i) __builtin_memcpy(&vw[i], pw[i] + k0 + kc, 16);
-        } else {
+        } else {                                          // (a group's step may lie behind the end: zeros)
 #pragma unroll
             for (int i = 0; i < LA; ++i) vx[i] = bytes16(px[i], k0 + kc, g.K);
 #pragma unroll
             for (int i = 0; i < LW; ++i) vw[i] = bytes16(pw[i], k0 + kc, g.K);
         }
     };
-    fetch(0);
-    for (int k0 = 0; k0 < g.K; k0 += BK) {
+    fetch(kg * BK);
+    for (int k0 = 0; k0 < g.K; k0 += KG * BK) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < LA; ++i) *reinterpret_cast<u32x4_t*>(lx + ((i * 256 + tid) >> 2) * LD + kc) = vx[i];
 #pragma unroll
         for (int i = 0; i < LW; ++i) *reinterpret_cast<u32x4_t*>(lw + ((i * 256 + tid) >> 2) * LD + kc) = vw[i];
         __syncthreads();
-        if (k0 + BK < g.K) fetch(k0 + BK);
+        if (k0 + KG * BK < g.K) fetch(k0 + (KG + kg) * BK);
         i32x4_t fx[MT], fw[NTL];
 #pragma unroll
         for (int i = 0; i < MT; ++i) fx[i] = *reinterpret_cast<const i32x4_t*>(lx + (wm + i * 16 + ls) * LD + lg * 16);
@@ -253,6 +257,24 @@ __global__ __launch_bounds__(256, 2) void int8_tile_kernel(const Int8Args g) {
 #pragma unroll
             for (int j = 0; j < NTL; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fx[i], acc[i][j], 0, 0, 0);
     }
+    // the upper half of the groups hands its sums to the lower, until one is left
+    i32x4_t* sums = reinterpret_cast<i32x4_t*>(lds[0]);
+#pragma unroll
+    for (int half = KG / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (kg >= half && kg < 2 * half)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) sums[((kg - half) * MT * NTL + i * NTL + j) * 256 + tid] = acc[i][j];
+        __syncthreads();
+        if (kg < half)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) acc[i][j] += sums[(kg * MT * NTL + i * NTL + j) * 256 + tid];
+    }
+    if (kg > 0) return;
     float xs[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) xs[i] = g.xs[min(m0 + wm + i * 16 + ls, g.M - 1)];
@@ -338,8 +360,10 @@ hipError_t dma_launch(const Int8Args& g, hipStream_t st) {
     return hipSuccess;
 }
 // Which kernel (K = N = 4096, bfloat16 out, us; x the chosen side):
-//   rows    7: x 6, 64 x 64 tiles 48    rows   64: x 7, 64 x 64 tiles 15     (up to 64 rows)
-//   rows  512: x 25 (64 x 64 tiles), 28 (128 x 128 by DMA)     rows 1024: x 30 (128 x 128 by DMA), 41 (64 x 64)     (by DMA from 192 tiles of 128 x 128 on)
+//   rows    7: x 5, 64 x 64 tiles 13    rows   64: x 12, 64 x 64 tiles 14    (up to 64 rows)
+//   rows   65: x 14 (64 x 64 tiles, four groups of k), 15 (two), 20 (one); 94 x 6976 x 4544: x 26, 31, 50; 1024 x 1001 x 771: x 10, 10, 11; 192 x 256 x 256: 4.5, 4.0, x 4.0
+//              (four groups up to 256 tiles, from 16 steps of 64 on; two up to 512, from 32 steps on: rows 512: x 24, one group 26; 2304 x 256 x 768: 5.2, x 4.9)
+//   rows  512: x 24 (64 x 64 tiles), 28 (128 x 128 by DMA)     rows 1024: x 30 (128 x 128 by DMA), 41 (64 x 64)     (by DMA from 192 tiles of 128 x 128 on)
 //   rows 3000: x 66 (256 x 256 by DMA), 84 (128 x 128)         rows 2048: x 49 (128 x 128), 61 (256 x 256)          (256 x 256 from 192 such tiles on)
 // 8192 x 4096 x 4096: 143 us = 1.92 P operations/s, 8192 x 8192 x 8192: 2.01 P/s; the dense peak is 5, and the large bfloat16 product of the vendor's library
 // reaches 56 % of its own here (the package's power limit).
@@ -361,8 +385,15 @@ hipError_t launch(const Int8Args& g, bool aligned, hipStream_t st) {
     }
     if (aligned && t256 >= 192) return dma_launch<E, 256, 256, 2, 4, 4>(g, st);
     if (aligned && t128 >= 192) return dma_launch<E, 128, 128, 2, 2, 4>(g, st);
-    if (!aligned && t128 >= 512) hipLaunchKernelGGL((int8_tile_kernel<E, 128, 128>), dim3((unsigned)t128), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((int8_tile_kernel<E, 64, 64>), dim3((unsigned)(((g.M + 63) / 64) * ((g.N + 63) / 64))), dim3(256), 0, st, g);
+    if (!aligned && t128 >= 512) {
+        hipLaunchKernelGGL((int8_tile_kernel<E, 128, 128, 1>), dim3((unsigned)t128), dim3(256), 0, st, g);
+        return hipSuccess;
+    }
+    const unsigned t64 = (unsigned)(((g.M + 63) / 64) * ((g.N + 63) / 64));
+    const int steps = (g.K + 63) / 64, kg = steps >= 16 && t64 <= 256 ? 4 : steps >= 32 && t64 <= 512 ? 2 : 1;
+    if (kg == 4) hipLaunchKernelGGL((int8_tile_kernel<E, 64, 64, 4>), dim3(t64), dim3(1024), 0, st, g);
+    else if (kg == 2) hipLaunchKernelGGL((int8_tile_kernel<E, 64, 64, 2>), dim3(t64), dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((int8_tile_kernel<E, 64, 64, 1>), dim3(t64), dim3(256), 0, st, g);
     return hipSuccess;
 }
 

@@ -626,7 +626,8 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs g) {
 // ---- recurrent form: one token a row, states updated in place.  A workgroup owns one (row, head): the state passes through the registers once
 // (read + written: 8 Dk Dv bytes are the whole cost), columns across the lanes, rows of the state across the rest of the workgroup.
 // Rows that name the same slot are successive tokens of that sequence, in row order: the first of them does the others' work as well.
-// 512 rows x 16 heads of 128 x 128: 224 us = 4.9 TB/s; one row x 4 heads of 64 x 64: 4.6 us, the launch's.
+// 512 rows x 16 heads of 128 x 128: 224 us = 4.9 TB/s; one row x 4 heads of 64 x 64: 4.6 us, the launch's; 2 rows x 3 heads
+// of 202 x 122 15 (21 with an element a load where rows do not start at 16-byte borders).
 struct StepArgs {
     const void *q, *k, *v;
     void* o;
@@ -673,7 +674,6 @@ __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
     int nct = 1;
     while (nct < nc) nct <<= 1;
     const int rows = 256 / nct, c4 = tid % nct, r0 = tid / nct;
-    const bool vec = (g.Dv & 3) == 0;
     while (true) {
         const E* q = (const E*)g.q + b * g.qs[0] + h * g.qs[1];
         const E* k = (const E*)g.k + b * g.ks[0] + h * g.ks[1];
@@ -685,20 +685,21 @@ __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
         float vv[4], acc[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < 4; ++x) vv[x] = c + x < g.Dv ? get(v + c + x) : 0.f;
-        if (vec) {
-            if (c < g.Dv) {
+        if (c + 4 <= g.Dv) {                              // (rows of a state need not start at 16-byte borders)
 #pragma unroll 4
-                for (int i = r0; i < g.Dk; i += rows) {
-                    f32x4_t s = *reinterpret_cast<f32x4_t*>(st + (long long)i * g.Dv + c);
+            for (int i = r0; i < g.Dk; i += rows) {
+                float* p = st + (long long)i * g.Dv + c;
+                f32x4_t s;
+                __builtin_memcpy(&s, p, 16);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) { s[x] = a * s[x] + sk[i] * vv[x]; acc[x] += sq[i] * s[x]; }
-                    *reinterpret_cast<f32x4_t*>(st + (long long)i * g.Dv + c) = s;
-                }
+                for (int x = 0; x < 4; ++x) { s[x] = a * s[x] + sk[i] * vv[x]; acc[x] += sq[i] * s[x]; }
+                __builtin_memcpy(p, &s, 16);
             }
         } else {
+#pragma unroll 4
             for (int i = r0; i < g.Dk; i += rows)
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
+                for (int x = 0; x < 3; ++x)
                     if (c + x < g.Dv) {
                         float* p = st + (long long)i * g.Dv + c + x;
                         const float s = a * *p + sk[i] * vv[x];
