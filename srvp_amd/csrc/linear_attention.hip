@@ -685,27 +685,32 @@ __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
         float vv[4], acc[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < 4; ++x) vv[x] = c + x < g.Dv ? get(v + c + x) : 0.f;
-        if (c + 4 <= g.Dv) {                              // (rows of a state need not start at 16-byte borders)
-#pragma unroll 4
-            for (int i = r0; i < g.Dk; i += rows) {
-                float* p = st + (long long)i * g.Dv + c;
-                f32x4_t s;
-                __builtin_memcpy(&s, p, 16);
+        // U rows in flight (the compiler does not move a load in front of a store that it cannot tell apart)
+        constexpr int U = 8;
+        const bool four = c + 4 <= g.Dv;                  // (rows of a state need not start at 16-byte borders; the last columns may be fewer than four)
+        for (int i0 = r0; i0 < g.Dk; i0 += rows * U) {
+            f32x4_t s[U];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) { s[x] = a * s[x] + sk[i] * vv[x]; acc[x] += sq[i] * s[x]; }
-                __builtin_memcpy(p, &s, 16);
+            for (int u = 0; u < U; ++u) {
+                const float* p = st + (long long)min(i0 + u * rows, g.Dk - 1) * g.Dv;
+                if (four) __builtin_memcpy(&s[u], p + c, 16);
+                else s[u] = f32x4_t{p[min(c, g.Dv - 1)], p[min(c + 1, g.Dv - 1)], p[min(c + 2, g.Dv - 1)], 0.f};
             }
-        } else {
-#pragma unroll 4
-            for (int i = r0; i < g.Dk; i += rows)
 #pragma unroll
-                for (int x = 0; x < 3; ++x)
-                    if (c + x < g.Dv) {
-                        float* p = st + (long long)i * g.Dv + c + x;
-                        const float s = a * *p + sk[i] * vv[x];
-                        *p = s;
-                        acc[x] += sq[i] * s;
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * rows;
+                if (i < g.Dk) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) { s[u][x] = a * s[u][x] + sk[i] * vv[x]; acc[x] += sq[i] * s[u][x]; }
+                    float* p = st + (long long)i * g.Dv + c;
+                    if (four) __builtin_memcpy(p, &s[u], 16);
+                    else {
+#pragma unroll
+                        for (int x = 0; x < 3; ++x)
+                            if (c + x < g.Dv) p[x] = s[u][x];
                     }
+                }
+            }
         }
         // sum over the row groups, in a fixed order
 #pragma unroll
