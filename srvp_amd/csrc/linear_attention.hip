@@ -623,11 +623,12 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs g) {
     }
 }
 
-// ---- recurrent form: one token a row, states updated in place.  A workgroup owns one (row, head): the state passes through the registers once
-// (read + written: 8 Dk Dv bytes are the whole cost), columns across the lanes, rows of the state across the rest of the workgroup.
+// ---- recurrent form: one token a row, states updated in place.  A workgroup owns BLOCK columns of one (row, head): the state passes through the registers
+// once (read + written: 8 Dk Dv bytes are the whole cost), columns across the lanes, rows of the state across the rest of the workgroup, eight in flight.
 // Rows that name the same slot are successive tokens of that sequence, in row order: the first of them does the others' work as well.
-// 512 rows x 16 heads of 128 x 128: 224 us = 4.9 TB/s; one row x 4 heads of 64 x 64: 4.6 us, the launch's; 2 rows x 3 heads
-// of 202 x 122 15 (21 with an element a load where rows do not start at 16-byte borders).
+// 128 columns (us; 64, 256 columns): 512 rows x 16 heads of 128 x 128 209 = 5.1 TB/s (220, 208); 64 x 8 of 256 x 255 52 (59, 49); 1 x 2 of 256 x 256 8.0 (5.4, 12.7);
+// 2 x 3 of 202 x 122 11 (10, 11); 1 x 4 of 64 x 64 4, the launch's.  One width for all, so that a row's result does not depend on how many there are.
+constexpr int BLOCK = 128;                                 // columns of a workgroup
 struct StepArgs {
     const void *q, *k, *v;
     void* o;
@@ -644,7 +645,7 @@ template <> __device__ __forceinline__ float get<float>(const float* p) { return
 
 template <class E>
 __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
-    __shared__ float sq[256], sk[256], red[256][4];
+    __shared__ float sq[256], sk[256], red[4][BLOCK / 4][4];
     __shared__ int first, next;
     const int tid = threadIdx.x, h = blockIdx.x % g.H;
     int b = blockIdx.x / g.H;
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
         slot = g.slots[b];
         if (slot < 0 || slot >= g.nslots) {               // a padded row: no state, output zero
             E* o = (E*)g.o + b * g.os[0] + h * g.os[1];
-            for (int c = tid; c < g.Dv; c += 256) put(o + c, 0.f);
+            for (int c = blockIdx.y * BLOCK + tid; c < min(g.Dv, (int)(blockIdx.y + 1) * BLOCK); c += 256) put(o + c, 0.f);
             return;
         }
         if (tid == 0) { first = 1; next = g.B; }
@@ -670,10 +671,10 @@ __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
     }
     const float a = expf(g.log_decay[h]);
     float* st = g.state + (slot * g.H + h) * (long long)g.Dk * g.Dv;
-    const int nc = (g.Dv + 3) / 4;                        // columns in fours (at most 64 of them); 256 / nct rows of the state at a time
+    const int nc = min((g.Dv + 3) / 4, BLOCK / 4);        // columns in fours; 256 / nct rows of the state at a time
     int nct = 1;
     while (nct < nc) nct <<= 1;
-    const int rows = 256 / nct, c4 = tid % nct, r0 = tid / nct;
+    const int rows = 256 / nct, c4 = tid % nct, r0 = tid / nct, col0 = blockIdx.y * BLOCK;
     while (true) {
         const E* q = (const E*)g.q + b * g.qs[0] + h * g.qs[1];
         const E* k = (const E*)g.k + b * g.ks[0] + h * g.ks[1];
@@ -681,7 +682,7 @@ __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
         E* o = (E*)g.o + b * g.os[0] + h * g.os[1];
         for (int i = tid; i < g.Dk; i += 256) { sq[i] = g.scale * get(q + i); sk[i] = get(k + i); }
         __syncthreads();
-        const int c = c4 * 4;
+        const int c = col0 + c4 * 4;
         float vv[4], acc[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < 4; ++x) vv[x] = c + x < g.Dv ? get(v + c + x) : 0.f;
@@ -712,17 +713,18 @@ __global__ __launch_bounds__(256) void step_kernel(const StepArgs g) {
                 }
             }
         }
-        // sum over the row groups, in a fixed order
+        // sum over the row groups, in a fixed order: within the wave, then the four waves
+        for (int o = nct; o < 64; o <<= 1)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) red[tid][x] = acc[x];
+            for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor(acc[x], o);
+        if ((tid & 63) < nct)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) red[tid >> 6][c4][x] = acc[x];
         __syncthreads();
-        if (r0 == 0) {
-            for (int x = 0; x < 4; ++x) {
-                float s = 0.f;
-                for (int y = 0; y < rows; ++y) s += red[y * nct + c4][x];
-                if (c + x < g.Dv) put(o + c + x, s);
-            }
-        }
+        if (tid < nct)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (c + x < g.Dv) put(o + c + x, (red[0][c4][x] + red[1][c4][x]) + (red[2][c4][x] + red[3][c4][x]));
         __syncthreads();
         if (!g.slots) return;
         b = next;
@@ -942,8 +944,8 @@ extern "C" int srvp_linear_attention_step(const srvp_linear_attention_step_desc*
     for (int i = 0; i < 2; ++i) { g.qs[i] = d->qs[i]; g.ks[i] = d->ks[i]; g.vs[i] = d->vs[i]; g.os[i] = d->os[i]; }
     g.log_decay = d->log_decay; g.state = d->state; g.slots = (const long long*)d->slots;
     g.B = d->B; g.H = d->H; g.Dk = d->Dk; g.Dv = d->Dv; g.nslots = d->nslots; g.scale = d->scale;
-    if (d->elem_f32) hipLaunchKernelGGL(step_kernel<float>, dim3(d->B * d->H), dim3(256), 0, (hipStream_t)stream, g);
-    else hipLaunchKernelGGL(step_kernel<bf16_t>, dim3(d->B * d->H), dim3(256), 0, (hipStream_t)stream, g);
+    if (d->elem_f32) hipLaunchKernelGGL(step_kernel<float>, dim3(d->B * d->H, (d->Dv + BLOCK - 1) / BLOCK), dim3(256), 0, (hipStream_t)stream, g);
+    else hipLaunchKernelGGL(step_kernel<bf16_t>, dim3(d->B * d->H, (d->Dv + BLOCK - 1) / BLOCK), dim3(256), 0, (hipStream_t)stream, g);
     SRVP_CHECK_LAUNCH("srvp_linear_attention_step");
     return SRVP_OK;
 }
