@@ -206,7 +206,9 @@ __device__ __forceinline__ void put4(float* p, const f32x4_t& v) { *reinterpret_
 // token c0 + i, or c0 + mm - 1 - i in reversed time: everything behind the loader sees time running forwards.
 // VEC: 16 bytes at a time, by buffer loads whose bound is the chunk's last row: what lies behind it and behind the operand's features comes as zero, with no
 // condition (a load under a branch makes the compiler wait for every load in flight where the paths meet, three memory latencies a chunk) and one address
-// register.  Otherwise the elements go straight to LDS in `store`.
+// register.  Otherwise (rows at other borders than 16 bytes, features not in eights) 16 bytes from any address: rows behind the last are the last again, the
+// last vector of a row ends with the row, and both are put right on the way into LDS.  Fewer features than a vector: one by one, in `store`.
+// 512 x 32, 16 heads of 127 x 127, forward / backward: 94 / 264 us (element by element 333 / 1160); of 128 x 128 through the same code's VEC form 59 / 153.
 constexpr unsigned OUTSIDE = 0x80000000u;      // an offset behind every bound: a chunk is at most 2^30 bytes (see operand())
 template <class E, int W, bool VEC> struct Tile {
     using V = View<E, W>;
@@ -217,8 +219,16 @@ template <class E, int W, bool VEC> struct Tile {
         const int c = col0 + tid % (W / VE) * VE;
         return c < d ? c * (unsigned)sizeof(E) : OUTSIDE;
     }
-    __device__ __forceinline__ void load(const char* chunk, unsigned step, unsigned col, int mm, int rev, int tid) {
-        if constexpr (VEC) {
+    __device__ __forceinline__ void load(const char* chunk, unsigned step, unsigned col, int mm, int rev, int tid, const Operand& s, int col0) {
+        if constexpr (!VEC) {
+            if (s.d < VE) return;
+            const int row = tid / (W / VE), at = min(col0 + tid % (W / VE) * VE, s.d - VE);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int r = min(row + i * ROWS, mm - 1);
+                __builtin_memcpy(&v[i], reinterpret_cast<const E*>(chunk) + (long long)(rev ? mm - 1 - r : r) * s.st + at, 16);
+            }
+        } else {
             const int row = tid / (W / VE);
             const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)chunk, 0, mm * step, 0x00027000);
             const unsigned next = rev ? 0u - ROWS * step : ROWS * step;
@@ -234,6 +244,19 @@ template <class E, int W, bool VEC> struct Tile {
             for (int i = 0; i < NV; ++i) {
                 if constexpr (ROWS % 16 == 0) V::put16(lds + i * V::elems(ROWS), row, col, v[i]);      // (the exchange of chunks repeats every 16 rows)
                 else V::put16(lds, row + i * ROWS, col, v[i]);
+            }
+        } else if (s.d >= VE) {
+            const int row = tid / (W / VE), col = (tid % (W / VE)) * VE;
+            const int behind = (col0 + col - min(col0 + col, s.d - VE)) * (int)sizeof(E) * 8;      // bits of the vector in front of its column
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                unsigned long long lo = v[i].x | (unsigned long long)v[i].y << 32, hi = v[i].z | (unsigned long long)v[i].w << 32;
+                if (behind >= 64) { lo = hi; hi = 0; }
+                const int bits = behind & 63;
+                lo = lo >> bits | (hi << 1 << (63 - bits));
+                hi >>= bits;
+                const bool in = row + i * ROWS < mm && behind < 128;
+                V::put16(lds, row + i * ROWS, col, in ? u32x4_t{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)} : u32x4_t{0, 0, 0, 0});
             }
         } else {
 #pragma unroll 1
@@ -303,9 +326,11 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kern
     const unsigned colb = Tile<E, DA, VEC>::column(da, 0, tid), colc = Tile<E, CB, VEC>::column(dc, col0, tid);
     auto fetch = [&](int cc) {
         const int c0 = t0 + (rev ? nch - 1 - cc : cc) * C, mm = min(C, t1 - c0);
-        if (OUT) ra.load((const char*)pa + (unsigned long long)c0 * stepa, stepa, colb, mm, rev, tid);
-        rb.load((const char*)pb + (unsigned long long)c0 * stepb, stepb, colb, mm, rev, tid);
-        rc.load((const char*)pc + (unsigned long long)c0 * stepc, stepc, colc, mm, rev, tid);
+        // (steps in 32 bits are those of the bounded loads)
+        const auto from = [&](const E* p, const Operand& s, unsigned step) { return (const char*)p + (VEC ? (long long)c0 * step : (long long)c0 * s.st * (long long)sizeof(E)); };
+        if (OUT) ra.load(from(pa, r.a, stepa), stepa, colb, mm, rev, tid, r.a, 0);
+        rb.load(from(pb, r.b, stepb), stepb, colb, mm, rev, tid, r.b, 0);
+        rc.load(from(pc, r.c, stepc), stepc, colc, mm, rev, tid, r.c, col0);
     };
 
     if (tid <= 2 * C) {
@@ -481,13 +506,26 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kern
                             at[ct] += next;
                         }
                     } else {
+                        // (a lane's columns are neighbours over all its tiles for bfloat16)
+                        constexpr int RUN = sizeof(E) == 2 ? NCT * 4 : 4;
                         const int i = ti * 16 + ls;
+                        unsigned e[NCT * sizeof(E)];      // (the lane's columns as they lie in memory)
 #pragma unroll
-                        for (int ct = 0; ct < NCT; ++ct) {
-                            const int c = col0 + Y::template col_of<NCT>(w, ct, lg * 4);
+                        for (int x = 0; x < NCT; ++x) {
+                            if constexpr (sizeof(E) == 2) { e[2 * x] = pack2bf(acc[x][0], acc[x][1]); e[2 * x + 1] = pack2bf(acc[x][2], acc[x][3]); }
+                            else __builtin_memcpy(e + 4 * x, &acc[x], 16);
+                        }
 #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                if (i < mm && c + x < dc) put(po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot + c + x, acc[ct][x]);
+                        for (int x = 0; x < NCT * 4; x += RUN) {
+                            const int c = col0 + Y::template col_of<NCT>(w, x / 4, lg * 4);
+                            E* q = po + (long long)(c0 + (rev ? mm - 1 - i : i)) * r.ot + c;
+                            if (i < mm && c + RUN <= dc) {
+                                __builtin_memcpy(q, (const char*)e + x * sizeof(E), RUN * sizeof(E));
+                            } else if (i < mm) {
+#pragma unroll
+                                for (int y = 0; y < RUN; ++y)
+                                    if (c + y < dc) put(q + y, acc[(x + y) / 4][(x + y) % 4]);
+                            }
                         }
                     }
                 }

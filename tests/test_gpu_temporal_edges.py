@@ -237,3 +237,36 @@ def test_refusals():
     with pytest.raises(torch.OutOfMemoryError):
         la(far, far, far, ld[:1])
     assert la(x, x, x, ld).shape == x.shape
+
+
+def inside(g, T, B, H, D, dt, off, pad):
+    """Rows of D features that begin `off` elements into rows of D + pad; what lies around them is NaN."""
+    wide = torch.full((T, B, H, D + pad), float('nan'), dtype=dt, device=DEV)
+    wide[..., off:off + D] = rnd(g, T, B, H, D, dtype=dt)
+    return wide[..., off:off + D]
+
+
+@pytest.mark.parametrize('T,Dk,Dv,off,pad,lengths', [
+    (1, 8, 9, 1, 2, None), (33, 7, 9, 3, 3, [33, 0]), (70, 9, 15, 1, 1, [70, 1]), (129, 83, 32, 1, 8, None), (150, 63, 60, 2, 5, [65, 150]),
+    (200, 127, 129, 7, 7, None), (66, 64, 128, 1, 8, [66, 64]), (300, 249, 250, 5, 6, [299, 2]), (900, 65, 11, 0, 3, None), (90, 4, 5, 1, 2, None),
+])
+@pytest.mark.parametrize('dt', [BF, FP])
+def test_linear_attention_of_rows_at_odd_places(T, Dk, Dv, off, pad, lengths, dt):
+    """Feature counts and addresses that no wide access divides, inside rows whose other elements are NaN."""
+    from srvp_amd import temporal as t
+    B, H = 2, 3
+    g = torch.Generator().manual_seed(T + Dk)
+    q, k, v, do = (inside(g, T, B, H, D, dt, off, pad) for D in (Dk, Dk, Dv, Dv))
+    ld, sc = decays(H), Dk ** -0.5
+    n = None if lengths is None else torch.tensor(lengths, device=DEV)
+    for b, m in enumerate(lengths or []):
+        for x in (q, k, v, do):
+            x[m:, b] = float('nan')
+    inn = inner_of(dt, T, max(Dk, Dv))
+    qc, kc, vc, gc = (torch.nan_to_num(x) for x in (q, k, v, do))
+    o = t.linear_attention(q, k, v, ld, lengths=n)
+    within(o, *scan(qc, kc, vc, ld, sc, False, lengths=lengths), dt, inn, 'o')
+    dq, dk, dv = t.linear_attention_backward(do, q, k, v, ld, lengths=n)[:3]
+    within(dq, *scan(gc, vc, kc, ld, sc, False, lengths=lengths), dt, inn, 'dq')
+    within(dk, *scan(vc, gc, qc, ld, sc, True, lengths=lengths), dt, inn, 'dk')
+    within(dv, *scan(kc, qc, gc, ld, sc, True, lengths=lengths), dt, inn, 'dv')
