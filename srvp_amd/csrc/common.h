@@ -30,6 +30,15 @@ __device__ __forceinline__ uint32_t pack2bf(float lo, float hi) {
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+// v moved down by `bits` (any number from 0 on), zeros from above: a vector that was read `bits` in front of its place
+__device__ __forceinline__ u32x4_t without_low(const u32x4_t& v, int bits) {
+    unsigned long long lo = v.x | (unsigned long long)v.y << 32, hi = v.z | (unsigned long long)v.w << 32;
+    if (bits >= 64) { lo = bits < 128 ? hi : 0; hi = 0; }
+    bits &= 63;
+    lo = lo >> bits | (hi << 1 << (63 - bits));
+    hi >>= bits;
+    return u32x4_t{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+}
 __device__ __forceinline__ void unpack8(const u32x4_t& v, float* f) {
     f[0] = bf_lo(v.x); f[1] = bf_hi(v.x); f[2] = bf_lo(v.y); f[3] = bf_hi(v.y);
     f[4] = bf_lo(v.z); f[5] = bf_hi(v.z); f[6] = bf_lo(v.w); f[7] = bf_hi(v.w);

@@ -250,13 +250,7 @@ template <class E, int W, bool VEC> struct Tile {
             const int behind = (col0 + col - min(col0 + col, s.d - VE)) * (int)sizeof(E) * 8;      // bits of the vector in front of its column
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                unsigned long long lo = v[i].x | (unsigned long long)v[i].y << 32, hi = v[i].z | (unsigned long long)v[i].w << 32;
-                if (behind >= 64) { lo = hi; hi = 0; }
-                const int bits = behind & 63;
-                lo = lo >> bits | (hi << 1 << (63 - bits));
-                hi >>= bits;
-                const bool in = row + i * ROWS < mm && behind < 128;
-                V::put16(lds, row + i * ROWS, col, in ? u32x4_t{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)} : u32x4_t{0, 0, 0, 0});
+                V::put16(lds, row + i * ROWS, col, row + i * ROWS < mm ? without_low(v[i], behind) : u32x4_t{0, 0, 0, 0});
             }
         } else {
 #pragma unroll 1

@@ -130,7 +130,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
 // and q = 0, i.e. stands for NaN.
 // TPR threads hold one row in registers: V vectors of VE elements each.
 // Measured (us): 16384 x 4096 bfloat16 with a residual forward 92 = 5.8 TB/s, backward 141 + 5 for dw = 4.8 TB/s; 2304 x 256 float32 4.0, 5.7 + 3.5 (launches);
-// 8-bit output 7 x 4096 6, 2305 x 1001 float32 11 (rows at odd bytes: an element a load).
+// 8-bit output 7 x 4096 5.  Rows that are not whole vectors at borders of 16 bytes take the same vectors from any address (one element a load, a value's
+// neighbours in the next threads: 16384 x 4095 forward 177, backward 436, 8-bit 246 us, now 125, 172, 134; 16384 x 4096 100, 130, 91).
 struct NormArgs {
     const void *x, *res;
     const float* w;
@@ -139,32 +140,40 @@ struct NormArgs {
     float* scale;
     long long xs, rs, ys, ss, qs;      // row strides
     long long M;
-    int N, vec;
+    int N;
     float eps;
 };
 
-// Value i of thread t of a row: column (i / VE * TPR + t) * VE + i % VE where rows are read 16 bytes at a time, i * TPR + t otherwise.
-template <int VE, int TPR> __device__ __forceinline__ int column(int i, int t, int vec) { return vec ? (i / VE * TPR + t) * VE + i % VE : i * TPR + t; }
+// Value i of thread t of a row is column (i / VE * TPR + t) * VE + i % VE.
+template <int VE, int TPR> __device__ __forceinline__ int column(int i, int t) { return (i / VE * TPR + t) * VE + i % VE; }
 
-// a row as it lies in memory: the next row's loads are in flight while this one is reduced and written
-template <class E, int VE, int V, int TPR> struct Raw {
+// A row as it lies in memory: the next row's loads are in flight while this one is reduced and written.  VEC: all vectors are whole, at borders of 16 bytes.
+// Otherwise they are read from any address and the last one ends with the row, to be put right when it has `arrived`.
+template <class E, int VE, int V, int TPR, bool VEC> struct Raw {
     u32x4_t v[V];
-    __device__ __forceinline__ void load(const E* p, int N, int vec, int t) {
+    __device__ __forceinline__ void load(const E* p, int N, int t) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            v[i] = u32x4_t{0, 0, 0, 0};
-            if (vec) {
-                const int c = (i * TPR + t) * VE;
+            const int c = (i * TPR + t) * VE;
+            if (VEC || N < VE) v[i] = u32x4_t{0, 0, 0, 0};
+            if constexpr (VEC) {
                 if (c < N) v[i] = *reinterpret_cast<const u32x4_t*>(p + c);
-            } else {
+            } else if (N >= VE) {
+                __builtin_memcpy(&v[i], p + min(c, N - VE), 16);
+            } else if (c == 0) {
                 E e[VE];
 #pragma unroll
-                for (int j = 0; j < VE; ++j) {
-                    const int c = (i * VE + j) * TPR + t;
-                    e[j] = c < N ? p[c] : E(0);
-                }
+                for (int j = 0; j < VE; ++j) e[j] = j < N ? p[j] : E(0);
                 __builtin_memcpy(&v[i], e, 16);
             }
+        }
+    }
+    __device__ __forceinline__ void arrived(int N, int t) {
+        if (VEC || N < VE) return;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (i * TPR + t) * VE;
+            v[i] = without_low(v[i], max(0, c - (N - VE)) * (int)sizeof(E) * 8);
         }
     }
     __device__ __forceinline__ float get(int i) const {      // (unrolled loops only: i is a constant)
@@ -173,31 +182,36 @@ template <class E, int VE, int V, int TPR> struct Raw {
         return El<E>::ld(e + i % VE);
     }
 };
-template <int VE, int V, int TPR> __device__ __forceinline__ void load_weight(const float* w, int N, int vec, int t, float* f) {
+template <int VE, int V, int TPR> __device__ __forceinline__ void load_weight(const float* w, int N, int t, float* f) {
 #pragma unroll
-    for (int i = 0; i < V * VE; ++i) {
-        const int c = column<VE, TPR>(i, t, vec);
-        f[i] = c < N ? w[c] : 0.f;
+    for (int i = 0; i < V * VE; i += 4) {
+        const int c = column<VE, TPR>(i, t);
+        if (c + 4 <= N) {
+            __builtin_memcpy(f + i, w + c, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[i + j] = c + j < N ? w[c + j] : 0.f;
+        }
     }
 }
-template <class E, int VE, int V, int TPR>
-__device__ __forceinline__ void row_store(E* p, int N, int vec, int t, const float* f) {
+template <class E, int VE, int V, int TPR, bool VEC>
+__device__ __forceinline__ void row_store(E* p, int N, int t, const float* f) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         E e[VE];
 #pragma unroll
         for (int j = 0; j < VE; ++j) El<E>::st(e + j, f[v * VE + j]);
-        if (vec) {
-            const int c = (v * TPR + t) * VE;
+        const int c = (v * TPR + t) * VE;
+        if constexpr (VEC) {
             u32x4_t x;
             __builtin_memcpy(&x, e, 16);
             if (c < N) *reinterpret_cast<u32x4_t*>(p + c) = x;
+        } else if (c + VE <= N) {
+            __builtin_memcpy(p + c, e, 16);
         } else {
 #pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                const int c = (v * VE + j) * TPR + t;
-                if (c < N) p[c] = e[j];
-            }
+            for (int j = 0; j < VE; ++j)
+                if (c + j < N) p[c + j] = e[j];
         }
     }
 }
@@ -242,23 +256,25 @@ template <int TPR> __device__ __forceinline__ double row_max(double v, double* r
     return v;
 }
 
-template <class E, int V, int TPR, bool Q8, bool NORM>
+template <class E, int V, int TPR, bool Q8, bool NORM, bool VEC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const NormArgs g) {
     constexpr int VE = 16 / sizeof(E), NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
     __shared__ double redd[NT / 64];
     float* red = reinterpret_cast<float*>(redd);
     const int tid = threadIdx.x, t = tid % TPR;
     float wv[V * VE];
-    if (NORM) load_weight<VE, V, TPR>(g.w, g.N, g.vec, t, wv);
-    Raw<E, VE, V, TPR> x, r;
+    if (NORM) load_weight<VE, V, TPR>(g.w, g.N, t, wv);
+    Raw<E, VE, V, TPR, VEC> x, r;
     const long long step = (long long)gridDim.x * RPW;
     long long row = (long long)blockIdx.x * RPW + tid / TPR;
     auto fetch = [&](long long at) {
-        x.load((const E*)g.x + at * g.xs, g.N, g.vec, t);
-        if (g.res) r.load((const E*)g.res + at * g.rs, g.N, g.vec, t);
+        x.load((const E*)g.x + at * g.xs, g.N, t);
+        if (g.res) r.load((const E*)g.res + at * g.rs, g.N, t);
     };
     if (row < g.M) fetch(row);
     for (; row < g.M; row += step) {                       // (the same for all threads of a row, and of a workgroup whose waves meet)
+        x.arrived(g.N, t);
+        if (g.res) r.arrived(g.N, t);
         float h[V * VE];
         double hd[Q8 ? V * VE : 1];
 #pragma unroll
@@ -268,7 +284,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
             if (Q8) hd[i] = (double)u + (double)v;
         }
         if (row + step < g.M) fetch(row + step);
-        if (g.sum) row_store<E, VE, V, TPR>((E*)g.sum + row * g.ss, g.N, g.vec, t, h);
+        if (g.sum) row_store<E, VE, V, TPR, VEC>((E*)g.sum + row * g.ss, g.N, t, h);
         if constexpr (!Q8) {
             float ss = 0.f;
 #pragma unroll
@@ -276,7 +292,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
             const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)g.N + g.eps);
 #pragma unroll
             for (int i = 0; i < V * VE; ++i) h[i] *= rstd * wv[i];
-            row_store<E, VE, V, TPR>((E*)g.y + row * g.ys, g.N, g.vec, t, h);
+            row_store<E, VE, V, TPR, VEC>((E*)g.y + row * g.ys, g.N, t, h);
         } else {
             double most = 0, ss = 0;                       // (the squares in 64 bits too: a row of 1e20s is not an infinite one)
 #pragma unroll
@@ -296,15 +312,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
                 signed char e[VE];
 #pragma unroll
                 for (int j = 0; j < VE; ++j) e[j] = fine ? (signed char)(int)rint(hd[v * VE + j] * to) : 0;
-                if (g.vec) {
-                    const int c = (v * TPR + t) * VE;
-                    if (c < g.N) __builtin_memcpy(q + c, e, VE);
+                const int c = (v * TPR + t) * VE;
+                if (c + VE <= g.N) {
+                    __builtin_memcpy(q + c, e, VE);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < VE; ++j) {
-                        const int c = (v * VE + j) * TPR + t;
-                        if (c < g.N) q[c] = e[j];
-                    }
+                    for (int j = 0; j < VE; ++j)
+                        if (c + j < g.N) q[c + j] = e[j];
                 }
             }
         }
@@ -318,30 +332,34 @@ struct NormBwdArgs {
     float* part;                      // [workgroup][N] sums of dy * n over the workgroup's rows
     long long xs, rs, dys, dss, dxs;
     long long M;
-    int N, vec;
+    int N;
     float eps;
 };
-template <class E, int V, int TPR>
+template <class E, int V, int TPR, bool VEC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(const NormBwdArgs g) {
     constexpr int VE = 16 / sizeof(E), NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
     __shared__ float red[NT / 32];
     __shared__ float cols[RPW > 1 ? NT * V * VE : 1];
     const int tid = threadIdx.x, t = tid % TPR;
     float wv[V * VE], dw[V * VE];
-    load_weight<VE, V, TPR>(g.w, g.N, g.vec, t, wv);
+    load_weight<VE, V, TPR>(g.w, g.N, t, wv);
 #pragma unroll
     for (int i = 0; i < V * VE; ++i) dw[i] = 0.f;
-    Raw<E, VE, V, TPR> x, r, dy, ds;
+    Raw<E, VE, V, TPR, VEC> x, r, dy, ds;
     const long long step = (long long)gridDim.x * RPW;
     long long row = (long long)blockIdx.x * RPW + tid / TPR;
     auto fetch = [&](long long at) {
-        x.load((const E*)g.x + at * g.xs, g.N, g.vec, t);
-        if (g.res) r.load((const E*)g.res + at * g.rs, g.N, g.vec, t);
-        dy.load((const E*)g.dy + at * g.dys, g.N, g.vec, t);
-        if (g.dsum) ds.load((const E*)g.dsum + at * g.dss, g.N, g.vec, t);
+        x.load((const E*)g.x + at * g.xs, g.N, t);
+        if (g.res) r.load((const E*)g.res + at * g.rs, g.N, t);
+        dy.load((const E*)g.dy + at * g.dys, g.N, t);
+        if (g.dsum) ds.load((const E*)g.dsum + at * g.dss, g.N, t);
     };
     if (row < g.M) fetch(row);
     for (; row < g.M; row += step) {
+        x.arrived(g.N, t);
+        if (g.res) r.arrived(g.N, t);
+        dy.arrived(g.N, t);
+        if (g.dsum) ds.arrived(g.N, t);
         float n[V * VE], d[V * VE], f[V * VE];
         float ss = 0.f, dot = 0.f;
 #pragma unroll
@@ -362,12 +380,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(const N
             dw[i] += d[i] * n[i];
             d[i] = rstd * (d[i] * wv[i] - n[i] * dot) + f[i];
         }
-        row_store<E, VE, V, TPR>((E*)g.dx + row * g.dxs, g.N, g.vec, t, d);
+        row_store<E, VE, V, TPR, VEC>((E*)g.dx + row * g.dxs, g.N, t, d);
     }
     float* part = g.part + (long long)blockIdx.x * g.N;
     if constexpr (RPW > 1) {
 #pragma unroll
-        for (int i = 0; i < V * VE; ++i) cols[(tid / TPR) * V * TPR * VE + column<VE, TPR>(i, t, g.vec)] = dw[i];
+        for (int i = 0; i < V * VE; ++i) cols[(tid / TPR) * V * TPR * VE + column<VE, TPR>(i, t)] = dw[i];
         __syncthreads();
         for (int c = tid; c < g.N; c += NT) {
             float s = 0.f;
@@ -377,9 +395,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(const N
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < V * VE; ++i) {
-            const int c = column<VE, TPR>(i, t, g.vec);
-            if (c < g.N) part[c] = dw[i];
+        for (int i = 0; i < V * VE; i += 4) {
+            const int c = column<VE, TPR>(i, t);
+            if (c + 4 <= g.N) {
+                __builtin_memcpy(part + c, dw + i, 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < g.N) part[c + j] = dw[i + j];
+            }
         }
     }
 }
@@ -422,29 +446,33 @@ bool al(const void* p, long long stride, int bytes, int e) { return (uintptr_t)p
         else if constexpr (VE == 4) GO(4, 1024);   \
     } while (0)
 
-template <class E, bool Q8, bool NORM>
-void fwd_launch(const NormArgs& g, hipStream_t st) {
+template <class E, bool Q8, bool NORM, bool VEC>
+void fwd_go(const NormArgs& g, hipStream_t st) {
     constexpr int VE = 16 / sizeof(E);
     const int N = g.N;
     const long long rows = N <= 128 * VE ? (g.M + 3) / 4 : g.M;
     const dim3 grid((unsigned)(rows < 1024 ? rows : 1024));
-#define GO(V, T) hipLaunchKernelGGL((norm_fwd_kernel<E, V, T, Q8, NORM>), grid, dim3(T > 256 ? T : 256), 0, st, g)
+#define GO(V, T) hipLaunchKernelGGL((norm_fwd_kernel<E, V, T, Q8, NORM, VEC>), grid, dim3(T > 256 ? T : 256), 0, st, g)
     NORM_ROWS(GO);
 #undef GO
 }
+template <class E, bool Q8, bool NORM>
+void fwd_launch(const NormArgs& g, bool vec, hipStream_t st) { vec ? fwd_go<E, Q8, NORM, true>(g, st) : fwd_go<E, Q8, NORM, false>(g, st); }
 int bwd_groups(long long M, int N, int VE) {
     const long long rows = N <= 128 * VE ? (M + 3) / 4 : M;
     const int most = N <= 128 * VE ? 256 : 512;
     return (int)(rows < most ? rows : most);
 }
-template <class E>
-void bwd_launch(const NormBwdArgs& g, hipStream_t st) {
+template <class E, bool VEC>
+void bwd_go(const NormBwdArgs& g, hipStream_t st) {
     constexpr int VE = 16 / sizeof(E);
     const int N = g.N, n = bwd_groups(g.M, N, VE);
-#define GO(V, T) hipLaunchKernelGGL((norm_bwd_kernel<E, V, T>), dim3(n), dim3(T > 256 ? T : 256), 0, st, g)
+#define GO(V, T) hipLaunchKernelGGL((norm_bwd_kernel<E, V, T, VEC>), dim3(n), dim3(T > 256 ? T : 256), 0, st, g)
     NORM_ROWS(GO);
 #undef GO
 }
+template <class E>
+void bwd_launch(const NormBwdArgs& g, bool vec, hipStream_t st) { vec ? bwd_go<E, true>(g, st) : bwd_go<E, false>(g, st); }
 constexpr int NORM_MAX = 16384;
 
 }  // namespace
@@ -506,14 +534,14 @@ extern "C" int srvp_rms_norm(const srvp_rms_norm_desc* d, void* stream) {
     g.x = d->x; g.res = d->residual; g.w = d->w; g.y = d->y; g.sum = d->sum; g.q = (signed char*)d->q8; g.scale = d->scale;
     g.xs = d->xs; g.rs = d->rs; g.ys = d->ys; g.ss = d->ss; g.qs = d->qs; g.M = d->M; g.N = d->N; g.eps = d->eps;
     const int e = d->elem_f32 ? 4 : 2, ve = 16 / e;
-    g.vec = d->N % ve == 0 && al(d->x, d->xs, 16, e) && (!d->residual || al(d->residual, d->rs, 16, e)) && (!d->sum || al(d->sum, d->ss, 16, e))
+    const bool vec = d->N % ve == 0 && al(d->x, d->xs, 16, e) && (!d->residual || al(d->residual, d->rs, 16, e)) && (!d->sum || al(d->sum, d->ss, 16, e))
             && (d->q8 ? al(d->q8, d->qs, ve, 1) : al(d->y, d->ys, 16, e));
     hipStream_t st = (hipStream_t)stream;
     if (d->q8) {
-        if (d->elem_f32) { if (d->w) fwd_launch<float, true, true>(g, st); else fwd_launch<float, true, false>(g, st); }
-        else { if (d->w) fwd_launch<bf16_t, true, true>(g, st); else fwd_launch<bf16_t, true, false>(g, st); }
+        if (d->elem_f32) { if (d->w) fwd_launch<float, true, true>(g, vec, st); else fwd_launch<float, true, false>(g, vec, st); }
+        else { if (d->w) fwd_launch<bf16_t, true, true>(g, vec, st); else fwd_launch<bf16_t, true, false>(g, vec, st); }
     } else {
-        if (d->elem_f32) fwd_launch<float, false, true>(g, st); else fwd_launch<bf16_t, false, true>(g, st);
+        if (d->elem_f32) fwd_launch<float, false, true>(g, vec, st); else fwd_launch<bf16_t, false, true>(g, vec, st);
     }
     SRVP_CHECK_LAUNCH("srvp_rms_norm");
     return SRVP_OK;
@@ -532,9 +560,9 @@ extern "C" int srvp_rms_norm_bwd(const srvp_rms_norm_bwd_desc* d, void* stream) 
     g.x = d->x; g.res = d->residual; g.dy = d->d_y; g.dsum = d->d_sum; g.w = d->w; g.dx = d->dx; g.part = (float*)d->ws;
     g.xs = d->xs; g.rs = d->rs; g.dys = d->dys; g.dss = d->dss; g.dxs = d->dxs; g.M = d->M; g.N = d->N; g.eps = d->eps;
     const int e = d->elem_f32 ? 4 : 2, ve = 16 / e;
-    g.vec = d->N % ve == 0 && al(d->x, d->xs, 16, e) && (!d->residual || al(d->residual, d->rs, 16, e)) && al(d->d_y, d->dys, 16, e) && (!d->d_sum || al(d->d_sum, d->dss, 16, e)) && al(d->dx, d->dxs, 16, e);
+    const bool vec = d->N % ve == 0 && al(d->x, d->xs, 16, e) && (!d->residual || al(d->residual, d->rs, 16, e)) && al(d->d_y, d->dys, 16, e) && (!d->d_sum || al(d->d_sum, d->dss, 16, e)) && al(d->dx, d->dxs, 16, e);
     hipStream_t st = (hipStream_t)stream;
-    if (d->elem_f32) bwd_launch<float>(g, st); else bwd_launch<bf16_t>(g, st);
+    if (d->elem_f32) bwd_launch<float>(g, vec, st); else bwd_launch<bf16_t>(g, vec, st);
     SRVP_CHECK_LAUNCH("srvp_rms_norm_bwd");
     hipLaunchKernelGGL(norm_dw_kernel, dim3((d->N + 15) / 16), dim3(1024), 0, st, (const float*)d->ws, bwd_groups(d->M, d->N, ve), d->N, d->dw);
     SRVP_CHECK_LAUNCH("srvp_rms_norm_bwd(weight)");

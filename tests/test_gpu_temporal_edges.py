@@ -1,6 +1,7 @@
 """
 Temporal operators at their edges: values that are not finite, offsets past 32 bits, rows of the largest values, calls from two threads, refusals.
 """
+import math
 import threading
 
 import pytest
@@ -270,3 +271,34 @@ def test_linear_attention_of_rows_at_odd_places(T, Dk, Dv, off, pad, lengths, dt
     within(dq, *scan(gc, vc, kc, ld, sc, False, lengths=lengths), dt, inn, 'dq')
     within(dk, *scan(vc, gc, qc, ld, sc, True, lengths=lengths), dt, inn, 'dk')
     within(dv, *scan(kc, qc, gc, ld, sc, True, lengths=lengths), dt, inn, 'dv')
+
+
+@pytest.mark.parametrize('N,off,pad', [(1, 1, 2), (3, 1, 1), (4, 1, 2), (5, 3, 4), (7, 1, 3), (8, 1, 1), (9, 7, 8), (77, 2, 2), (513, 1, 5), (1001, 3, 3), (1024, 1, 8), (2050, 5, 6),
+                                       (4095, 1, 2), (4096, 3, 8), (8191, 1, 1), (10001, 5, 7), (16384, 1, 1)])
+@pytest.mark.parametrize('dt', [BF, FP])
+def test_rms_norm_of_rows_at_odd_places(N, off, pad, dt):
+    """Rows that begin at any element, inside rows whose other elements are NaN; rows of whole vectors give what the same rows give at wide borders."""
+    from srvp_amd import temporal as t
+    M = 11
+    g = torch.Generator().manual_seed(N)
+    x, r, dy, ds = (inside(g, M, 1, 1, N, dt, off, pad)[:, 0, 0] for _ in range(4))
+    w = inside(g, 1, 1, 1, N, FP, off, pad)[0, 0, 0]
+    u, h, wd = 2.0 ** -24, x.double() + r.double(), w.double()
+    rs = 1 / torch.sqrt((h * h).mean(1, keepdim=True) + 1e-6)
+    y, total = t.rms_norm(x, w, residual=r)
+    within(y, h * rs * wd, (h * rs * wd).abs(), dt, (math.log2(N) + 24) * u, 'y')
+    within(total, h, h.abs(), dt, u, 'sum')
+    dx, dw = t.rms_norm_backward(dy, x, w, residual=r, d_sum=ds)[:2]
+    n, dn = h * rs, dy.double() * wd
+    size = rs * (dn.abs() + n.abs() * (dn * n).abs().mean(1, keepdim=True)) + ds.double().abs()
+    within(dx, rs * (dn - n * (dn * n).mean(1, keepdim=True)) + ds.double(), size, dt, (N / 256 + 40) * u, 'dx')
+    within(dw, (dy.double() * n).sum(0), (dy.double() * n).abs().sum(0), FP, (M / 512 + 60) * u, 'dw')
+    q, s, again = t.rms_norm_int8(x, w, residual=r)
+    rq, rscale = rows8(h, wd, 1e-6)
+    assert torch.equal(q.double(), rq) and torch.equal(again, total)
+    within(s, rscale, rscale, FP, (math.log2(N) + 24) * u, 'scale')
+    if N % (16 // x.element_size()) == 0:
+        xa, ra, dya, dsa, wa = (a.contiguous().clone() for a in (x, r, dy, ds, w))
+        assert torch.equal(t.rms_norm(xa, wa, residual=ra)[0], y)
+        for a, b in zip(t.rms_norm_backward(dya, xa, wa, residual=ra, d_sum=dsa), (dx, dw)):
+            assert torch.equal(a, b)
