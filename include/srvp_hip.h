@@ -599,7 +599,7 @@ int srvp_stream_is_capturing(void* stream, int* capturing);
 int srvp_linear_attention_step(const srvp_linear_attention_step_desc* d, void* stream);
 /* Rotary positions of q (T, B, Hq, D) and k (T, B, Hk, D; Hk = 0: none): pair p of every head -- features (2p, 2p + 1) if interleaved, (p, pairs + p)
  * otherwise -- is turned by positions[t][b] * freq[p] radians (back = 1: by the negative angle) and multiplied by `magnitude`; features from 2 * pairs on
- * are copied.  positions int64 with strides pos_t, pos_b; freq float64 [pairs]. */
+ * are copied.  positions int64 with strides pos_t, pos_b; freq float64 [pairs].  Outputs do not overlap inputs. */
 typedef struct {
     const void *q, *k; void *oq, *ok;
     int64_t qs[3], ks[3], oqs[3], oks[3];

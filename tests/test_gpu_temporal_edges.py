@@ -7,7 +7,7 @@ import threading
 import pytest
 import torch
 
-from test_gpu_temporal import BF, DEV, FP, decays, inner_of, rnd, rows8, scan, within
+from test_gpu_temporal import BF, DEV, FP, decays, inner_of, rnd, rows8, scan, turned, within
 
 pytestmark = pytest.mark.gpu
 
@@ -302,3 +302,23 @@ def test_rms_norm_of_rows_at_odd_places(N, off, pad, dt):
         assert torch.equal(t.rms_norm(xa, wa, residual=ra)[0], y)
         for a, b in zip(t.rms_norm_backward(dya, xa, wa, residual=ra, d_sum=dsa), (dx, dw)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('D,rot', [(1, 0), (2, 2), (5, 4), (7, 6), (8, 8), (9, 8), (16, 0), (17, 16), (21, 18), (33, 16), (63, 62), (65, 32), (84, 84), (126, 126), (127, 126), (127, 34),
+                                   (128, 128), (250, 200), (515, 514)])
+@pytest.mark.parametrize('inter', [False, True])
+@pytest.mark.parametrize('dt', [BF, FP])
+def test_rotary_of_heads_at_odd_places(D, rot, inter, dt):
+    """Heads that begin at any element and turn any number of pairs, inside rows whose other elements are NaN; the rest of a head is copied as it is."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(D + rot)
+    T, B = 19, 3
+    q, k = inside(g, T, B, 5, D, dt, 1, 2), inside(g, T, B, 2, D, dt, 3, 4)
+    pos = torch.randint(0, 10 ** 6, (T, B), generator=g).to(DEV)
+    w = t.rotary_frequencies(rot, device=DEV)
+    back = D % 2 == 1
+    for x, o in zip((q, k), t.rotary(q, k, pos, w, interleaved=inter, back=back)):
+        ref, size = turned(x, pos, w, inter, 1.0, back)
+        within(o, ref, size, dt, 12 * 2.0 ** -24, 'rotary')
+        assert torch.equal(o[..., rot:], x[..., rot:])
+        assert torch.equal(o, t.rotary(x.contiguous(), None, pos, w, interleaved=inter, back=back))
