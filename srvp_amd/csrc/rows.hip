@@ -501,7 +501,6 @@ extern "C" int srvp_rotary(const srvp_rotary_desc* d, void* stream) {
     const long long rows = (long long)d->T * d->B;
     if (rows == 0 || d->Hq + d->Hk == 0) return SRVP_OK;
     SRVP_REQUIRE((d->Hq == 0 || (d->q && d->oq)) && (d->Hk == 0 || (d->k && d->ok)) && d->positions && (d->freq || d->pairs == 0), "srvp_rotary: null pointer");
-    SRVP_REQUIRE((d->Hq == 0 || d->q != d->oq) && (d->Hk == 0 || d->k != d->ok), "srvp_rotary: an output in the place of its input");
     RotArgs g;
     memset(&g, 0, sizeof(g));
     const int e = d->elem_f32 ? 4 : 2, ve = 16 / e;
@@ -526,6 +525,7 @@ extern "C" int srvp_rotary(const srvp_rotary_desc* d, void* stream) {
     const int items = vec ? (half + ve - 1) / ve + (rest + ve - 1) / ve : d->pairs + rest;
     const long long grid = (rows + R - 1) / R;
     SRVP_REQUIRE(rows < (1LL << 31) && grid < (1 << 24) && R * H * items < (1LL << 30), "srvp_rotary: too many rows or heads");
+    SRVP_REQUIRE((d->Hq == 0 || d->q != d->oq) && (d->Hk == 0 || d->k != d->ok), "srvp_rotary: an output in the place of its input");
     g.dB = divide(d->B); g.dn = divide(n); g.dH = divide(H); g.ditems = divide(items);
     hipStream_t st = (hipStream_t)stream;
 #define ROTARY(E, VE, MODE) hipLaunchKernelGGL((rotary_kernel<E, VE, MODE>), dim3((unsigned)grid), dim3(256), 0, st, g)

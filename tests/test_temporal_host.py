@@ -126,3 +126,10 @@ def test_posterior_option():
     assert o['posterior'] == 'attention' and o['posterior_heads'] == 4
     with pytest.raises(SystemExit):
         p.parse_args(req + ['--posterior', 'other'])
+
+
+def test_rotary_in_place_is_refused():
+    """Threads share features at the end of a head: an output over its input would turn them twice."""
+    one = dict(q=16, oq=32, positions=16, freq=16, T=1, B=1, Hq=1, D=8, pairs=4, magnitude=1.0)
+    for same in (dict(oq=16), dict(k=64, ok=64, Hk=1)):
+        assert L.load().srvp_rotary(C.byref(L.RotaryDesc(**dict(one, **same))), None) == 1 and b'in the place' in L.load().srvp_last_error()
