@@ -14,15 +14,27 @@ struct Int8Args {
     int M, N, K, vecy, vecy16;      // 4 outputs / 16 bytes of them may be stored together
 };
 
-// 16 bytes of row `p` from byte k on, zero behind K (rows may start at any byte)
+// 16 bytes of row `p` from byte k on, zero behind K (rows may start at any byte; K >= 16: the row's last 16 bytes, moved, are one load)
 __device__ __forceinline__ u32x4_t bytes16(const signed char* p, int k, int K) {
     u32x4_t v = {0, 0, 0, 0};
-    if (k + 16 <= K) __builtin_memcpy(&v, p + k, 16);
-    else if (k < K) {
+    if (K >= 16) {
+        const int at = min(k, K - 16);
+        __builtin_memcpy(&v, p + at, 16);
+        v = without_low(v, (k - at) * 8);
+    } else if (k < K) {
         signed char e[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) e[i] = k + i < K ? p[k + i] : 0;
         __builtin_memcpy(&v, e, 16);
+    }
+    return v;
+}
+// the first n bytes of v zero
+__device__ __forceinline__ u32x4_t without_first(u32x4_t v, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int m = n - 4 * i;
+        v[i] = m >= 4 ? 0 : m > 0 ? v[i] >> 8 * m << 8 * m : v[i];
     }
     return v;
 }
@@ -291,7 +303,9 @@ __global__ __launch_bounds__(256 * KG, KG > 2 ? 1 : 2) void int8_tile_kernel(con
 }
 
 // Few rows (M <= 16 MT): the weight's bytes are the cost (7 x 4096 x 4096: 5.3 us = 3.2 TB/s, the launch included).  A workgroup owns 16 rows of w and all rows of x; its 8 waves deal the steps of 64 bytes of k among
-// them, w straight from memory into the fragments, UNROLL steps in flight; the partial sums (whole numbers: any order) meet in LDS.
+// them, w straight from memory into the fragments, UNROLL steps in flight; the partial sums (whole numbers: any order) meet in LDS.  Other rows than whole vectors
+// at borders of 16 bytes: behind the last whole ones the last 16 bytes of a row are read, of both operands, and the bytes already taken are zero in w.  Rows at
+// borders of 4 bytes cost little (7 x 4092 x 4096: 6.0), at odd bytes the memory system splits the loads (7 x 4095: 13.3, 64 x 4095 x 4095 37).
 template <class E, int MT, bool ALIGNED>
 __global__ __launch_bounds__(512) void int8_rows_kernel(const Int8Args g) {
     constexpr int UNROLL = MT == 1 ? 8 : 4;
@@ -320,6 +334,12 @@ __global__ __launch_bounds__(512) void int8_rows_kernel(const Int8Args g) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i) fx[u][i] = *reinterpret_cast<const u32x4_t*>(x[i] + at);
                 if (!in) fw[u] = u32x4_t{0, 0, 0, 0};
+            } else if (g.K >= 16) {
+                const int at = min(k, g.K - 16);
+                __builtin_memcpy(&fw[u], w + at, 16);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) __builtin_memcpy(&fx[u][i], x[i] + at, 16);
+                fw[u] = without_first(fw[u], k - at);
             } else {
                 fw[u] = bytes16(w, k, g.K);
 #pragma unroll
