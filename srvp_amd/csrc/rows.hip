@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
 // quotient are formed in 64 bits, so q does not depend on the order of any sum.  A row of zeros has scale 0; a row with an infinity or NaN has scale NaN
 // and q = 0, i.e. stands for NaN.
 // TPR threads hold one row in registers: V vectors of VE elements each.
-// Measured (us): 16384 x 4096 bfloat16 with a residual forward 92 = 5.8 TB/s, backward 141 + 5 for dw = 4.8 TB/s; 2304 x 256 float32 4.0, 5.7 + 3.5 (launches);
+// Measured (us): 16384 x 4096 bfloat16 with a residual forward 89 = 6.0 TB/s, backward 141 + 5 for dw = 4.8 TB/s; 2304 x 256 float32 3.8, 5.5 + 3.6 (launches);
 // 8-bit output 7 x 4096 5.  Rows that are not whole vectors at borders of 16 bytes take the same vectors from any address (one element a load, a value's
 // neighbours in the next threads: 16384 x 4095 forward 177, backward 436, 8-bit 246 us, now 125, 172, 134; 16384 x 4096 100, 130, 91).
 struct NormArgs {
