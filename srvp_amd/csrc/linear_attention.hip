@@ -95,6 +95,16 @@ template <> struct Ty<bf16_t> {
         v.z = pack2bf(t[1][0], t[1][1]); v.w = pack2bf(t[1][2], t[1][3]);
         return __builtin_bit_cast(frag, v);
     }
+    // 8 values as the sum of two bf16 terms (to 2^-17 of each)
+    static __device__ __forceinline__ void terms(const f32x4_t* t, frag* out) {
+        out[0] = pack(t);
+        float h[8];
+        unpack8(__builtin_bit_cast(u32x4_t, out[0]), h);
+        f32x4_t rest[2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rest[i >> 2][i & 3] = t[i >> 2][i & 3] - h[i];
+        out[1] = pack(rest);
+    }
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, const f32x4_t& c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
     }
@@ -171,7 +181,7 @@ template <> struct Ty<float> {
         for (int i = 0; i < 4; ++i) x[i] = x[i] - x[i] == 0.f ? x[i] : 0.f;
         return x;
     }
-    static __device__ __forceinline__ frag pack(const f32x4_t* t) { return t[0]; }
+    static __device__ __forceinline__ void terms(const f32x4_t* t, frag* out) { out[0] = t[0]; }
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, f32x4_t c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
@@ -267,24 +277,27 @@ template <class E, int W, bool VEC> struct Tile {
 // A chunk: the three tiles go to LDS (the next chunk's loads are in flight meanwhile); the lower-triangular 16 x 16 tiles of the scores are dealt to the
 // waves and exchanged through LDS; then every wave forms its columns of the output and of the state.
 //
-// Bound: HBM, where two workgroups share a CU.  A chunk of bfloat16, 128 features, moves 64 KB: 7400 cycles at the CU's part of 5.3 TB/s; it costs 164 matrix
-// instructions (2600 cycles), 650 others (2600) and 2700 cycles of LDS, in turn within a wave, under each other between the waves.  Measured (16 heads of 128,
-// bfloat16): 512 x 32 forward 61 us = 4.4 TB/s, backward (three roles, each reads three operands) 155; 2048 x 16 (one workgroup a CU: the latency of a chunk's
-// steps, 10 700 cycles) 147 and 330.  fp32 (12 x 192, 4 heads of 64, one chunk a workgroup) 8 and 17 us; 1024 x 16 206 and 526: fp32 products at a sixteenth of the rate.
+// Bound: HBM and the matrix cores, where two workgroups share a CU.  A chunk of bfloat16, 128 features, moves 64 KB: 7400 cycles at the CU's part of 5.3 TB/s; it
+// costs 196 matrix instructions (3100 cycles a wave, two waves a matrix core), 800 others and 2700 cycles of LDS, in turn within a wave, under each other between
+// the waves.  Measured (16 heads of 128, bfloat16): 512 x 32 forward 67 us = 4.0 TB/s, backward (three roles, each reads three operands) 168; 2048 x 16 (one
+// workgroup a CU: the latency of a chunk's steps) 161 and 359.  With the state rounded once these were 61, 153, 147 and 330: the second term is a sixth of the matrix
+// instructions.  fp32 (12 x 192, 4 heads of 64, one chunk a workgroup) 8 and 17 us; 1024 x 16 210 and 521: fp32 products at a sixteenth of the rate.
 // Four waves of 32 columns: eight of 16 read every tile of a and b twice as often; one chunk of 64 tokens: 32 halve the products between barriers.  The limit
-// is the registers: 255 of 256 (the state 64, the loads in flight 48), whatever is added is spilt.
+// is the registers: 243 of 256 (the state 64, the loads in flight 48, sums of past tokens 32).  64 features of a and 32 columns a wave would spill at three
+// workgroups a CU: 512 x 32, 16 heads of 64 -> 128: 52 us against 47.
 //
 // The products run over whole tiles, tokens behind the row's own weighted with zero, which a NaN or infinity in c would pass through: it enters them as zero,
 // and its column of the output (from its row on) and of the state are made NaN behind them.
 template <class E, int DA, int NCT, bool OUT, bool VEC, int SPLIT>
-__global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kernel(const ScanArgs g) {
+__global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 || (sizeof(E) == 2 && OUT && NCT == 2) ? 2 : 3) void scan_kernel(const ScanArgs g) {
     using Y = Ty<E>;
     typedef typename Y::frag frag;
     constexpr int C = Y::C, KS = Y::KS, TPK = Y::TPK, CB = 64 * NCT, ND = DA / KS, NJ = C / KS, NTA = DA / 16, NTI = C / 16;
     using VA = View<E, DA>;
     using VC = View<E, CB>;
     using VP = View<E, C>;
-    constexpr int PT = sizeof(E) == 2 ? 2 : 1;              // bf16: a score is the sum of two terms, as the products that formed it are fp32
+    constexpr int TG = sizeof(E) == 2 ? NTI : 1;            // tiles of 16 tokens whose product with the state is formed at a time
+    constexpr int PT = sizeof(E) == 2 ? 2 : 1;              // bf16: scores, and the state that multiplies a, are sums of two terms, as the products that formed them are fp32
     __shared__ __align__(16) E lb[VA::elems(C)], lc[VC::elems(C)], la[OUT ? VA::elems(C) : 1], lp[OUT ? PT * VP::elems(C) : 1];      // lp: scores [term][i][j]
     __shared__ float power[2][2 * C + 4];                    // a^n and scale a^n, n = -C .. C: zero in front of n = 0
     const float *pw = power[0] + C, *spw = power[1] + C;
@@ -431,11 +444,30 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kern
             for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = VC::at_column(lc, j * KS, vcol[ct]);
 
         if (OUT) {
-            frag sf[ND][NCT];                             // bf16: the state is rounded once for the product with a (it is kept in fp32)
+            // a S, for TG tiles of 16 tokens at a time, a step of the features after the other.  bf16: the state as two terms, as the scores (rounded once it
+            // alone would add two thirds of the output's own rounding, 0.0022 of the output against 0.0017, and be the larger part of short sums that cancel).
+            f32x4_t old[TG][NCT];
+            auto past_products = [&](int t0) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+                for (int t = 0; t < TG; ++t)
 #pragma unroll
-                for (int ct = 0; ct < NCT; ++ct) sf[d][ct] = Y::pack(S[ct] + d * TPK);
+                    for (int ct = 0; ct < NCT; ++ct) old[t][ct] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    frag sf[NCT][PT];
+#pragma unroll
+                    for (int ct = 0; ct < NCT; ++ct) Y::terms(S[ct] + d * TPK, sf[ct]);
+#pragma unroll
+                    for (int t = 0; t < TG; ++t) {
+                        const frag af = va.rows(la, (t0 + t) * 16, d);
+#pragma unroll
+                        for (int x = 0; x < PT; ++x)
+#pragma unroll
+                            for (int ct = 0; ct < NCT; ++ct) old[t][ct] = Y::mfma(sf[ct][x], af, old[t][ct]);
+                    }
+                }
+            };
+            past_products(0);
             __syncthreads();                              // the scores are complete
             unsigned x = 0;
 #pragma unroll
@@ -450,7 +482,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kern
                     for (int ct = 0; ct < NCT; ++ct) vf[j][ct] = Y::tame(vf[j][ct]);
             }
             // output^T tiles: rows = columns of c (4 lg + ..), column = token ti * 16 + ls
-            frag af[ND], pf[PT][NJ];
+            frag pf[PT][NJ];
             // stores by offsets whose bound is the chunk's last row, as the loads
             const unsigned step = (unsigned)r.ot * sizeof(E), next = rev ? 0u - 16 * step : 16 * step;
             const auto out = __builtin_amdgcn_make_buffer_rsrc(po + (long long)c0 * r.ot, 0, mm * step, 0x00027000);
@@ -465,19 +497,15 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kern
                 // bf16: all four tiles of 16 tokens in one run of code (with a branch a tile the waits of one tile do not overlap the next's products)
                 if (VEC && sizeof(E) == 2 || ti * 16 < mm) {
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) af[d] = va.rows(la, ti * 16, d);
-#pragma unroll
                     for (int j = 0; j < NJ; ++j)
                         if (j * KS <= ti * 16 + 15)
 #pragma unroll
                             for (int x = 0; x < PT; ++x) pf[x][j] = vp.rows(lp + x * VP::elems(C), ti * 16, j);
-                    f32x4_t acc[NCT], old[NCT];
+                    if (ti > 0 && ti % TG == 0) past_products(ti);
+                    f32x4_t* acc = old[ti % TG];
+                    const float past = spw[ti * 16 + ls + e];
 #pragma unroll
-                    for (int ct = 0; ct < NCT; ++ct) acc[ct] = old[ct] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int ct = 0; ct < NCT; ++ct) old[ct] = Y::mfma(sf[d][ct], af[d], old[ct]);
+                    for (int ct = 0; ct < NCT; ++ct) acc[ct] *= past;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
                         if (j * KS <= ti * 16 + 15)
@@ -485,9 +513,6 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 ? 2 : 3) void scan_kern
                             for (int x = 0; x < PT; ++x)
 #pragma unroll
                                 for (int ct = 0; ct < NCT; ++ct) acc[ct] = Y::mfma(vf[j][ct], pf[x][j], acc[ct]);
-                    const float past = spw[ti * 16 + ls + e];
-#pragma unroll
-                    for (int ct = 0; ct < NCT; ++ct) acc[ct] += old[ct] * past;
                     if constexpr (VEC && sizeof(E) == 2 && NCT == 2) {
                         const u32x4_t v = {pack2bf(acc[0][0], acc[0][1]), pack2bf(acc[0][2], acc[0][3]), pack2bf(acc[1][0], acc[1][1]), pack2bf(acc[1][2], acc[1][3])};
                         __builtin_amdgcn_raw_buffer_store_b128(v, out, at[0], 0, 0);
