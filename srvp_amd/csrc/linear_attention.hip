@@ -108,9 +108,9 @@ template <> struct Ty<bf16_t> {
     static __device__ __forceinline__ f32x4_t mfma(const frag& x, const frag& y, const f32x4_t& c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
     }
-    // x * w as a sum of SPLIT bf16 values of 8 significant bits each.  Three are the fp32 product to its last bit, so the state (a result of its own) has fp32's
-    // accuracy.  Two (2^-17) serve the gradients' sums, which only pass into bfloat16 values (16 % of the backward pass); the forward pass takes three always,
-    // or its output would depend on whether the state was asked for.
+    // x * w as a sum of SPLIT bf16 values of 8 significant bits each.  Three are the fp32 product to its last bit, so the state and its gradient (results of their
+    // own) have fp32's accuracy.  Two (2^-17) serve the other gradients' sums, which only pass into bfloat16 values (10 % of the backward pass).  Neither depends on
+    // what else the caller asks for: the forward pass takes three with the new state wanted or not, the state's gradient has a pass of its own.
     template <int SPLIT> static __device__ __forceinline__ void weigh(const frag& x, const float* w, frag* out) {
         float f[8];
         unpack8(__builtin_bit_cast(u32x4_t, x), f);
@@ -273,7 +273,8 @@ template <class E, int W, bool VEC> struct Tile {
 };
 
 // One workgroup (4 waves) walks one segment of one (sequence, head) in scan order; wave w owns 16 * NCT columns of c, hence of the state (registers,
-// fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel).
+// fp32) and of the output.  OUT = false: only the segment's own sum  sum_j a^(..) b_j c_j^T  is formed (segments are joined by join_kernel), or, of a sequence in
+// one piece, the carry behind it (fin).
 // A chunk: the three tiles go to LDS (the next chunk's loads are in flight meanwhile); the lower-triangular 16 x 16 tiles of the scores are dealt to the
 // waves and exchanged through LDS; then every wave forms its columns of the output and of the state.
 //
@@ -373,7 +374,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 || (sizeof(E) == 2 && O
     {
         const float* src = nullptr;
         float mul = 1.f;
-        if (OUT) {
+        if (OUT || r.fin) {
             if (r.prefix) src = r.prefix + (bh * g.nseg + seg) * (long long)da * dc;
             else if (r.init) { src = r.init + bh * (long long)da * dc; mul = r.init_mul; }
         }
@@ -615,7 +616,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 || (sizeof(E) == 2 && O
 
     float* dst = nullptr;
     float mul = 1.f;
-    if (!OUT) {
+    if (!OUT && !r.fin) {
         dst = g.part + (((long long)ro * g.B * g.H + bh) * g.nseg + seg) * (long long)da * dc;
     } else if (r.fin) {
         const int last = rev ? 0 : n > 0 ? (n - 1) / g.seg_len : 0;
@@ -641,12 +642,12 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 || (sizeof(E) == 2 && O
     }
 }
 
-// Segment sums -> the carry in front of every segment, in place.  One thread owns one element of the state and walks the segments in scan order.
-// 512 states of 128 x 128 (67 MB in and out): 12.5 us = 5.4 TB/s.
+// Segment sums -> the carry in front of every segment, in place, and (fin) behind the last.  One thread owns one element
+// of the state and walks the segments in scan order.  512 states of 128 x 128 (67 MB in and out): 12.5 us = 5.4 TB/s.
 struct JoinArgs {
-    float* part;
+    float *part, *fin;
     const float* init[2];
-    float init_mul[2];
+    float init_mul[2], fin_mul;
     int rev[2];
     const float* log_decay;
     const long long* lengths;
@@ -678,6 +679,7 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs g) {
             }
         }
     }
+    if (g.fin) g.fin[(long long)bh * g.n + el] = g.fin_mul * carry;
 }
 
 // ---- recurrent form: one token a row, states updated in place.  A workgroup owns BLOCK columns of one (row, head): the state passes through the registers
@@ -892,11 +894,11 @@ extern "C" int64_t srvp_linear_attention_ws_bytes(const srvp_linear_attention_de
     return nseg <= 1 ? 0 : (int64_t)(backward ? 2 : 1) * d->B * d->H * nseg * d->Dk * d->Dv * 4;
 }
 
-static int run_join(const ScanArgs& base, const srvp_linear_attention_desc* d, int sets, const float* const* init, const float* mul, float* part, hipStream_t st) {
+static int run_join(const ScanArgs& base, const srvp_linear_attention_desc* d, int sets, const float* const* init, const float* mul, const int* rev, float* part, float* fin, float fin_mul, hipStream_t st) {
     JoinArgs j;
     memset(&j, 0, sizeof(j));
-    j.part = part; j.log_decay = d->log_decay; j.lengths = base.lengths;
-    for (int i = 0; i < sets; ++i) { j.init[i] = init[i]; j.init_mul[i] = mul[i]; j.rev[i] = i; }
+    j.part = part; j.fin = fin; j.fin_mul = fin_mul; j.log_decay = d->log_decay; j.lengths = base.lengths;
+    for (int i = 0; i < sets; ++i) { j.init[i] = init[i]; j.init_mul[i] = mul[i]; j.rev[i] = rev[i]; }
     j.T = d->T; j.B = d->B; j.H = d->H; j.nseg = base.nseg; j.seg_len = base.seg_len; j.n = d->Dk * d->Dv;
     // (grid.y: a sequence is cut where there are fewer than 256 pairs)
     hipLaunchKernelGGL(join_kernel, dim3((j.n + 255) / 256, d->B * d->H, sets), dim3(256), 0, st, j);
@@ -930,11 +932,14 @@ extern "C" int srvp_linear_attention_fwd(const srvp_linear_attention_desc* d, vo
     r.init_a = d->Dv; r.init_c = 1;
     if (g.nseg > 1) {
         float* part = (float*)d->ws;
-        if (d->elem_f32) launch<float>(g, &r, 1, false, true, part, st); else launch<bf16_t>(g, &r, 1, false, true, part, st);
+        Role sums = r;
+        sums.fin = nullptr;
+        if (d->elem_f32) launch<float>(g, &sums, 1, false, true, part, st); else launch<bf16_t>(g, &sums, 1, false, true, part, st);
         SRVP_CHECK_LAUNCH("srvp_linear_attention_fwd(segments)");
         const float* init[1] = {d->state_in};
         const float mul[1] = {1.f};
-        if (int rc = run_join(g, d, 1, init, mul, part, st)) return rc;
+        const int rev[1] = {0};
+        if (int rc = run_join(g, d, 1, init, mul, rev, part, nullptr, 0.f, st)) return rc;
         r.prefix = part;
     }
     if (d->elem_f32) launch<float>(g, &r, 1, true, true, nullptr, st); else launch<bf16_t>(g, &r, 1, true, true, nullptr, st);
@@ -954,13 +959,13 @@ extern "C" int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* b
     const int64_t need = srvp_linear_attention_ws_bytes(d, 1);
     SRVP_REQUIRE(need == 0 || (d->ws && d->ws_bytes >= need), "srvp_linear_attention_bwd: workspace of %lld bytes needed", (long long)need);
     const int f32 = d->elem_f32, Dk = d->Dk, Dv = d->Dv;
-    const bool exact = bd->d_state_in != nullptr;          // (the carry leaves as an fp32 gradient)
     const Operand q = operand(d->q, d->qs, Dk, f32), k = operand(d->k, d->ks, Dk, f32), v = operand(d->v, d->vs, Dv, f32), go = operand(bd->d_o, bd->d_os, Dv, f32);
     Role r[3];
     memset(r, 0, sizeof(r));
     // dv: (k, q, do), reversed, carry X (Dk x Dv)
     r[0].a = k; r[0].b = q; r[0].c = go; output(r[0], bd->dv, bd->dvs, Dv, f32);
-    r[0].rev = 1; r[0].init = bd->d_state_out; r[0].init_mul = 1.f / d->scale; r[0].fin = bd->d_state_in; r[0].fin_mul = d->scale;
+    r[0].rev = 1; r[0].init = bd->d_state_out; r[0].init_mul = 1.f / d->scale;
+    if (f32) { r[0].fin = bd->d_state_in; r[0].fin_mul = d->scale; }
     r[0].init_a = Dv; r[0].init_c = 1;
     // dk: (v, do, q), reversed, carry X^T
     r[1].a = v; r[1].b = go; r[1].c = q; output(r[1], bd->dk, bd->dks, Dk, f32);
@@ -968,22 +973,34 @@ extern "C" int srvp_linear_attention_bwd(const srvp_linear_attention_bwd_desc* b
     // dq: (do, v, k), forwards, carry S^T
     r[2].a = go; r[2].b = v; r[2].c = k; output(r[2], bd->dq, bd->dqs, Dk, f32);
     r[2].init = d->state_in; r[2].init_mul = 1.f; r[2].init_a = 1; r[2].init_c = Dv;
+    Role p[2];                                            // segment sums of S (k, v) and of X (q, do)
+    memset(p, 0, sizeof(p));
+    p[0].a = k; p[0].b = k; p[0].c = v; p[0].init_a = Dv; p[0].init_c = 1;
+    p[1].a = q; p[1].b = q; p[1].c = go; p[1].init_a = Dv; p[1].init_c = 1; p[1].rev = 1;
+    const float* init[2] = {d->state_in, bd->d_state_out};
+    const float mul[2] = {1.f, 1.f / d->scale};
+    const int rev[2] = {0, 1};
+    if (bd->d_state_in && !f32) {
+        // dS_0 of bfloat16 tensors: X once more, in fp32's accuracy.  (One of the roles with three terms instead of two takes the others' time too where all are in
+        // flight at once, also for callers without a state: 8192 x 2, 16 heads of 128: 288 -> 322 us.  With this pass only those with one pay: 512 x 32, 16 heads of
+        // 128 -> 64: 138, with a state 167; three terms for all roles 156.)
+        Role x = p[1];
+        if (g.nseg == 1) { x.init = init[1]; x.init_mul = mul[1]; x.fin = bd->d_state_in; x.fin_mul = d->scale; }
+        launch<bf16_t>(g, &x, 1, false, true, (float*)d->ws, st);
+        SRVP_CHECK_LAUNCH("srvp_linear_attention_bwd(state)");
+        if (g.nseg > 1)
+            if (int rc = run_join(g, d, 1, init + 1, mul + 1, rev + 1, (float*)d->ws, bd->d_state_in, d->scale, st)) return rc;
+    }
     if (g.nseg > 1) {
         float* part = (float*)d->ws;
         const long long set = (long long)d->B * d->H * g.nseg * Dk * Dv;
-        Role p[2];                                        // segment sums of S (k, v) and of X (q, do)
-        memset(p, 0, sizeof(p));
-        p[0].a = k; p[0].b = k; p[0].c = v; p[0].init_a = Dv; p[0].init_c = 1;
-        p[1].a = q; p[1].b = q; p[1].c = go; p[1].init_a = Dv; p[1].init_c = 1; p[1].rev = 1;
-        if (f32) launch<float>(g, p, 2, false, exact, part, st); else launch<bf16_t>(g, p, 2, false, exact, part, st);
+        if (f32) launch<float>(g, p, 2, false, false, part, st); else launch<bf16_t>(g, p, 2, false, false, part, st);
         SRVP_CHECK_LAUNCH("srvp_linear_attention_bwd(segments)");
-        const float* init[2] = {d->state_in, bd->d_state_out};
-        const float mul[2] = {1.f, 1.f / d->scale};
-        if (int rc = run_join(g, d, 2, init, mul, part, st)) return rc;
+        if (int rc = run_join(g, d, 2, init, mul, rev, part, nullptr, 0.f, st)) return rc;
         r[0].prefix = r[1].prefix = part + set;
         r[2].prefix = part;
     }
-    if (f32) launch<float>(g, r, 3, true, exact, nullptr, st); else launch<bf16_t>(g, r, 3, true, exact, nullptr, st);
+    if (f32) launch<float>(g, r, 3, true, false, nullptr, st); else launch<bf16_t>(g, r, 3, true, false, nullptr, st);
     SRVP_CHECK_LAUNCH("srvp_linear_attention_bwd");
     return SRVP_OK;
 }
