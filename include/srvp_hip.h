@@ -609,7 +609,7 @@ typedef struct {
 int srvp_rotary(const srvp_rotary_desc* d, void* stream);
 /* h = x + residual (NULL: h = x); y = h * w / sqrt(mean(h^2) + eps) over rows of N features; sum (may be NULL) = h.
  * q8 != NULL: instead of y, int8 rows and float32 scale [M] with y ~ q8 * scale: scale = max|y| / 127, q8 = round-half-even(h w * (127 / max|h w|)) in 64 bits;
- * w == NULL then quantises h itself.  A row of zeros has scale 0, a row with an infinity or NaN scale NaN.  xs .. qs: row strides. */
+ * w == NULL then quantises h itself.  A row of zeros has scale 0, a row of y with an infinity or NaN (its own or the weight's) scale NaN.  xs .. qs: row strides. */
 typedef struct {
     const void *x, *residual; const float* w; void *y, *sum, *q8; float* scale;
     int64_t xs, rs, ys, ss, qs, M;

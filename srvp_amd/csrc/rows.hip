@@ -143,8 +143,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
 // of the unrounded sum, which is formed again from x and residual (from a bfloat16 sum the fp32 dw would be off by its rounding, 2e-3), as is its row norm,
 // beside the other sum of the row: nothing is kept between the passes but the inputs.
 // 8-bit output: row scale s = max|y| / 127, q = round-half-even(h w * (127 / max|h w|)), i.e. y / s: the row's root mean square cancels.  Products and the
-// quotient are formed in 64 bits, so q does not depend on the order of any sum.  A row of zeros has scale 0; a row with an infinity or NaN has scale NaN
-// and q = 0, i.e. stands for NaN.
+// quotient are formed in 64 bits, so q does not depend on the order of any sum.  A row of zeros has scale 0; a row of y with an infinity or NaN (its own, or the
+// weight's) has scale NaN and q = 0, i.e. stands for NaN.
 // TPR threads hold one row in registers: V vectors of VE elements each.
 // Measured (us): 16384 x 4096 bfloat16 with a residual forward 89 = 6.0 TB/s, backward 141 + 5 for dw = 4.8 TB/s; 2304 x 256 float32 3.8, 5.5 + 3.6 (launches);
 // 8-bit output 7 x 4096 5.  Rows that are not whole vectors at borders of 16 bytes take the same vectors from any address (one element a load, a value's
@@ -289,6 +289,20 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
         if (g.res) r.load((const E*)g.res + at * g.rs, g.N, t);
     };
     if (row < g.M) fetch(row);
+    bool wild = false;                                     // whether a weight is NaN or infinite, which leaves no row finite (and `most` would pass over a NaN)
+    if constexpr (Q8 && NORM) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < V * VE; ++i) x += 0.f * wv[i];
+        wild = __any(!(x == 0.f));
+        if constexpr (TPR > 64) {
+            if ((tid & 63) == 0) red[tid >> 6] = wild;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < TPR / 64; ++i) wild = wild || red[i] != 0.f;
+            wild = __builtin_amdgcn_readfirstlane(wild);
+        }
+    }
     for (; row < g.M; row += step) {                       // (the same for all threads of a row, and of a workgroup whose waves meet)
         x.arrived(g.N, t);
         if (g.res) r.arrived(g.N, t);
@@ -320,7 +334,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
             }
             ss = row_sum<TPR>(ss, redd, tid);
             most = row_max<TPR>(most, redd, tid);
-            const bool fine = ss < (double)INFINITY && most < (double)INFINITY;      // (false for NaN)
+            const bool fine = !wild && ss < (double)INFINITY && most < (double)INFINITY;      // (false for NaN)
             const double to = fine && most > 0 ? 127.0 / most : 0.0;
             if (t == 0) g.scale[row] = fine ? (float)(most * (NORM ? 1.0 / sqrt(ss / g.N + (double)g.eps) : 1.0) / 127.0) : NAN;
             signed char* q = g.q + row * g.qs;

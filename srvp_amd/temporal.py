@@ -116,8 +116,8 @@ def rms_norm_backward(d_y, x, weight, *, residual=None, d_sum=None, eps=1e-6):
 
 def rms_norm_int8(x, weight, *, residual=None, eps=1e-6):
     """rms_norm with its output in 8 bits: (q int8 (..., N), scale float32 (...)[, h]) with y ~ q * scale, scale = max|y| / 127 a row and q =
-    round(h weight * (127 / max|h weight|)), half to even, in 64 bits (it does not depend on the order of a sum).  A row of zeros has scale 0, a row with an
-    infinity or NaN scale NaN."""
+    round(h weight * (127 / max|h weight|)), half to even, in 64 bits (it does not depend on the order of a sum).  A row of zeros has scale 0, a row of y with
+    an infinity or NaN, its own or the weight's, scale NaN."""
     return (_ext or load()).rms_norm_int8(x, weight, residual, eps)
 
 

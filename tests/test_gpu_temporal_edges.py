@@ -322,3 +322,23 @@ def test_rotary_of_heads_at_odd_places(D, rot, inter, dt):
         within(o, ref, size, dt, 12 * 2.0 ** -24, 'rotary')
         assert torch.equal(o[..., rot:], x[..., rot:])
         assert torch.equal(o, t.rotary(x.contiguous(), None, pos, w, interleaved=inter, back=back))
+
+
+@pytest.mark.parametrize('M,N', [(3, 7), (9, 300), (5, 1024), (3, 4095), (4, 9000), (2, 16384)])
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), float('-inf')])
+@pytest.mark.parametrize('dt', [BF, FP])
+def test_int8_rows_of_a_weight_that_is_not_finite(M, N, bad, dt):
+    """One weight that is NaN or infinite leaves no row of the norm finite, rows of zeros among them (0 * infinity): scale NaN, and NaN behind the product."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(N)
+    x, r, w = rnd(g, M, N, dtype=dt), rnd(g, M, N, dtype=dt), rnd(g, N)
+    x[1], r[1] = 0, 0
+    for col in {0, N // 2, N - 1}:
+        spoilt = w.clone()
+        spoilt[col] = bad
+        q, s, total = t.rms_norm_int8(x, spoilt, residual=r)
+        assert torch.isnan(s).all() and not q.any()
+        assert torch.equal(total, (x.float() + r.float()).to(dt))
+        assert not torch.isfinite(t.rms_norm(x, spoilt, residual=r)[0][:, col]).any()
+    y = t.linear_int8(q, s, torch.ones(3, N, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV))
+    assert torch.isnan(y).all()
