@@ -91,6 +91,11 @@ bool any_grad(std::initializer_list<const Tensor*> ts) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
+// (a launch would come back without the tangent, whether or not the tensors ask for a gradient)
+void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(std::string(what) + ": forward-mode derivatives are not supported");
+}
 void* stream_of(const Tensor& x) { return (void*)c10::hip::getCurrentHIPStream(x.get_device()).stream(); }
 // whether the call is to be recorded for autograd.  Not inside a capture: leaves whose eager graph is still alive would pull its stream into the captured
 // backward pass, which ends the process.
@@ -224,6 +229,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
 py::object linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Maybe& state, const Maybe& lengths,
                             std::optional<double> scale, bool return_state) {
     const Attention a = attention_args("linear_attention", q, k, v, log_decay, state, lengths, scale);
+    no_tangent("linear_attention", {&a.q, &a.k, &a.v, &a.log_decay, &a.state});
     variable_list r;
     if (records("linear_attention", a.q, {&a.q, &a.k, &a.v, &a.state}))
         r = AttentionNode::apply(a.q, a.k, a.v, a.log_decay, a.state.defined() ? Maybe(a.state) : Maybe(), a.lengths.defined() ? Maybe(a.lengths) : Maybe(), a.scale, return_state);
@@ -236,6 +242,7 @@ py::tuple linear_attention_backward(const Tensor& d_out, const Tensor& q, const 
     const char* what = "linear_attention_backward";
     const Attention a = attention_args(what, q, k, v, log_decay, state, lengths, scale);
     const Tensor dn = get(d_state);
+    no_tangent(what, {&d_out, &a.q, &a.k, &a.v, &a.log_decay, &a.state, &dn});
     no_gradient(what, {&d_out, &a.q, &a.k, &a.v, &a.state, &dn});
     if (d_out.sizes() != a.v.sizes()) value_error(std::string(what) + ": d_out " + shape(a.v) + ", got " + shape(d_out));
     floats(what, {&a.q, &d_out});
@@ -252,6 +259,7 @@ Tensor linear_attention_step(const Tensor& q0, const Tensor& k0, const Tensor& v
     if (q0.dim() != 3 || k0.sizes() != q0.sizes() || v0.dim() != 3 || v0.size(0) != q0.size(0) || v0.size(1) != q0.size(1))
         value_error(std::string(what) + ": q, k (B, H, Dk) and v (B, H, Dv), got " + shape(q0) + ", " + shape(k0) + ", " + shape(v0));
     floats(what, {&q0, &k0, &v0});
+    no_tangent(what, {&q0, &k0, &v0, &log_decay, &state});
     no_gradient(what, {&q0, &k0, &v0, &state});
     const int64_t B = q0.size(0), H = q0.size(1), Dk = q0.size(2), Dv = v0.size(2);
     if (Dk < 1 || Dk > 256 || Dv < 1 || Dv > 256) value_error(std::string(what) + ": heads of 1 to 256 features, got " + std::to_string(Dk) + " and " + std::to_string(Dv));
@@ -337,6 +345,7 @@ py::object rotary(const Tensor& q, const Maybe& k, const Tensor& positions0, con
     if (q.dim() != 4 || (k && (kk.dim() != 4 || kk.size(0) != q.size(0) || kk.size(1) != q.size(1) || kk.size(3) != q.size(3))))
         value_error(std::string(what) + ": q (T, B, Hq, D) and k (T, B, Hk, D), got " + shape(q) + (k ? ", " + shape(kk) : ""));
     floats(what, {&q, &kk});
+    no_tangent(what, {&q, &kk, &freq});
     const int64_t T = q.size(0), B = q.size(1), D = q.size(3);
     if (T >= (1LL << 31) || B >= (1LL << 31) || T * B >= (1LL << 31) || q.size(2) >= (1 << 20) || (k && kk.size(2) >= (1 << 20)))
         value_error(std::string(what) + ": fewer than 2^31 rows and 2^20 heads, got " + shape(q) + (k ? ", " + shape(kk) : ""));
@@ -357,6 +366,7 @@ py::object rotary(const Tensor& q, const Maybe& k, const Tensor& positions0, con
 void norm_args(const char* what, const Tensor& x, const Tensor& weight, const Tensor& residual) {
     on_device(what, x);
     floats(what, {&x, &residual});
+    no_tangent(what, {&x, &weight, &residual});
     if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > 16384) value_error(std::string(what) + ": rows of 1 to 16384 features, got " + shape(x));
     if (x.numel() / x.size(-1) >= (1LL << 31)) value_error(std::string(what) + ": fewer than 2^31 rows");
     if (residual.defined() && residual.sizes() != x.sizes()) value_error(std::string(what) + ": residual " + shape(residual) + " for x " + shape(x));
@@ -470,6 +480,7 @@ Tensor linear_int8(const Tensor& x, const Tensor& x_scale, const Tensor& w0, con
     if (bias) scales(b0, {N}, "bias");
     if (out != at::kFloat && out != at::kBFloat16) type_error(std::string(what) + ": float32 or bfloat16 output");
     same_device(what, x, {&x_scale, &w0, &w_scale, &b0});
+    no_tangent(what, {&x_scale, &w_scale, &b0});
     no_gradient(what, {&x_scale, &w_scale, &b0});
     const c10::DeviceGuard guard(x.device());
     s.push_back(N);

@@ -7,7 +7,7 @@ Tensors are time-major, (T, B, heads, features), float32 or bfloat16; any stride
 copied first), so a batch-major tensor is passed as a transposed view and shared heads as an expanded one.  Every sum, state and norm is held in 32
 bits or more.  Launches go to torch's current stream on the tensors' device; workspaces are ordinary tensors of the call.
 
-Gradients: `linear_attention`, `rotary` and `rms_norm` are autograd nodes, differentiable once.  Inside a stream capture they record none (a captured backward
+Gradients: `linear_attention`, `rotary` and `rms_norm` are autograd nodes, differentiable once, in reverse mode (tensors with a forward-mode tangent are refused).  Inside a stream capture they record none (a captured backward
 pass cannot be told apart from the eager one of the same leaves) and raise: call `linear_attention_backward`, `rotary(..., back=True)`, `rms_norm_backward`
 there.
 

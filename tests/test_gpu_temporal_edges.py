@@ -342,3 +342,36 @@ def test_int8_rows_of_a_weight_that_is_not_finite(M, N, bad, dt):
         assert not torch.isfinite(t.rms_norm(x, spoilt, residual=r)[0][:, col]).any()
     y = t.linear_int8(q, s, torch.ones(3, N, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV))
     assert torch.isnan(y).all()
+
+
+def test_forward_mode_is_refused():
+    """A tangent on any input of any operator, with gradients enabled or not: an error, never an output without its tangent."""
+    import torch.autograd.forward_ad as fwd
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(13)
+    x, st, ld = rnd(g, 4, 2, 3, 8), rnd(g, 2, 3, 8, 8), decays(3)
+    w, pos, freq = rnd(g, 8), torch.arange(4, device=DEV), t.rotary_frequencies(8, device=DEV)
+    i8, one = torch.ones(4, 8, dtype=torch.int8, device=DEV), torch.ones(4, device=DEV)
+    calls = [
+        (lambda q, k, v, l, s: t.linear_attention(q, k, v, l, state=s), (x, x, x, ld, st)),
+        (lambda d, q, k, v, l, s, n: t.linear_attention_backward(d, q, k, v, l, state=s, d_state=n), (x, x, x, x, ld, st, st)),
+        (lambda q, k, v, l, s: t.linear_attention_step(q, k, v, l, s), (x[0], x[0], x[0], ld, st)),
+        (lambda q, k, f: t.rotary(q, k, pos, f), (x, x, freq)),
+        (lambda a, b, r: t.rms_norm(a, b, residual=r), (x, w, x)),
+        (lambda d, a, b, r, s: t.rms_norm_backward(d, a, b, residual=r, d_sum=s), (x, x, w, x, x)),
+        (lambda a, b, r: t.rms_norm_int8(a, b, residual=r), (x, w, x)),
+        (lambda a: t.quantize_int8(a), (x,)),
+        (lambda a, b, c: t.linear_int8(i8, a, i8, b, bias=c), (one, one, one)),
+    ]
+    for f, args in calls:
+        f(*args)
+        before = [a.clone() for a in args]
+        for i in range(len(args)):
+            for enabled in (True, False):
+                with fwd.dual_level(), torch.set_grad_enabled(enabled):
+                    duals = list(args)
+                    duals[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                    with pytest.raises(RuntimeError, match='forward-mode'):
+                        f(*duals)
+        for a, b in zip(args, before):
+            assert torch.equal(a, b)
