@@ -354,6 +354,7 @@ py::object rotary(const Tensor& q, const Maybe& k, const Tensor& positions0, con
         value_error(std::string(what) + ": positions (" + std::to_string(T) + ",) or (" + std::to_string(T) + ", " + std::to_string(B) + "), got " + shape(positions0));
     if (freq.scalar_type() != at::kDouble || freq.dim() != 1 || 2 * freq.size(0) > D || !freq.is_contiguous())
         value_error(std::string(what) + ": frequencies is a contiguous float64 tensor of at most " + std::to_string(D / 2) + " pairs, got " + shape(freq) + " " + dtype(freq));
+    if (any_grad({&freq})) value_error(std::string(what) + ": the frequencies are constants: they must not require a gradient");
     if (!std::isfinite((float)magnitude)) value_error(std::string(what) + ": magnitude must be finite");
     const Tensor positions = whole(what, "positions", positions0);
     same_device(what, q, {&kk, &positions, &freq});

@@ -375,3 +375,16 @@ def test_forward_mode_is_refused():
                         f(*duals)
         for a, b in zip(args, before):
             assert torch.equal(a, b)
+
+
+def test_frequencies_take_no_gradient():
+    """Frequencies that ask for a gradient would be left without one: refused, as decays are; without recording they are taken as they are."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(14)
+    x, pos, w = rnd(g, 4, 2, 3, 8), torch.arange(4, device=DEV), t.rotary_frequencies(8, device=DEV)
+    learnt = w.clone().requires_grad_()
+    for q in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match='frequencies'):
+            t.rotary(q, None, pos, learnt)
+    with torch.no_grad():
+        assert torch.equal(t.rotary(x, None, pos, learnt), t.rotary(x, None, pos, w))
