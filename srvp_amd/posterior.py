@@ -45,7 +45,7 @@ class AttentionPosterior(nn.Module):
         self.last_norm = _Scale(nh)
         self.register_buffer('log_decay', temporal.decay_rates(heads), persistent=False)
         self.register_buffer('frequencies', temporal.rotary_frequencies(self.width // 2 * 2), persistent=False)
-        self._q8 = None
+        self._eight_bits = False
 
     def _constants(self):
         """The constants in their own types, whatever .half() / .double() of the model did to the buffers."""
@@ -56,22 +56,21 @@ class AttentionPosterior(nn.Module):
         return self.log_decay, self.frequencies
 
     # ---- 8-bit inference
-    def _versions(self):
-        return self.qkv.weight._version, self.out.weight._version, self.qkv.weight.data_ptr()
-
-    @torch.no_grad()
     def quantize(self):
-        """8-bit copies of the two inner weights as they are now, for the inference calls from here on (dropped by the next training pass)."""
-        self._q8 = (temporal.quantize_int8(self.qkv.weight), temporal.quantize_int8(self.out.weight), self._versions())
+        """The two inner products on 8-bit integers, for the inference calls from here on (dropped by the next training pass)."""
+        self._eight_bits = True
 
     def drop_quantized(self):
-        self._q8 = None
+        self._eight_bits = False
 
+    @torch.no_grad()
     def quantized(self):
-        """The 8-bit weights, or None.  Weights that were replaced since are quantised again."""
-        if self._q8 is not None and self._q8[2] != self._versions():
-            self.quantize()
-        return self._q8
+        """None, or the two inner weights in 8 bits as they are now (w, scales of its rows), and the weights these stand for.  Formed anew for every call (one launch a
+        weight): the fused optimizer and writes through .data leave nothing by which a kept copy would know that it is old."""
+        if not self._eight_bits:
+            return None
+        w = self.qkv.weight, self.out.weight
+        return temporal.quantize_int8(w[0]), temporal.quantize_int8(w[1]), w
 
     # ---- the block
     def _project(self, x, weight, out):

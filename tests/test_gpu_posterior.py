@@ -200,3 +200,45 @@ def test_lstm_model_refuses():
     for f in (model.quantize_posterior, lambda: model.posterior_stream(2)):
         with pytest.raises(ValueError):
             f()
+
+
+@pytest.mark.parametrize('change', ['out.data', 'qkv.data in place', 'out.data in place', 'optimizer', 'state dict', 'parameter'])
+def test_quantized_inference_uses_the_weights_of_the_call(change):
+    """Whatever changes a weight after quantize_posterior: the next sequence, and the next frame of a stream, run on 8-bit copies of the new one."""
+    import srvp_amd
+    from srvp_amd.posterior import AttentionPosterior, PosteriorStream
+    ctor, model = small_model()
+    model = model.cuda().eval()
+    net = model.inf_z
+    optim = srvp_amd.FusedAdam(model, lr=1e-2)
+    optim.zero_grad()
+    g = torch.Generator().manual_seed(9)
+    hx = torch.randn(6, 5, 16, generator=g).cuda()
+    model.quantize_posterior()
+    before = net.run(hx, False)[0].clone()
+    stream = model.posterior_stream(5)
+    first = stream.step(hx[0])[0].clone()
+    other = (0.3 * torch.randn(24, 24, generator=g)).cuda()
+    if change == 'out.data':
+        net.out.weight.data = other
+    elif change == 'qkv.data in place':
+        net.qkv.weight.data.mul_(-1.5)
+    elif change == 'out.data in place':
+        net.out.weight.data.copy_(other)
+    elif change == 'optimizer':
+        model._flat[1].normal_()
+        optim.step()
+    elif change == 'state dict':
+        net.load_state_dict({**net.state_dict(), 'out.weight': other})
+    else:
+        net.out.weight = torch.nn.Parameter(other)
+    fresh = AttentionPosterior(16, 24, 2).cuda()
+    fresh.load_state_dict({k: v.clone() for k, v in net.state_dict().items()})
+    fresh.quantize()
+    want = fresh.run(hx, False)[0]
+    got = net.run(hx, False)[0]
+    assert torch.equal(got, want) and not torch.equal(got, before)
+    stream.reset()
+    again = PosteriorStream(fresh, model.q_z, 5, 'cuda')
+    frame = stream.step(hx[0])[0]
+    assert torch.equal(frame, again.step(hx[0])[0]) and not torch.equal(frame, first)
