@@ -440,7 +440,7 @@ def elbo(x: Tensor, outs, obs_scale: float, beta_y: float, beta_z: float, l2_res
 
 def split_state(sd: SD) -> Tuple[List[str], List[str]]:
     """Parameter keys (in module registration order = state-dict order) and buffer keys."""
-    buf = ('running_mean', 'running_var', 'num_batches_tracked')
+    buf = ('running_mean', 'running_var', 'num_batches_tracked', 'log_decay')
     p = [k for k in sd if not k.endswith(buf)]
     b = [k for k in sd if k.endswith(buf)]
     return p, b

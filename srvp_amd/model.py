@@ -143,7 +143,8 @@ class _SrvpForward(torch.autograd.Function):
 
 class StochasticLatentResidualVideoPredictor(nn.Module):
     def __init__(self, nx, nc, nf, nhx, ny, nz, skipco, nt_inf, nh_inf, nlayers_inf, nh_res, nlayers_res, archi, *, posterior='lstm', posterior_heads=None):
-        """posterior: 'lstm' (the reference's) or 'attention' (srvp_amd.posterior; posterior_heads: default heads of 64 features)."""
+        """posterior: 'lstm' (the reference's) or 'attention' (srvp_amd.posterior; posterior_heads: default heads of 64 features; a state dict of another number is
+        refused)."""
         super().__init__()
         if posterior not in ('lstm', 'attention'):
             raise ValueError(f"posterior 'lstm' or 'attention', got {posterior!r}")
@@ -249,6 +250,20 @@ class StochasticLatentResidualVideoPredictor(nn.Module):
         self._plans = {}
         self._pack_version = None
         return self
+
+    # ------------------------------------------------------------------------------------------------ state dict
+    # The attention posterior's decays stand beside its parameters (whose names are inf_z.*), as posterior_log_decay.
+    def state_dict(self, *args, **kw):
+        sd = super().state_dict(*args, **kw)
+        if self.posterior == 'attention':
+            prefix = args[1] if len(args) > 1 else kw.get('prefix', '')
+            sd[prefix + 'posterior_log_decay'] = sd.pop(prefix + 'inf_z.log_decay')
+        return sd
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        if self.posterior == 'attention' and prefix + 'posterior_log_decay' in state_dict:
+            state_dict[prefix + 'inf_z.log_decay'] = state_dict.pop(prefix + 'posterior_log_decay')
+        super()._load_from_state_dict(state_dict, prefix, *args)
 
     # ------------------------------------------------------------------------------------------------ plumbing
     def _cfg(self):

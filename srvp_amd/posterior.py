@@ -8,6 +8,8 @@ a single new frame costs one update of a state (`PosteriorStream`).
 
 fp32 like the rest of the latent path; for inference the two inner products can run on 8-bit integers (`quantize`).
 """
+import warnings
+
 import torch
 import torch.nn as nn
 
@@ -29,7 +31,10 @@ class _Scale(nn.Module):
 
 
 class AttentionPosterior(nn.Module):
-    """Parameter container (like every module of the model, its forward is never called): decays and frequencies are constants."""
+    """Parameter container (like every module of the model, its forward is never called): decays and frequencies are constants.  The decays, one a head, are part of the
+    state dict: no parameter's shape tells the number of heads, and weights of another number are refused by their length."""
+
+    _version = 2                                       # 1: without the decays
 
     def __init__(self, nhx, nh, heads=None):
         super().__init__()
@@ -43,9 +48,15 @@ class AttentionPosterior(nn.Module):
         self.out_norm = _Scale(nh)
         self.out = nn.Linear(nh, nh, bias=False)
         self.last_norm = _Scale(nh)
-        self.register_buffer('log_decay', temporal.decay_rates(heads), persistent=False)
+        self.register_buffer('log_decay', temporal.decay_rates(heads))
         self.register_buffer('frequencies', temporal.rotary_frequencies(self.width // 2 * 2), persistent=False)
         self._eight_bits = False
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, *args):
+        if prefix + 'log_decay' not in state_dict and local_metadata.get('version') == 1:
+            warnings.warn(f'srvp_amd: weights of an attention posterior that were saved without its number of heads: taken for {self.heads}')
+            state_dict[prefix + 'log_decay'] = self.log_decay
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, *args)
 
     def _constants(self):
         """The constants in their own types, whatever .half() / .double() of the model did to the buffers."""

@@ -133,3 +133,51 @@ def test_rotary_in_place_is_refused():
     one = dict(q=16, oq=32, positions=16, freq=16, T=1, B=1, Hq=1, D=8, pairs=4, magnitude=1.0)
     for same in (dict(oq=16), dict(k=64, ok=64, Hk=1)):
         assert L.load().srvp_rotary(C.byref(L.RotaryDesc(**dict(one, **same))), None) == 1 and b'in the place' in L.load().srvp_last_error()
+
+
+def test_posterior_weights_of_another_number_of_heads_are_refused(tmp_path):
+    """No parameter's shape tells the heads apart: the decays do, through every way a state dict travels; weights saved before they were in it come with a warning."""
+    import warnings
+    import srvp_amd
+    from srvp_amd.posterior import AttentionPosterior
+    torch.manual_seed(0)
+    three, two = AttentionPosterior(8, 24, 3), AttentionPosterior(8, 24, 2)
+    with pytest.raises(RuntimeError, match='size mismatch for log_decay'):
+        two.load_state_dict(three.state_dict())
+    ctor = (64, 1, 4, 8, 3, 3, False, 2, 24, 3, 16, 4, 'dcgan')
+    make = lambda heads: srvp_amd.StochasticLatentResidualVideoPredictor(*ctor, posterior='attention', posterior_heads=heads)
+    a = make(3)
+    a.inf_z.log_decay[1] = -0.25                       # (decays travel as values)
+    path = tmp_path / 'model.pt'
+    torch.save(dict(model=a.state_dict()), path)
+    ways = {'itself': a.state_dict(), 'plain': {k: v.clone() for k, v in a.state_dict().items()}, 'file': torch.load(path, weights_only=True)['model']}
+    for way, sd in ways.items():
+        with pytest.raises(RuntimeError, match='size mismatch for inf_z.log_decay'):
+            make(2).load_state_dict(sd)
+        b = make(3)
+        assert str(b.load_state_dict(sd)) == '<All keys matched successfully>', way
+        for (k, x), (l, y) in zip(a.state_dict().items(), b.state_dict().items()):
+            assert k == l and torch.equal(x, y)
+        assert b.inf_z.log_decay[1] == -0.25
+    inside = torch.nn.Sequential(a)
+    assert '0.posterior_log_decay' in inside.state_dict()
+    torch.nn.Sequential(make(3)).load_state_dict(inside.state_dict())
+    with pytest.raises(RuntimeError, match='size mismatch'):
+        torch.nn.Sequential(make(2)).load_state_dict(inside.state_dict())
+    missing = {k: v for k, v in a.state_dict().items() if k != 'posterior_log_decay'}
+    with pytest.raises(RuntimeError, match='Missing key'):
+        make(3).load_state_dict(missing)
+    # the form without the decays
+    old = a.state_dict()
+    del old['posterior_log_decay']
+    old._metadata['inf_z']['version'] = 1
+    c = make(3)
+    with pytest.warns(UserWarning, match='number of heads'):
+        c.load_state_dict(old)
+    assert torch.equal(c.inf_z.qkv.weight, a.inf_z.qkv.weight) and torch.equal(c.inf_z.log_decay, t.decay_rates(3))
+    # the LSTM's state dict is the reference's
+    lstm = srvp_amd.StochasticLatentResidualVideoPredictor(*ctor)
+    with warnings.catch_warnings():
+        warnings.simplefilter('error')
+        lstm.load_state_dict(lstm.state_dict())
+    assert not any('decay' in k for k in lstm.state_dict())
