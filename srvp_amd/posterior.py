@@ -58,12 +58,17 @@ class AttentionPosterior(nn.Module):
             state_dict[prefix + 'log_decay'] = self.log_decay
         super()._load_from_state_dict(state_dict, prefix, local_metadata, *args)
 
+    def _apply(self, fn, *args, **kw):
+        # the constants follow the model to its device and keep their types and values: .half() or .float() would round them for good
+        ld, fr = self.log_decay, self.frequencies
+        r = super()._apply(fn, *args, **kw)
+        dev = self.log_decay.device
+        if ld.is_meta and dev.type != 'meta':
+            ld, fr = temporal.decay_rates(self.heads), temporal.rotary_frequencies(self.width // 2 * 2)
+        self.log_decay, self.frequencies = ld.to(dev), fr.to(dev)
+        return r
+
     def _constants(self):
-        """The constants in their own types, whatever .half() / .double() of the model did to the buffers."""
-        if self.log_decay.dtype is not torch.float32:
-            self.log_decay = self.log_decay.float()
-        if self.frequencies.dtype is not torch.float64:
-            self.frequencies = temporal.rotary_frequencies(self.width // 2 * 2, device=self.log_decay.device)
         return self.log_decay, self.frequencies
 
     # ---- 8-bit inference

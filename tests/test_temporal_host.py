@@ -181,3 +181,21 @@ def test_posterior_weights_of_another_number_of_heads_are_refused(tmp_path):
         warnings.simplefilter('error')
         lstm.load_state_dict(lstm.state_dict())
     assert not any('decay' in k for k in lstm.state_dict())
+
+
+def test_posterior_constants_keep_their_types():
+    """Casts of the model, one after another, leave the decays and frequencies as they are."""
+    from srvp_amd.posterior import AttentionPosterior
+    net = torch.nn.Sequential(AttentionPosterior(8, 24, 3))
+    ld, fr = t.decay_rates(3), t.rotary_frequencies(8)
+    for cast in (lambda: net.half(), lambda: net.float(), lambda: net.bfloat16(), lambda: net.double(), lambda: net.to(torch.float32), lambda: net.float().double().float()):
+        cast()
+        a, b = net[0]._constants()
+        assert a.dtype is torch.float32 and b.dtype is torch.float64 and torch.equal(a, ld) and torch.equal(b, fr)
+    net[0].log_decay.fill_(-0.5)
+    net.half().float()
+    assert (net[0].log_decay == -0.5).all()
+    with torch.device('meta'):
+        far = AttentionPosterior(8, 24, 3)
+    far.to_empty(device='cpu')
+    assert torch.equal(far.log_decay, ld) and torch.equal(far.frequencies, fr)
