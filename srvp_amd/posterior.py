@@ -22,6 +22,11 @@ def default_heads(nh):
     return nh // 64 if nh % 64 == 0 else 1
 
 
+def _empty(like, *shape):
+    """fp32, which is what the launches write, whatever torch's default type is."""
+    return torch.empty(*shape, dtype=torch.float32, device=like.device)
+
+
 class _Scale(nn.Module):
     """Parameter container of a row norm."""
 
@@ -98,12 +103,12 @@ class AttentionPosterior(nn.Module):
         from .latent import linear_fwd
         if hx.shape[-1] != self.inp.weight.shape[1] or hx.device != self.inp.weight.device:
             raise ValueError(f'posterior attention: encodings of {self.inp.weight.shape[1]} features on {self.inp.weight.device}, got {tuple(hx.shape)} on {hx.device}')
-        u = torch.empty(hx.shape[0], self.heads * self.width, device=hx.device)
+        u = _empty(hx, hx.shape[0], self.heads * self.width)
         linear_fwd(L.stream(), hx, self.inp.weight, self.inp.bias, u)
         if q8 is not None:
             return u, None, temporal.linear_int8(*temporal.rms_norm_int8(u, self.norm.weight), *q8[0])
         n = temporal.rms_norm(u, self.norm.weight)
-        return u, n, self._project(n, self.qkv.weight, torch.empty(hx.shape[0], 3 * u.shape[1], device=hx.device))
+        return u, n, self._project(n, self.qkv.weight, _empty(hx, hx.shape[0], 3 * u.shape[1]))
 
     def _outputs(self, o, u, q8):
         """Attention's output (rows, nh) and u -> norm(o) (None in 8 bits), z, hz."""
@@ -165,7 +170,7 @@ class PosteriorStream:
 
     def __init__(self, net, q_z, rows, device):
         self.net, self.q_z = net, q_z
-        self.state = torch.zeros(rows, net.heads, net.width, net.width, device=device)
+        self.state = torch.zeros(rows, net.heads, net.width, net.width, dtype=torch.float32, device=device)
         self.position = torch.zeros(1, rows, dtype=torch.int64, device=device)
 
     def reset(self, rows=None):
@@ -189,6 +194,6 @@ class PosteriorStream:
         o = temporal.linear_attention_step(q[0], k[0], v[0], ld, self.state).view(B, -1)
         self.position += 1
         hz = net._outputs(o, u, q8)[2]
-        p = torch.empty(B, self.q_z.weight.shape[0], device=hz.device)
+        p = _empty(hz, B, self.q_z.weight.shape[0])
         linear_fwd(L.stream(), hz, self.q_z.weight, self.q_z.bias, p)
         return hz, p

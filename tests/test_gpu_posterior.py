@@ -242,3 +242,40 @@ def test_quantized_inference_uses_the_weights_of_the_call(change):
     again = PosteriorStream(fresh, model.q_z, 5, 'cuda')
     frame = stream.step(hx[0])[0]
     assert torch.equal(frame, again.step(hx[0])[0]) and not torch.equal(frame, first)
+
+
+@pytest.mark.parametrize('default', [torch.float64, torch.bfloat16])
+def test_default_type_does_not_matter(default):
+    """The block's buffers are float32 whatever torch's default type is (a smaller one would be written past its end)."""
+    from srvp_amd.posterior import AttentionPosterior, PosteriorStream
+    torch.manual_seed(2)
+    net, qz = AttentionPosterior(16, 24, 2).cuda(), torch.nn.Linear(24, 14).cuda()
+    g = torch.Generator().manual_seed(4)
+    hx, d = torch.randn(7, 3, 16, generator=g).cuda(), torch.randn(21, 24, generator=g).cuda()
+
+    def everything():
+        out = []
+        net.drop_quantized()
+        hz, saved = net.run(hx, True)
+        grads = {f'inf_z.{k}': torch.zeros_like(p) for k, p in net.named_parameters()}
+        d_hx = torch.zeros(21, 16, dtype=torch.float32, device='cuda')
+        keep = net.backward(hx, d, saved, grads, 'inf_z', d_hx)
+        for bits in (False, True):
+            if bits:
+                net.quantize()
+            out.append(net.run(hx, False)[0])
+            stream = PosteriorStream(net, qz, 3, 'cuda')
+            for t in range(3):
+                out += stream.step(hx[t])
+        torch.cuda.synchronize()
+        del keep
+        return [hz, d_hx] + list(grads.values()) + out
+    want = everything()
+    torch.set_default_dtype(default)
+    try:
+        got = everything()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    for a, b in zip(got, want):
+        # (weight gradients are sums over parts of the rows in any order)
+        assert a.dtype is torch.float32 and rel(a, b) < 1e-5
