@@ -99,10 +99,12 @@ class AttentionPosterior(nn.Module):
         return linear_fwd(L.stream(), x, weight, None, out)
 
     def _inputs(self, hx, q8):
-        """hx (rows, nhx) -> u, norm(u) (None in 8 bits), (rows, 3 nh)."""
+        """hx (rows, nhx), contiguous -> u, norm(u) (None in 8 bits), (rows, 3 nh)."""
         from .latent import linear_fwd
         if hx.shape[-1] != self.inp.weight.shape[1] or hx.device != self.inp.weight.device:
             raise ValueError(f'posterior attention: encodings of {self.inp.weight.shape[1]} features on {self.inp.weight.device}, got {tuple(hx.shape)} on {hx.device}')
+        if any(x.dtype is not torch.float32 for x in (hx, self.inp.weight, self.qkv.weight, self.out.weight)):
+            raise TypeError(f'posterior attention: float32 encodings and weights, got {hx.dtype} and {self.inp.weight.dtype}, {self.qkv.weight.dtype}, {self.out.weight.dtype}')
         u = _empty(hx, hx.shape[0], self.heads * self.width)
         linear_fwd(L.stream(), hx, self.inp.weight, self.inp.bias, u)
         if q8 is not None:
@@ -127,7 +129,7 @@ class AttentionPosterior(nn.Module):
             self.drop_quantized()
         q8 = None if training else self.quantized()
         ld, fr = self._constants()
-        u, n, qkv = self._inputs(hx.reshape(T * B, -1), q8)
+        u, n, qkv = self._inputs(hx.reshape(T * B, -1).contiguous(), q8)      # (rows of a slice may lie apart: the products take whole ones)
         q, k, v = qkv.view(T, B, 3, self.heads, self.width).unbind(2)
         pos = torch.arange(T, device=hx.device)
         q, k = temporal.rotary(q, k, pos, fr)
@@ -160,7 +162,7 @@ class AttentionPosterior(nn.Module):
         linear_bwd(st, n, self.qkv.weight, d_qkv, grads[f'{prefix}.qkv.weight'], None, dx=d_n, defer=defer)
         d_u, dw = temporal.rms_norm_backward(d_n, u, self.norm.weight, d_sum=d_zu)
         add('norm', dw)
-        linear_bwd(st, hx.reshape(R, -1), self.inp.weight, d_u, grads[f'{prefix}.inp.weight'], grads[f'{prefix}.inp.bias'], dx=d_hx, dx_acc=1, defer=defer)
+        linear_bwd(st, hx.reshape(R, -1).contiguous(), self.inp.weight, d_u, grads[f'{prefix}.inp.weight'], grads[f'{prefix}.inp.bias'], dx=d_hx, dx_acc=1, defer=defer)
         return d_zu, d_qkv, d_u, saved
 
 

@@ -279,3 +279,32 @@ def test_default_type_does_not_matter(default):
     for a, b in zip(got, want):
         # (weight gradients are sums over parts of the rows in any order)
         assert a.dtype is torch.float32 and rel(a, b) < 1e-5
+
+
+def test_encodings_of_any_strides():
+    """Slices and transposed views of encodings: the results of their copies; other types than float32 are refused."""
+    from srvp_amd.posterior import AttentionPosterior
+    torch.manual_seed(2)
+    net = AttentionPosterior(16, 24, 2).cuda()
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randn(7, 3, 40, generator=g).cuda()
+    for hx in (wide[..., 5:21], wide[:, :, :16], torch.randn(3, 7, 16, generator=g).cuda().transpose(0, 1)):
+        copy = hx.clone(memory_format=torch.contiguous_format)
+        d = torch.randn(24, 21, generator=g).cuda().t()
+        results = []
+        for x, dy in ((hx, d), (copy, d.contiguous())):
+            hz, saved = net.run(x, True)
+            grads = {f'inf_z.{k}': torch.zeros_like(p) for k, p in net.named_parameters()}
+            d_hx = torch.zeros(21, 16, device='cuda')
+            keep = net.backward(x, dy, saved, grads, 'inf_z', d_hx)
+            torch.cuda.synchronize()
+            results.append([hz, d_hx] + list(grads.values()))
+            del keep
+        assert torch.equal(results[0][0], results[1][0])
+        for a, b in zip(*results):
+            assert rel(a, b) < 1e-5
+    for bad in (wide[..., :16].double(), wide[..., :16].bfloat16()):
+        with pytest.raises(TypeError):
+            net.run(bad, False)
+    with pytest.raises(TypeError):
+        AttentionPosterior(16, 24, 2).cuda().double().run(wide[..., :16], False)
