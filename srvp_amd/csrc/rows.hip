@@ -6,7 +6,7 @@
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------------------- rotary
-// Pair p of a head is turned by positions[t][b] * freq[p] radians.  The angle is formed in 64 bits as a number of whole turns, of which only the
+// Pair p of a head is turned by positions[t][b] * freq[p] radians.  The angle is formed as a number of whole turns in pairs of 64-bit values, of which only the
 // fraction matters; its sine and cosine are computed once a (row, pair) for all heads of q and k, in LDS.
 struct Div {                               // n / d for n < 2^31 as one high product: m = ceil(2^(32 + s) / d), s = ceil(log2 d) - 1
     unsigned d, m, s;
@@ -19,6 +19,16 @@ Div divide(unsigned d) {
         r.m = (unsigned)(((1ull << (32 + r.s)) + d - 1) / d);
     }
     return r;
+}
+// pos * freq / (2 pi) without its whole turns, to 2^-52 of a turn for |pos| up to 2^53: every product with its rounding (the fma's) beside it, 1 / (2 pi) in two
+// values.  In one value each, the angle would be off by 2.5 * 2^-53 of itself: by more than the sine's own rounding from 10^8 radians on.
+__device__ __forceinline__ double fraction_of_turns(double pos, double freq) {
+#pragma clang fp contract(off)
+    constexpr double c = 0x1.45f306dc9c883p-3, c_rest = -0x1.6b01ec5417056p-57;
+    const double w = freq * c, w_rest = fma(freq, c, -w) + freq * c_rest;
+    const double t = pos * w, t_rest = fma(pos, w, -t) + pos * w_rest;
+    const double r = (t - rint(t)) + t_rest;
+    return r - rint(r);
 }
 struct RotArgs {
     const void *x[2];
@@ -51,8 +61,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
     const int R = (int)min((long long)g.R, rows - row0);
     for (int i = tid; i < R * g.n; i += 256) {
         const unsigned r = g.dn.of(i), p = i - r * g.n, row = (unsigned)row0 + r, t = g.dB.of(row), b = row - t * g.B;
-        double turns = (double)g.pos[t * g.pt + b * g.pb] * (g.freq[p] * 0.15915494309189535);
-        turns -= rint(turns);
+        const double turns = fraction_of_turns((double)g.pos[t * g.pt + b * g.pb], g.freq[p]);
         float s, c;
         sincospif(2.f * (float)turns, &s, &c);
         tc[i] = c * g.mult;

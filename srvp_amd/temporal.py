@@ -95,7 +95,7 @@ def rotary_frequencies(features, base=10000.0, *, method='none', factor=1.0, tra
 def rotary(q, k, positions, frequencies, *, interleaved=False, back=False, magnitude=1.0):
     """Turns the pairs of features of q (T, B, Hq, D) and, in the same launch, of k (T, B, Hk, D; None: q alone) by positions * frequencies radians.
 
-    positions (T,) or (T, B), whole numbers of any size (angles are formed in 64 bits); frequencies float64 (pairs,) on the device, 2 * pairs <= D
+    positions (T,) or (T, B), whole numbers up to 2^53 (angles are formed to 2^-52 of a turn); frequencies float64 (pairs,) on the device, 2 * pairs <= D
     (rotary_frequencies; constants, no gradient): features behind the first 2 * pairs are passed on unchanged.  interleaved: pair p is features (2p, 2p + 1), otherwise
     (p, pairs + p).  magnitude multiplies the turned features.  back: the negative angle, which is the gradient's.  Returns q', or (q', k')."""
     return (_ext or load()).rotary(q, k, positions, frequencies, interleaved, back, magnitude)

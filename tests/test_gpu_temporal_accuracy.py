@@ -48,3 +48,43 @@ def test_results_do_not_depend_on_what_else_was_asked_for(T, B, H, Dk, Dv, dt):
         outs.append((o.detach(),) + torch.autograd.grad(o, leaves + ([s] if wanted else []), do)[:3])
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def exact_angle(position, frequency):
+    """position * frequency without its whole turns, to about 1e-30 (the double nearest to it)."""
+    from decimal import Decimal, getcontext
+    getcontext().prec = 70
+
+    def arctan_of_inverse(n):                             # its series; pi = 16 arctan(1/5) - 4 arctan(1/239)
+        term = total = Decimal(1) / n
+        k = 1
+        while abs(term) > Decimal(10) ** -68:
+            term, k = -term / (n * n), k + 2
+            total += term / k
+        return total
+    pi = 16 * arctan_of_inverse(5) - 4 * arctan_of_inverse(239)
+    a = Decimal(position) * Decimal(frequency)
+    return float(a - (a / (2 * pi)).to_integral_value() * 2 * pi)
+
+
+@pytest.mark.parametrize('far', [10 ** 3, 10 ** 8, 2 ** 33 + 5, 10 ** 12, 2 ** 45 + 1, 2 ** 53 - 9])
+@pytest.mark.parametrize('inter', [False, True])
+def test_rotary_at_any_position(far, inter):
+    """Angles against exact arithmetic, negative positions among them: the sine's and cosine's own rounding wherever the position lies (an angle formed in 64 bits
+    alone would be off by 1e-4 radians at 10^12 and by whole turns at 2^53)."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(far % 1000)
+    T, D = 8, 16
+    x = rnd(g, T, 1, 2, D)
+    pos = [far - i if i % 2 else i - far for i in range(T)]
+    w = t.rotary_frequencies(D, base=500.0)
+    angles = torch.tensor([[exact_angle(p, f) for f in w.tolist()] for p in pos], dtype=torch.float64, device=DEV).view(T, 1, 1, D // 2)
+    c, s = torch.cos(angles), torch.sin(angles)
+    at = (slice(0, D, 2), slice(1, D, 2)) if inter else (slice(0, D // 2), slice(D // 2, D))
+    u, v = x.double()[..., at[0]], x.double()[..., at[1]]
+    ref, size = torch.empty(T, 1, 2, D, dtype=torch.float64, device=DEV), torch.empty(T, 1, 2, D, dtype=torch.float64, device=DEV)
+    ref[..., at[0]], ref[..., at[1]] = u * c - v * s, u * s + v * c
+    size[..., at[0]] = size[..., at[1]] = u.abs() + v.abs()
+    out = t.rotary(x, None, torch.tensor(pos, device=DEV), w.to(DEV), interleaved=inter)
+    # the fraction of a turn in fp32, half a turn at most: pi 2^-24 radians; sine and cosine 2 units each, two products and a sum
+    within(out, ref, size, torch.float32, 8 * 2.0 ** -24, 'turned')
