@@ -63,9 +63,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
         const unsigned r = g.dn.of(i), p = i - r * g.n, row = (unsigned)row0 + r, t = g.dB.of(row), b = row - t * g.B;
         const double turns = fraction_of_turns((double)g.pos[t * g.pt + b * g.pb], g.freq[p]);
         float s, c;
-        sincospif(2.f * (float)turns, &s, &c);
-        tc[i] = c * g.mult;
-        ts[i] = s * g.mult * g.sign;
+        const float near = (float)turns, rest = (float)(turns - (double)near) * 6.28318531f;      // (to the first order: what the fp32 fraction leaves, up to 10^-7 radians)
+        sincospif(2.f * near, &s, &c);
+        tc[i] = __builtin_fmaf(-s, rest, c) * g.mult;
+        ts[i] = __builtin_fmaf(c, rest, s) * g.mult * g.sign;
     }
     __syncthreads();
     const int H = g.H0 + g.H1, items = g.ditems.d, total = R * H * items;

@@ -2,6 +2,9 @@
 What the bfloat16 attention may round: its outputs to their own type, and nothing else to as few bits.  Short sequences behind a state, so that the bound counts a handful of
 roundings and not the length of the sums.
 """
+import math
+from decimal import Context, Decimal, localcontext
+
 import pytest
 import torch
 
@@ -50,21 +53,30 @@ def test_results_do_not_depend_on_what_else_was_asked_for(T, B, H, Dk, Dv, dt):
         assert torch.equal(a, b)
 
 
-def exact_angle(position, frequency):
-    """position * frequency without its whole turns, to about 1e-30 (the double nearest to it)."""
-    from decimal import Decimal, getcontext
-    getcontext().prec = 70
+DIGITS = Context(prec=70)
 
-    def arctan_of_inverse(n):                             # its series; pi = 16 arctan(1/5) - 4 arctan(1/239)
+
+def exact_pi():
+    """pi = 16 arctan(1/5) - 4 arctan(1/239), by the series."""
+    def arctan_of_inverse(n):
         term = total = Decimal(1) / n
         k = 1
         while abs(term) > Decimal(10) ** -68:
             term, k = -term / (n * n), k + 2
             total += term / k
         return total
-    pi = 16 * arctan_of_inverse(5) - 4 * arctan_of_inverse(239)
-    a = Decimal(position) * Decimal(frequency)
-    return float(a - (a / (2 * pi)).to_integral_value() * 2 * pi)
+    with localcontext(DIGITS):
+        return 16 * arctan_of_inverse(5) - 4 * arctan_of_inverse(239)
+
+
+PI = exact_pi()
+
+
+def exact_angle(position, frequency):
+    """position * frequency without its whole turns, to about 1e-30 (the double nearest to it)."""
+    with localcontext(DIGITS):
+        a = Decimal(position) * Decimal(frequency)
+        return float(a - (a / (2 * PI)).to_integral_value() * 2 * PI)
 
 
 @pytest.mark.parametrize('far', [10 ** 3, 10 ** 8, 2 ** 33 + 5, 10 ** 12, 2 ** 45 + 1, 2 ** 53 - 9])
@@ -88,3 +100,20 @@ def test_rotary_at_any_position(far, inter):
     out = t.rotary(x, None, torch.tensor(pos, device=DEV), w.to(DEV), interleaved=inter)
     # the fraction of a turn in fp32, half a turn at most: pi 2^-24 radians; sine and cosine 2 units each, two products and a sum
     within(out, ref, size, torch.float32, 8 * 2.0 ** -24, 'turned')
+
+
+@pytest.mark.parametrize('far', [0, 5 * 10 ** 6])
+def test_sines_and_cosines_are_exact_to_their_own_rounding(far):
+    """Unit vectors show the table itself.  Relative to each sine and cosine, also where it is close to zero: two units of the function's own (2^-22), a sum's rounding;
+    the fraction of a turn in fp32 alone would put 10^-7 radians on it, all of a cosine of that size."""
+    from srvp_amd import temporal as t
+    T, D = 256, 128
+    x = torch.zeros(T, 1, 1, D, device=DEV)
+    x[..., :D // 2] = 1
+    w, pos = t.rotary_frequencies(D), far + torch.arange(T)
+    out = t.rotary(x, None, pos.to(DEV), w.to(DEV)).double().cpu().view(T, D)
+    angles = [[exact_angle(p, f) for f in w.tolist()] for p in pos.tolist()]
+    ref = torch.tensor([[math.cos(a) for a in row] + [math.sin(a) for a in row] for row in angles], dtype=torch.float64)
+    assert ref.abs()[ref != 0].min() < 1e-4
+    bad = (out - ref).abs() / (6 * 2.0 ** -24 * ref.abs() + 2.0 ** -44)
+    assert bad.max().item() <= 1.0, bad.max().item()
