@@ -423,7 +423,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
                 for (int m = 0; m < 4; ++m)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) { const float v = acc[m][i]; s1 += v; s2 += v * v; }
+                    for (int i = 0; i < 16; ++i) { add_square(s1, s2, acc[m][i]); }
                 d1 += (double)s1; d2 += (double)s2;
             }
             if (a.ep_coef) {                                   // inference: eval-mode BatchNorm + LeakyReLU from the fp32 accumulators

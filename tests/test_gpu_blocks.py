@@ -1015,3 +1015,40 @@ def test_splitk_finish(M, C, sk, with_stats):
         assert rel_err(stats[0], r64.sum(dim=(0, 1))) < 1e-6 and rel_err(stats[1], (r64 ** 2).sum(dim=(0, 1))) < 1e-6
     else:
         assert stats.abs().max().item() == 0
+
+
+def test_conv_stream_sub64_statistics_round_squares_apart():
+    """Statistics of the sub-pixel streaming kernel: every square is rounded before it is added, as in the other convolutions, so that the last bits do not depend on
+    whether a build fuses the two.  One channel, the middle tap, a constant frame: a thread adds 64 equal values a band, which float32 arithmetic on the host repeats."""
+    import numpy as np
+    from srvp_amd import _lib as L
+    from srvp_amd.convnet import Block
+    dev = torch.device('cuda')
+    g = torch.Generator().manual_seed(3)
+    T, B = 12, 8
+    N = T * B
+    f0, f1 = make_feat(N, 32, 32, 64, dev, g), make_feat(B, 64, 64, 64, dev, g)
+    f0.interior().zero_()
+    f0.interior()[..., 0] = 1.1328125                                    # 145 / 128: bfloat16
+    sel = torch.arange(B, dtype=torch.int32, device=dev)
+    spec = dict(kind='conv', key='w', bnkey='bn', cin=128, cout=64, k=3, s=1, p=1, act='leaky_relu')
+    blk = Block(spec, 'mfma', [f0, f1], True, N, dev, True, skip_map=sel.repeat(T), skip_sel=sel)
+    blk._fwd = blk.fwd_descs()
+    w = torch.zeros(64, 128, 3, 3)
+    w[:, 0, 1, 1] = bf(torch.rand(64, generator=g) + 0.5)
+    st = L.stream()
+    blk.pack(w.to(dev), st)
+    L.call('srvp_conv_mfma', C.byref(blk._fwd[0]), st)
+    blk.stats.zero_()
+    cnt = L.load().srvp_conv_stream_count(2)
+    L.call('srvp_conv_mfma_multi', (L.ConvDesc * 4)(*blk._fwd[-4:]), 4, st)
+    torch.cuda.synchronize()
+    assert L.load().srvp_conv_stream_count(2) == cnt + 1
+    v = (np.float32(1.1328125) * w[:, 0, 1, 1].numpy()).astype(np.float32)      # (16 significant bits: exact)
+    apart, fused = np.zeros_like(v), np.zeros_like(v)
+    for _ in range(64):
+        apart = apart + v * v
+        fused = (fused.astype(np.float64) + v.astype(np.float64) ** 2).astype(np.float32)
+    assert (apart != fused).any()                                       # (the two ways differ on some of the 64 channels)
+    threads = N * 64 * 64 // 64
+    assert np.array_equal(blk.stats[1].cpu().numpy(), apart.astype(np.float64) * threads)
