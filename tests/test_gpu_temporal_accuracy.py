@@ -8,7 +8,7 @@ from decimal import Context, Decimal, localcontext
 import pytest
 import torch
 
-from test_gpu_temporal import BF, DEV, decays, rnd, scan, within
+from test_gpu_temporal import BF, DEV, decays, rnd, scan, state_sum, within
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +117,21 @@ def test_sines_and_cosines_are_exact_to_their_own_rounding(far):
     assert ref.abs()[ref != 0].min() < 1e-4
     bad = (out - ref).abs() / (6 * 2.0 ** -24 * ref.abs() + 2.0 ** -44)
     assert bad.max().item() <= 1.0, bad.max().item()
+
+
+SHORT = [(2, 2, 64, 64), (3, 3, 128, 128), (5, 2, 40, 72), (8, 2, 256, 96), (6, 2, 83, 35)]
+
+
+@pytest.mark.parametrize('T,H,Dk,Dv', SHORT)
+def test_bf16_state_and_its_gradient_have_fp32_accuracy(T, H, Dk, Dv):
+    """A few tokens, decays well below one, no state in front: every term is decay x value as three bfloat16 values (2^-24 of it), a product and a sum in fp32; the decays'
+    exponents are off by 2^-23 of themselves, at most half of a term for what still weighs.  (Two values, 2^-17, are four to six times over this bound.)"""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(T)
+    B = 3
+    q, k, v, do = rnd(g, T, B, H, Dk, dtype=BF), rnd(g, T, B, H, Dk, dtype=BF), rnd(g, T, B, H, Dv, dtype=BF), rnd(g, T, B, H, Dv, dtype=BF)
+    ld, sc = torch.linspace(-0.15, -0.8, H, device=DEV), Dk ** -0.5
+    new = t.linear_attention(q, k, v, ld, return_state=True)[1]
+    within(new, *state_sum(k, v, ld, None, None), torch.float32, (T + 16) * 2.0 ** -24, 'state')
+    ds = t.linear_attention_backward(do, q, k, v, ld, state=torch.zeros(B, H, Dk, Dv, device=DEV))[3]
+    within(ds, *state_sum(q, do, ld, None, None, scale=sc, from_end=False, off=1), torch.float32, (T + 18) * 2.0 ** -24, 'dstate')
