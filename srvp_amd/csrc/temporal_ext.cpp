@@ -82,7 +82,7 @@ Tensor whole(const char* what, const char* name, const Tensor& x) {
 Tensor decays(const char* what, const Tensor& l, int64_t H) {
     if (l.scalar_type() != at::kFloat || l.dim() != 1 || l.size(0) != H)
         value_error(std::string(what) + ": log_decay is a float32 tensor of one value a head (" + std::to_string(H) + "), got " + shape(l) + " " + dtype(l));
-    if (l.requires_grad()) value_error(std::string(what) + ": the decays are constants: log_decay must not require a gradient");
+    if (at::GradMode::is_enabled() && l.requires_grad()) value_error(std::string(what) + ": the decays are constants: log_decay must not require a gradient");
     return l.contiguous();
 }
 bool any_grad(std::initializer_list<const Tensor*> ts) {

@@ -54,7 +54,9 @@ def linear_attention(q, k, v, log_decay, *, state=None, lengths=None, scale=None
     q, k (T, B, H, Dk), v (T, B, H, Dv), heads of 1 to 256 features; log_decay (H,) float32, normally <= 0 (-inf: no memory); state (B, H, Dk, Dv)
     float32: S in front of the first token (None: zero; it is not changed); lengths (B,): tokens of each sequence (outputs behind them are zero, values
     there are not read); scale: default Dk ** -0.5.  Returns o (T, B, H, Dv), or (o, new state) with return_state.  Gradients: q, k, v, state.
-    A NaN or infinity reaches the outputs of its own token and of those behind it."""
+    A NaN or infinity reaches the outputs of its own token and of those behind it, as an infinity or as NaN (which
+    of the two is not kept apart: an infinity in v mostly comes out as NaN, in its column).
+    The decays are constants: no gradient."""
     return (_ext or load()).linear_attention(q, k, v, log_decay, state, lengths, scale, return_state)
 
 

@@ -388,3 +388,16 @@ def test_frequencies_take_no_gradient():
             t.rotary(q, None, pos, learnt)
     with torch.no_grad():
         assert torch.equal(t.rotary(x, None, pos, learnt), t.rotary(x, None, pos, w))
+
+
+def test_learnt_decays_without_recording():
+    """Decays that ask for a gradient are refused where one would be recorded, and taken as they are elsewhere."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(15)
+    x, s, ld = rnd(g, 4, 2, 3, 8), rnd(g, 2, 3, 8, 8), decays(3)
+    learnt = ld.clone().requires_grad_()
+    for f in (lambda l: t.linear_attention(x, x, x, l), lambda l: t.linear_attention_backward(x, x, x, x, l)[0], lambda l: t.linear_attention_step(x[0], x[0], x[0], l, s.clone())):
+        with pytest.raises(ValueError, match='constants'):
+            f(learnt)
+        with torch.no_grad():
+            assert torch.equal(f(learnt), f(ld))
