@@ -401,3 +401,23 @@ def test_learnt_decays_without_recording():
             f(learnt)
         with torch.no_grad():
             assert torch.equal(f(learnt), f(ld))
+
+
+def test_step_of_many_rows():
+    """Thousands of rows, slots in any order, padded ones and slots that come several times: one call is as many calls of rows of different slots."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(16)
+    B, H, D, N = 6000, 1, 16, 7000
+    q, k, v, ld = rnd(g, B, H, D), rnd(g, B, H, D), rnd(g, B, H, D), decays(H)
+    slots = torch.randperm(N, generator=g)[:B]
+    slots[5::7] = -1
+    slots[4000:4020] = slots[0:20]                        # a second token for some
+    pool = rnd(g, N, H, D, D)
+    again = pool.clone()
+    slots = slots.to(DEV)
+    o = t.linear_attention_step(q, k, v, ld, pool, slots=slots)
+    for a, b in ((0, 4000), (4000, B)):
+        assert torch.equal(o[a:b], t.linear_attention_step(q[a:b], k[a:b], v[a:b], ld, again, slots=slots[a:b]))
+    assert torch.equal(pool, again)
+    on = (slots >= 0)[:4000]
+    assert not o[:4000][~on].any() and o[:4000][on].any(-1).all()
