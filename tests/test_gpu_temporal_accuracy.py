@@ -135,3 +135,15 @@ def test_bf16_state_and_its_gradient_have_fp32_accuracy(T, H, Dk, Dv):
     within(new, *state_sum(k, v, ld, None, None), torch.float32, (T + 16) * 2.0 ** -24, 'state')
     ds = t.linear_attention_backward(do, q, k, v, ld, state=torch.zeros(B, H, Dk, Dv, device=DEV))[3]
     within(ds, *state_sum(q, do, ld, None, None, scale=sc, from_end=False, off=1), torch.float32, (T + 18) * 2.0 ** -24, 'dstate')
+
+
+def test_norm_weight_gradient_sums_in_pairs():
+    """2048 equal rows: 2048 times the gradient of one, but for the sum of four rows a workgroup holds (two roundings); everything behind it adds equal numbers in pairs,
+    which is exact.  One behind the other the workgroups' sums are several times over this."""
+    from srvp_amd import temporal as t
+    g = torch.Generator().manual_seed(17)
+    M, N = 2048, 256
+    x, w, dy = rnd(g, 1, N), rnd(g, N), rnd(g, 1, N)
+    one = t.rms_norm_backward(dy, x, w)[1].double()
+    many = t.rms_norm_backward(dy.expand(M, N), x.expand(M, N), w)[1].double()
+    assert ((many - M * one).abs() / (M * one.abs())).max().item() <= 2.25 * 2.0 ** -24
