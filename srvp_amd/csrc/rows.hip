@@ -299,19 +299,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
         if (g.res) r.load((const E*)g.res + at * g.rs, g.N, t);
     };
     if (row < g.M) fetch(row);
-    bool wild = false;                                     // whether a weight is NaN or infinite, which leaves no row finite (and `most` would pass over a NaN)
+    // the exponent of NaN if a weight of this wave's is NaN or infinite, which leaves no row finite (fmax passes over a NaN): put over the row's sum of squares
+    unsigned wild = 0;
     if constexpr (Q8 && NORM) {
         float x = 0.f;
 #pragma unroll
         for (int i = 0; i < V * VE; ++i) x += 0.f * wv[i];
-        wild = __any(!(x == 0.f));
-        if constexpr (TPR > 64) {
-            if ((tid & 63) == 0) red[tid >> 6] = wild;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < TPR / 64; ++i) wild = wild || red[i] != 0.f;
-            wild = __builtin_amdgcn_readfirstlane(wild);
-        }
+        wild = __builtin_amdgcn_readfirstlane(__any(!(x == 0.f)) ? 0x7ff80000u : 0u);
     }
     for (; row < g.M; row += step) {                       // (the same for all threads of a row, and of a workgroup whose waves meet)
         x.arrived(g.N, t);
@@ -342,9 +336,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(const N
                 if (NORM) hd[i] *= (double)wv[i];
                 most = fmax(most, fabs(hd[i]));
             }
+            if (NORM) ss = __hiloint2double(__double2hiint(ss) | wild, __double2loint(ss));
             ss = row_sum<TPR>(ss, redd, tid);
             most = row_max<TPR>(most, redd, tid);
-            const bool fine = !wild && ss < (double)INFINITY && most < (double)INFINITY;      // (false for NaN)
+            const bool fine = ss < (double)INFINITY && most < (double)INFINITY;      // (false for NaN)
             const double to = fine && most > 0 ? 127.0 / most : 0.0;
             if (t == 0) g.scale[row] = fine ? (float)(most * (NORM ? 1.0 / sqrt(ss / g.N + (double)g.eps) : 1.0) / 127.0) : NAN;
             signed char* q = g.q + row * g.qs;
