@@ -27,6 +27,13 @@ def _empty(like, *shape):
     return torch.empty(*shape, dtype=torch.float32, device=like.device)
 
 
+def _taken(x):
+    """x, if the products can take it: float32, one row behind the other."""
+    if x.dtype is not torch.float32 or not x.is_contiguous():
+        raise TypeError(f'posterior attention: contiguous float32 encodings and weights, got {x.dtype} {tuple(x.shape)} with strides {x.stride()}')
+    return x
+
+
 class _Scale(nn.Module):
     """Parameter container of a row norm."""
 
@@ -96,17 +103,17 @@ class AttentionPosterior(nn.Module):
     # ---- the block
     def _project(self, x, weight, out):
         from .latent import linear_fwd
-        return linear_fwd(L.stream(), x, weight, None, out)
+        return linear_fwd(L.stream(), x, _taken(weight), None, out)
 
     def _inputs(self, hx, q8):
         """hx (rows, nhx), contiguous -> u, norm(u) (None in 8 bits), (rows, 3 nh)."""
         from .latent import linear_fwd
-        if hx.shape[-1] != self.inp.weight.shape[1] or hx.device != self.inp.weight.device:
-            raise ValueError(f'posterior attention: encodings of {self.inp.weight.shape[1]} features on {self.inp.weight.device}, got {tuple(hx.shape)} on {hx.device}')
-        if any(x.dtype is not torch.float32 for x in (hx, self.inp.weight, self.qkv.weight, self.out.weight)):
-            raise TypeError(f'posterior attention: float32 encodings and weights, got {hx.dtype} and {self.inp.weight.dtype}, {self.qkv.weight.dtype}, {self.out.weight.dtype}')
+        inp = self.inp
+        w = _taken(inp.weight)
+        if hx.shape[-1] != w.shape[1] or hx.device != w.device:
+            raise ValueError(f'posterior attention: encodings of {w.shape[1]} features on {w.device}, got {tuple(hx.shape)} on {hx.device}')
         u = _empty(hx, hx.shape[0], self.heads * self.width)
-        linear_fwd(L.stream(), hx, self.inp.weight, self.inp.bias, u)
+        linear_fwd(L.stream(), _taken(hx), w, inp.bias, u)
         if q8 is not None:
             return u, None, temporal.linear_int8(*temporal.rms_norm_int8(u, self.norm.weight), *q8[0])
         n = temporal.rms_norm(u, self.norm.weight)

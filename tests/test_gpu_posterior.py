@@ -308,3 +308,9 @@ def test_encodings_of_any_strides():
             net.run(bad, False)
     with pytest.raises(TypeError):
         AttentionPosterior(16, 24, 2).cuda().double().run(wide[..., :16], False)
+    for name in ('inp', 'qkv', 'out'):
+        net = AttentionPosterior(16, 24, 2).cuda()
+        w = getattr(net, name).weight
+        w.data = w.data.t().contiguous().t()              # (another order in memory)
+        with pytest.raises(TypeError):
+            net.run(wide[..., :16], False)
