@@ -218,7 +218,7 @@ __device__ __forceinline__ void put4(float* p, const f32x4_t& v) { *reinterpret_
 // condition (a load under a branch makes the compiler wait for every load in flight where the paths meet, three memory latencies a chunk) and one address
 // register.  Otherwise (rows at other borders than 16 bytes, features not in eights) 16 bytes from any address: rows behind the last are the last again, the
 // last vector of a row ends with the row, and both are put right on the way into LDS.  Fewer features than a vector: one by one, in `store`.
-// 512 x 32, 16 heads of 127 x 127, forward / backward: 94 / 264 us (element by element 333 / 1160); of 128 x 128 through the same code's VEC form 59 / 153.
+// 512 x 32, 16 heads of 127 x 127, forward / backward: 95 / 266 us (element by element 333 / 1160); of 128 x 128 through the same code's VEC form 66 / 165.
 constexpr unsigned OUTSIDE = 0x80000000u;      // an offset behind every bound: a chunk is at most 2^30 bytes (see operand())
 template <class E, int W, bool VEC> struct Tile {
     using V = View<E, W>;
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256, DA > 128 ? 1 : DA > 64 || (sizeof(E) == 2 && O
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lg = lane >> 4, ls = lane & 15;
     // what reads the same tokens (roles, column blocks) follows one another on one XCD, whose L2 (or the memory-side cache, for the role that walks the other
-    // way) then holds them: workgroups go round the 8 XCDs (backward, 512 x 32 x 16 x 128: 179 us; one role behind the other: 184)
+    // way) then holds them: workgroups go round the 8 XCDs (backward, 512 x 32 x 16 x 128, an earlier kernel: 179 us; one role behind the other: 184)
     int id = blockIdx.x / 8;
     const int cb = id % g.ncb; id /= g.ncb;
     const int ro = id % g.nroles;
@@ -858,7 +858,7 @@ void launch(const ScanArgs& base, const Role* roles, int n, bool out, bool exact
 
 // Segments: with fewer (sequence, head) pairs than the chip has room for (two workgroups on each of 256 CUs), a sequence is cut into as many segments as fill
 // it, of four chunks or more, walked side by side.  That costs the segments' own sums first and a pass over them, so three segments are the least.  bfloat16, us,
-// whole and cut (pairs x roles; forward unless said):
+// whole and cut (pairs x roles; forward unless said; both sides of an earlier kernel, now 5 to 10 % longer):
 //   192, 1024 tokens: 65 and 110 (2 segments)      210, 4096 tokens, backward: 224 and 283 (2)      256, 2048 tokens: 160 and 271 (2)
 //   128, 2048 tokens: 122 and 129 (4); 8192 tokens: 481 and 416; float32, 64 features: 145 and 96      144, 4096 tokens, backward: 220 and 202 (3)
 // Twice as many segments: 8192 x 2 x 16 x 128 115 -> 144, 4096 x 3 x 12 x 128 77 -> 94; half as many: 141 -> 147 (an earlier kernel).

@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs g) {
 // quotient are formed in 64 bits, so q does not depend on the order of any sum.  A row of zeros has scale 0; a row of y with an infinity or NaN (its own, or the
 // weight's) has scale NaN and q = 0, i.e. stands for NaN.
 // TPR threads hold one row in registers: V vectors of VE elements each.
-// Measured (us): 16384 x 4096 bfloat16 with a residual forward 89 = 6.0 TB/s, backward 141 + 5 for dw = 4.8 TB/s; 2304 x 256 float32 3.8, 5.5 + 3.6 (launches);
+// Measured (us): 16384 x 4096 bfloat16 with a residual forward 84 to 89 = 6.0 TB/s, backward 143 + 5 for dw = 4.7 TB/s; 2304 x 256 float32 3.8, 5.5 + 3.6 (launches);
 // 8-bit output 7 x 4096 5.  Rows that are not whole vectors at borders of 16 bytes take the same vectors from any address (one element a load, a value's
 // neighbours in the next threads: 16384 x 4095 forward 177, backward 436, 8-bit 246 us, now 125, 172, 134; 16384 x 4096 100, 130, 91).
 struct NormArgs {
@@ -538,7 +538,7 @@ extern "C" int srvp_rotary(const srvp_rotary_desc* d, void* stream) {
     g.T = d->T; g.B = d->B; g.H0 = d->Hq; g.H1 = d->Hk; g.D = d->D; g.n = d->pairs; g.inter = d->interleaved;
     g.sign = d->back ? -1.f : 1.f; g.mult = d->magnitude;
     // rows a workgroup: one sine and cosine a thread, at most 64 KB (16 items a thread).  2048 x 4, 16 + 16 heads of 128, bfloat16, us, half and all of it turned: 22.8 and 21.1
-    // (5.9, 6.4 TB/s; tensors of 34 MB, partly from cache); 16 KB 25.7, 21.7; one row 33.6, 38.7; two sines a thread 25.3, 22.2; four 25.3, 24.5 (but 4096 x 3, 2 + 2
+    // (5.9, 6.4 TB/s; tensors of 34 MB, partly from cache: half of it turned from memory 26); 16 KB 25.7, 21.7; one row 33.6, 38.7; two sines a thread 25.3, 22.2; four 25.3, 24.5 (but 4096 x 3, 2 + 2
     // heads of 256, where the sines are the cost: 22, two 20, four 15)
     const int n = d->pairs > 0 ? d->pairs : 1, H = d->Hq + d->Hk;
     long long R = (256 + n - 1) / n, most = 65536LL / ((long long)H * d->D * e) + 1;
