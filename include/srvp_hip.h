@@ -583,7 +583,7 @@ typedef struct {
     const float* d_state_out; float* d_state_in;
 } srvp_linear_attention_bwd_desc;
 /* one token for each of B rows: q, k, v, o (B, H, D) with strides over b, h; state float32 [nslots][H][Dk][Dv], updated in place; slots (int64 [B],
- * may be NULL: row b has state b).  A slot outside [0, nslots) marks a padded row (output zero, no state touched); rows that name the same slot are
+ * may be NULL: row b has state b; otherwise B <= 65536).  A slot outside [0, nslots) marks a padded row (output zero, no state touched); rows that name the same slot are
  * successive tokens of one sequence, in row order. */
 typedef struct {
     const void *q, *k, *v; void* o;

@@ -1011,6 +1011,8 @@ extern "C" int srvp_linear_attention_step(const srvp_linear_attention_step_desc*
     SRVP_REQUIRE(d->Dk >= 1 && d->Dk <= 256 && d->Dv >= 1 && d->Dv <= 256, "srvp_linear_attention_step: heads of 1 to 256 features (got %d, %d)", d->Dk, d->Dv);
     if (d->B == 0 || d->H == 0) return SRVP_OK;
     SRVP_REQUIRE(d->q && d->k && d->v && d->o && d->log_decay && (d->state || d->nslots == 0), "srvp_linear_attention_step: null pointer");
+    // (every workgroup looks through all slots: the search grows with the square of the rows, 65536 of them read 34 GB of slots a head)
+    SRVP_REQUIRE(!d->slots || d->B <= 65536, "srvp_linear_attention_step: at most 65536 rows with slots, got %d", d->B);
     SRVP_REQUIRE(d->slots || d->B <= d->nslots, "srvp_linear_attention_step: %d rows for %d states", d->B, d->nslots);
     SRVP_REQUIRE((uintptr_t)d->state % 16 == 0, "srvp_linear_attention_step: state must be 16-byte aligned");
     StepArgs g;

@@ -271,6 +271,7 @@ Tensor linear_attention_step(const Tensor& q0, const Tensor& k0, const Tensor& v
                     std::to_string(Dv) + "), got " + shape(state) + " " + dtype(state));
     Tensor sl;
     if (slots) {
+        if (B > 65536) value_error(std::string(what) + ": at most 65536 rows with slots, got " + std::to_string(B));
         if (slots->dim() != 1 || slots->size(0) != B) value_error(std::string(what) + ": one slot a row (" + std::to_string(B) + "), got " + shape(*slots));
         sl = whole(what, "slots", *slots).contiguous();
     } else if (B > state.size(0)) {

@@ -68,7 +68,7 @@ def linear_attention_backward(d_out, q, k, v, log_decay, *, state=None, lengths=
 
 def linear_attention_step(q, k, v, log_decay, state, *, slots=None, scale=None):
     """One token of each of B sequences: q, k (B, H, Dk), v (B, H, Dv) -> o (B, H, Dv); state (slots, H, Dk, Dv) float32, contiguous, is advanced in place.
-    slots (B,): where each row's state lies (None: row b has state b).  A slot outside the pool marks a padded row: its output is zero, no state is
+    slots (B,): where each row's state lies (None: row b has state b), for at most 65536 rows.  A slot outside the pool marks a padded row: its output is zero, no state is
     touched.  Rows that name the same slot are successive tokens of one sequence, in row order."""
     return (_ext or load()).linear_attention_step(q, k, v, log_decay, state, slots, scale)
 

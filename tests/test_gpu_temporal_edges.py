@@ -421,3 +421,12 @@ def test_step_of_many_rows():
     assert torch.equal(pool, again)
     on = (slots >= 0)[:4000]
     assert not o[:4000][~on].any() and o[:4000][on].any(-1).all()
+
+
+def test_rows_with_slots_have_a_bound():
+    from srvp_amd import temporal as t
+    x, st, slots = torch.zeros(65537, 1, 1, device=DEV), torch.zeros(65537, 1, 1, 1, device=DEV), torch.arange(65537, device=DEV)
+    with pytest.raises(ValueError, match='65536 rows'):
+        t.linear_attention_step(x, x, x, decays(1), st, slots=slots)
+    assert t.linear_attention_step(x, x, x, decays(1), st).shape == x.shape          # (without a search)
+    assert t.linear_attention_step(x[1:], x[1:], x[1:], decays(1), st, slots=slots[1:]).shape == (65536, 1, 1)

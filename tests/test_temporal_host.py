@@ -199,3 +199,10 @@ def test_posterior_constants_keep_their_types():
         far = AttentionPosterior(8, 24, 3)
     far.to_empty(device='cpu')
     assert torch.equal(far.log_decay, ld) and torch.equal(far.frequencies, fr)
+
+
+def test_step_refuses_rows_without_bound():
+    """The search through the slots grows with the square of the rows: where it would hold the GPU for minutes the call is refused, on the host."""
+    one = dict(q=16, k=16, v=16, o=16, log_decay=16, state=16, slots=16, H=1, Dk=8, Dv=8, nslots=2 ** 24, scale=1.0)
+    for B in (65537, 2 ** 23):
+        assert L.load().srvp_linear_attention_step(C.byref(L.LinearAttentionStepDesc(**dict(one, B=B))), None) == 1 and b'65536 rows' in L.load().srvp_last_error()
