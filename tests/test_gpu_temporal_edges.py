@@ -430,3 +430,31 @@ def test_rows_with_slots_have_a_bound():
         t.linear_attention_step(x, x, x, decays(1), st, slots=slots)
     assert t.linear_attention_step(x, x, x, decays(1), st).shape == x.shape          # (without a search)
     assert t.linear_attention_step(x[1:], x[1:], x[1:], decays(1), st, slots=slots[1:]).shape == (65536, 1, 1)
+
+
+@pytest.mark.parametrize('T,B,lengths', [(0, 2, None), (1, 2, None), (90, 2, [0, 90]), (700, 1, None), (700, 1, [0]), (700, 1, [300])])
+@pytest.mark.parametrize('dt', [BF, FP])
+def test_state_gradients_at_the_ends_of_sequences(T, B, lengths, dt):
+    """No tokens, one, none in a sequence of several, segments behind the last token; with and without a gradient of the new state; eager, and captured and replayed."""
+    from srvp_amd import temporal as t
+    from test_gpu_temporal import state_sum
+    g = torch.Generator().manual_seed(T + B)
+    H, Dk, Dv = 2, 64, 40
+    q, k, v, do = rnd(g, T, B, H, Dk, dtype=dt), rnd(g, T, B, H, Dk, dtype=dt), rnd(g, T, B, H, Dv, dtype=dt), rnd(g, T, B, H, Dv, dtype=dt)
+    s0, dn, ld, sc = rnd(g, B, H, Dk, Dv), rnd(g, B, H, Dk, Dv), decays(H), Dk ** -0.5
+    n = None if lengths is None else torch.tensor(lengths, device=DEV)
+    for d in (dn, None):
+        call = lambda: t.linear_attention_backward(do, q, k, v, ld, state=s0, lengths=n, d_state=d)
+        eager = call()
+        ref, size = state_sum(q, do, ld, lengths, d, scale=sc, from_end=False, off=1)
+        within(eager[3], ref, size, FP, (T + 64) * 2.0 ** -24, 'dstate')
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        for i in range(3):
+            for x in (q, do) if T else ():
+                x.copy_(rnd(g, *x.shape, dtype=dt))
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, call()):
+                assert torch.equal(a, b), i
