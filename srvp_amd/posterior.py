@@ -169,8 +169,9 @@ class AttentionPosterior(nn.Module):
         linear_bwd(st, n, self.qkv.weight, d_qkv, grads[f'{prefix}.qkv.weight'], None, dx=d_n, defer=defer)
         d_u, dw = temporal.rms_norm_backward(d_n, u, self.norm.weight, d_sum=d_zu)
         add('norm', dw)
-        linear_bwd(st, hx.reshape(R, -1).contiguous(), self.inp.weight, d_u, grads[f'{prefix}.inp.weight'], grads[f'{prefix}.inp.bias'], dx=d_hx, dx_acc=1, defer=defer)
-        return d_zu, d_qkv, d_u, saved
+        x = hx.reshape(R, -1).contiguous()
+        linear_bwd(st, x, self.inp.weight, d_u, grads[f'{prefix}.inp.weight'], grads[f'{prefix}.inp.bias'], dx=d_hx, dx_acc=1, defer=defer)
+        return x, d_zu, d_qkv, d_u, saved
 
 
 class PosteriorStream:

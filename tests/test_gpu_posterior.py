@@ -296,7 +296,15 @@ def test_encodings_of_any_strides():
             hz, saved = net.run(x, True)
             grads = {f'inf_z.{k}': torch.zeros_like(p) for k, p in net.named_parameters()}
             d_hx = torch.zeros(21, 16, device='cuda')
-            keep = net.backward(x, dy, saved, grads, 'inf_z', d_hx)
+            later = []
+            keep = net.backward(x, dy, saved, grads, 'inf_z', d_hx, defer=later)
+            assert any(torch.is_tensor(a) and a.shape == (21, 16) and torch.equal(a, copy.view(21, 16)) for a in keep)      # (a slice's copy lives until the deferred launches end)
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for f in later:
+                    f(side.cuda_stream)
+            del later
             torch.cuda.synchronize()
             results.append([hz, d_hx] + list(grads.values()))
             del keep
